@@ -616,6 +616,65 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
                        int32_t s_max, float scale, int32_t n_split, void *ws, size_t ws_bytes, void *out,
                        void *stream);
 
+/*
+ * A key/value cache in 8-bit floating point, and decode attention over it and over a
+ * prefix that the whole batch shares.  (No counterpart in the reference: its cache is
+ * the Transformers one, in the model dtype, one copy of every position per sequence.)
+ *
+ * Quantised cache: codes_k [B,n_kv,s_max,dk] and codes_v [B,n_kv,s_max,dv] e4m3 bytes,
+ * scale_k / scale_v [B,n_kv,s_max] bytes.  A row (one sequence, head and position) stands
+ * for code * 2^(scale - 127), scale byte 255 for NaN throughout; the writer takes the least
+ * power of two, 2^-127 or more, by which the row's largest magnitude is at most 448 (codes
+ * then stop at 240 where 256 would stand for 2^128), and byte 255 with zero codes for a row that holds an infinity or a NaN.  All codes and bf16
+ * caches must be 16-byte aligned.
+ *
+ * sb_rope_append_fp8  rotates the first rope_dim elements of every q and k head (pairs
+ *                  (i, i + rope_dim/2), angle pos * theta^(-2i/rope_dim)), stores q to
+ *                  q_out [T,n_q,dk] bf16 (q itself is not written) and quantises k and v
+ *                  into row (seq_of_token[t], pos_of_token[t]).  Angles, products and the
+ *                  scaled row are fp32, a value is rounded once; angles are those of the
+ *                  64-bit formula for positions up to 2^24.  A key head's first rope_dim
+ *                  elements come from k_rot and the others from k_rest (NULL where there
+ *                  are none).  strides: eight int64 (host), the elements between tokens
+ *                  and between heads of q, k_rot, k_rest, v; a head stride of 0 shares one
+ *                  row between the heads.  A token whose sequence is outside [0,B) or whose
+ *                  position is outside [0,s_max) stores nothing but its q; two tokens of one
+ *                  call must not name the same row.  dk, dv: multiples of 16 up to 256,
+ *                  rope_dim a multiple of 16 up to dk.
+ * sb_cache_read_fp8   positions begin .. begin+count-1 of every sequence as bf16, out_k
+ *                  [B,n_kv,count,dk], out_v [B,n_kv,count,dv]; exact (a code has four
+ *                  significant bits).  Positions below shared_len come from sequence 0.
+ * sb_attn_decode_fp8  one query per sequence, q [B,n_q,dk] bf16 (q_stride elements between
+ *                  sequences, 0 = packed), against the first seq_lens[b] (device int32)
+ *                  positions of its quantised cache; softmax in fp32; out [B,n_q,dv] bf16,
+ *                  zeros for a sequence without positions.  Query head h reads key head
+ *                  h / (n_q / n_kv).  With shared_len > 0 positions below it are read from
+ *                  sequence 0's rows, once for all sequences that are longer than it.  ws:
+ *                  sb_attn_cached_workspace_bytes(), 16-byte aligned, not shared by calls
+ *                  that may overlap on the GPU.  status: device int32 (may be NULL), set
+ *                  non-zero if a bounded wait gave up.  (dk,dv) = (128,128), (192,128),
+ *                  (64,64).
+ * sb_attn_decode_shared  the same over a bf16 cache, cache_k [B,s_max,n_kv,dk], cache_v
+ *                  [B,s_max,n_kv,dv].
+ */
+int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest, const void *v,
+                           const int32_t *seq_of_token, const int32_t *pos_of_token, int32_t T, int32_t B, int32_t n_q,
+                           int32_t n_kv, int32_t dk, int32_t dv, int32_t rope_dim, float theta, int32_t s_max,
+                           const int64_t *strides, void *q_out, void *codes_k, void *scale_k, void *codes_v,
+                           void *scale_v, void *stream);
+int32_t sb_cache_read_fp8(const void *codes_k, const void *scale_k, const void *codes_v, const void *scale_v, int32_t B,
+                          int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max, int32_t begin, int32_t count,
+                          int32_t shared_len, void *out_k, void *out_v, void *stream);
+size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t dv, int32_t s_max, int32_t shared_len);
+int32_t sb_attn_decode_fp8(const void *q, int64_t q_stride, const void *codes_k, const void *scale_k, const void *codes_v,
+                           const void *scale_v, const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk,
+                           int32_t dv, int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
+                           int32_t *status, void *stream);
+int32_t sb_attn_decode_shared(const void *q, int64_t q_stride, const void *cache_k, const void *cache_v,
+                              const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk, int32_t dv,
+                              int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
+                              int32_t *status, void *stream);
+
 /* Number of kernels the last sb_moe_layer_forward of this thread launched. */
 int32_t sb_last_launch_count(void);
 

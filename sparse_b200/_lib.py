@@ -21,7 +21,7 @@ SB_COPY_PEER_TO_DEVICE = 1
 SB_COPY_DEVICE_LOCAL = 2
 SB_TILE_M = 128
 
-i32, vp, sz = C.c_int32, C.c_void_p, C.c_size_t
+i32, i64, vp, sz = C.c_int32, C.c_int64, C.c_void_p, C.c_size_t
 
 
 class MoeLayer(C.Structure):
@@ -100,6 +100,13 @@ SIGNATURES: Dict[str, Tuple[object, list]] = {
                                  vp]),
     "sb_attn_decode_workspace_bytes": (sz, [i32, i32, i32, i32]),
     "sb_attn_decode": (i32, [vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, C.c_float, i32, vp, sz, vp, vp]),
+    "sb_rope_append_fp8": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, i32,
+                                 C.POINTER(i64), vp, vp, vp, vp, vp, vp]),
+    "sb_cache_read_fp8": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
+    "sb_attn_cached_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+    "sb_attn_decode_fp8": (i32, [vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, sz, vp, vp,
+                                 vp]),
+    "sb_attn_decode_shared": (i32, [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, sz, vp, vp, vp]),
     "sb_moe_layer_struct_bytes": (sz, []),
     "sb_moe_layer_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
     "sb_moe_layer_forward": (i32, [C.POINTER(MoeLayer), vp, vp]),

@@ -1,0 +1,280 @@
+// The quantised key/value cache: rotary embedding with the rows quantised as they are
+// written, and reading positions back as bf16.  Row format: kv_fp8.cuh.
+//
+// Both kernels move bytes.  The append reads q, k and v once (bf16) and writes q once
+// (bf16) and half the bytes of k and v; the read-back reads one byte and writes two per
+// value.
+//
+// The bf16 cache's append (model_ops.cu) rounds cos, sin and both products to bf16, as
+// the model classes it stands for do.  Here angles and products stay in fp32 and a value is
+// rounded once, to its code or to the bf16 query: an 8-bit code has no bits to spare for
+// three earlier roundings.
+#include <math.h>
+
+#include "kv_fp8.cuh"
+
+namespace sb {
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kMaxHead = 256;                    // a row is at most one warp of 8-value vectors
+constexpr int kMaxHalf = kMaxHead / 2;
+
+// theta^(-2j / rope_dim) / (2 pi), turns per position, as the sum of two floats
+struct RopeFreq { float2 turns[kMaxHalf]; };
+
+// rows of token t, head h at base + t * token + h * head
+struct RowSource {
+  const __nv_bfloat16 *base;
+  int64_t token, head;
+  __device__ __forceinline__ const __nv_bfloat16 *at(int t, int h) const { return base + t * token + h * head; }
+};
+
+template <bool VEC>
+__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8]) {
+  if constexpr (VEC) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = bf16_lo(w[i]); x[2 * i + 1] = bf16_hi(w[i]); }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __bfloat162float(p[i]);
+  }
+}
+
+// Values e .. e+7 of a row whose first `rope` values are rotated: a vector of the first
+// half needs its partner of the second half and the other way round.
+template <bool VEC>
+__device__ __forceinline__ void load_rotated(const __nv_bfloat16 *rot, int e, int half, const float2 *table,
+                                             float (&x)[8]) {
+  float y[8];
+  const bool first = e < half;
+  const int j = first ? e : e - half;
+  load8<VEC>(rot + e, x);
+  load8<VEC>(rot + (first ? e + half : j), y);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 cs = table[j + i];
+    x[i] = first ? x[i] * cs.x - y[i] * cs.y : x[i] * cs.x + y[i] * cs.y;
+  }
+}
+
+// One row per group of L lanes, eight values a lane: codes and scale byte of the row.
+template <int L>
+__device__ __forceinline__ void store_codes(float (&x)[8], int e, int d, uint8_t *codes, uint8_t *scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int off = L / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const uint32_t byte = e8m0_of_amax(top);
+  const float inv = e8m0_inverse(byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= inv;
+  if (byte == kScaleTop) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -kCodeTop), kCodeTop);
+  }
+  uint2 c = make_uint2(0, 0);
+  if (byte != kScaleNan) c = make_uint2(e4m3x4(x[0], x[1], x[2], x[3]), e4m3x4(x[4], x[5], x[6], x[7]));
+  if (e < d && codes != nullptr) {
+    *reinterpret_cast<uint2 *>(codes + e) = c;
+    if (e == 0) *scale = (uint8_t)byte;
+  }
+}
+
+// grid = (tokens, shares of a token's rows).  A token's angles are worked out once per CTA:
+// turns = pos * frequency as a product of three floats without error in its fraction, so
+// positions far into a long context have the angle of the 64-bit formula to fp32's last bits.
+template <int L, bool VEC>
+__global__ void __launch_bounds__(kAppendThreads)
+rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource v, __nv_bfloat16 *__restrict__ q_out,
+                       const int32_t *__restrict__ seq_of_token, const int32_t *__restrict__ pos_of_token, int B,
+                       int n_q, int n_kv, int dk, int dv, int rope, int s_max, uint8_t *__restrict__ codes_k,
+                       uint8_t *__restrict__ scale_k, uint8_t *__restrict__ codes_v, uint8_t *__restrict__ scale_v,
+                       const __grid_constant__ RopeFreq freq) {
+  __shared__ float2 table[kMaxHalf];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int t = blockIdx.x;
+  const int pos = pos_of_token[t], seq = seq_of_token[t];
+  const int half = rope >> 1;
+  if (threadIdx.x < half) {
+    const float p = (float)pos, hi = freq.turns[threadIdx.x].x, lo = freq.turns[threadIdx.x].y;
+    const float a = p * hi;
+    const float turn = (a - rintf(a)) + (fmaf(p, hi, -a) + p * lo);
+    float sn, cs;
+    sincospif(2.f * turn, &sn, &cs);
+    table[threadIdx.x] = make_float2(cs, sn);
+  }
+  __syncthreads();
+  const bool cached = pos >= 0 && pos < s_max && seq >= 0 && seq < B;
+  const int rows = n_q + (cached ? 2 * n_kv : 0);
+  const int e = (threadIdx.x % L) * 8;
+  constexpr int kRows = kAppendThreads / L;              // rows of a CTA in one turn
+  // (all lanes of a warp take the same turns: the scale's reduction shuffles across a row)
+  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
+    const int r = r0 + threadIdx.x / L;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    uint8_t *codes = nullptr, *scale = nullptr;
+    int d = dk;
+    if (r < n_q) {
+      if (e < rope) load_rotated<VEC>(q.at(t, r), e, half, table, x);
+      else if (e < dk) load8<VEC>(q.at(t, r) + e, x);
+      if (e < dk) {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        *reinterpret_cast<uint4 *>(q_out + ((size_t)t * n_q + r) * dk + e) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    } else if (r < rows) {
+      const int h = r - n_q < n_kv ? r - n_q : r - n_q - n_kv;
+      const size_t row = ((size_t)seq * n_kv + h) * s_max + pos;
+      if (r - n_q < n_kv) {
+        if (e < rope) load_rotated<VEC>(k_rot.at(t, h), e, half, table, x);
+        else if (e < dk) load8<VEC>(k_rest.at(t, h) + (e - rope), x);
+        codes = codes_k + row * dk;
+        scale = scale_k + row;
+      } else {
+        d = dv;
+        if (e < dv) load8<VEC>(v.at(t, h) + e, x);
+        codes = codes_v + row * dv;
+        scale = scale_v + row;
+      }
+    }
+    if (r0 + kRows > n_q) store_codes<L>(x, e, d, codes, scale);      // (the same for the whole CTA)
+  }
+}
+
+template <int L>
+int32_t launch_append(bool vec, dim3 grid, cudaStream_t st, RowSource q, RowSource k_rot, RowSource k_rest, RowSource v,
+                      void *q_out, const int32_t *seq, const int32_t *pos, int B, int n_q, int n_kv, int dk, int dv,
+                      int rope, int s_max, void *ck, void *sk, void *cv, void *sv, const RopeFreq &freq) {
+  auto kern = vec ? rope_append_fp8_kernel<L, true> : rope_append_fp8_kernel<L, false>;
+  SB_CUDA_CHECK(launch_pdl(kern, grid, dim3(kAppendThreads), 0, st, q, k_rot, k_rest, v,
+                           static_cast<__nv_bfloat16 *>(q_out), seq, pos, B, n_q, n_kv, dk, dv, rope, s_max,
+                           static_cast<uint8_t *>(ck), static_cast<uint8_t *>(sk), static_cast<uint8_t *>(cv),
+                           static_cast<uint8_t *>(sv), freq));
+  SB_LAUNCH_CHECK();
+  return SB_OK;
+}
+
+// grid = (shares of the positions, heads, sequences).  A position of a head is dk/16 + dv/16 vectors of
+// sixteen codes; a thread keeps its place in the row and walks over positions.
+constexpr int kReadThreads = 256;
+__global__ void __launch_bounds__(kReadThreads)
+cache_read_fp8_kernel(const uint8_t *__restrict__ codes_k, const uint8_t *__restrict__ scale_k,
+                      const uint8_t *__restrict__ codes_v, const uint8_t *__restrict__ scale_v, int n_kv, int dk, int dv,
+                      int s_max, int begin, int count, int shared_len, __nv_bfloat16 *__restrict__ out_k,
+                      __nv_bfloat16 *__restrict__ out_v) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int per_row = (dk + dv) >> 4;
+  const int lane = threadIdx.x % per_row, step = kReadThreads / per_row;
+  const int first = threadIdx.x / per_row;
+  if (first >= step) return;                              // (threads left over where per_row does not divide the CTA)
+  const int h = blockIdx.y, b = blockIdx.z;
+  const bool key = lane < (dk >> 4);
+  const int d = key ? dk : dv, e = (key ? lane : lane - (dk >> 4)) * 16;
+  const uint8_t *codes = key ? codes_k : codes_v, *scales = key ? scale_k : scale_v;
+  __nv_bfloat16 *dst = (key ? out_k : out_v) + ((size_t)b * n_kv + h) * count * d + e;
+  for (int i = blockIdx.x * step + first; i < count; i += gridDim.x * step) {
+    const int pos = begin + i;
+    const size_t row = ((size_t)(pos < shared_len ? 0 : b) * n_kv + h) * s_max + pos;
+    const uint4 c = __ldg(reinterpret_cast<const uint4 *>(codes + row * d + e));
+    const float scale = e8m0_value(__ldg(scales + row));
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    uint32_t o[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 lo = f16x2_to_float2(e4m3x2_to_f16x2(w[k])), hi = f16x2_to_float2(e4m3x2_to_f16x2(w[k] >> 16));
+      o[2 * k] = pack_bf16x2(lo.x * scale, lo.y * scale);
+      o[2 * k + 1] = pack_bf16x2(hi.x * scale, hi.y * scale);
+    }
+    uint4 *p = reinterpret_cast<uint4 *>(dst + (size_t)i * d);
+    p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+bool head_ok(int d) { return d >= 16 && d <= kMaxHead && d % 16 == 0; }
+
+}  // namespace
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" {
+
+int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest, const void *v,
+                           const int32_t *seq_of_token, const int32_t *pos_of_token, int32_t T, int32_t B, int32_t n_q,
+                           int32_t n_kv, int32_t dk, int32_t dv, int32_t rope_dim, float theta, int32_t s_max,
+                           const int64_t *strides, void *q_out, void *codes_k, void *scale_k, void *codes_v,
+                           void *scale_v, void *stream) {
+  if (T < 0 || B < 1 || n_q < 1 || n_kv < 1 || n_q > 65536 || n_kv > 65536 || s_max < 1 || !head_ok(dk) || !head_ok(dv) ||
+      rope_dim < 0 || rope_dim > dk || rope_dim % 16 != 0 || !(theta > 0.f) || !isfinite(theta))
+    return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: bad shape (T=%d B=%d heads %d/%d widths %d/%d rope %d s_max=%d)", T,
+                B, n_q, n_kv, dk, dv, rope_dim, s_max);
+  if (T == 0) return SB_OK;
+  if (!q || (rope_dim > 0 && !k_rot) || (rope_dim < dk && !k_rest) || !v || !seq_of_token || !pos_of_token || !strides ||
+      !q_out || !codes_k || !scale_k || !codes_v || !scale_v)
+    return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: null pointer");
+  if (!aligned(q_out, 16) || !aligned(codes_k, 16) || !aligned(codes_v, 16))
+    return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: q_out and the codes must be 16-byte aligned");
+  const void *base[4] = {q, k_rot, k_rest, v};
+  RowSource src[4];
+  bool vec = true;
+  for (int i = 0; i < 4; ++i) {
+    src[i] = RowSource{static_cast<const __nv_bfloat16 *>(base[i]), strides[2 * i], strides[2 * i + 1]};
+    vec = vec && aligned(base[i], 16) && strides[2 * i] % 8 == 0 && strides[2 * i + 1] % 8 == 0;
+  }
+  RopeFreq freq = {};
+  for (int j = 0; j < rope_dim / 2; ++j) {
+    const double turns = exp(-2.0 * j / rope_dim * log((double)theta)) / (2.0 * M_PI);
+    freq.turns[j].x = (float)turns;
+    freq.turns[j].y = (float)(turns - (double)freq.turns[j].x);
+  }
+  const int widest = dk > dv ? dk : dv;
+  const int lanes = widest <= 64 ? 8 : widest <= 128 ? 16 : 32;
+  // at most two waves of CTAs: more would only repeat the angle table
+  const int sms = sb_device_sm_count() > 0 ? sb_device_sm_count() : 148;
+  const int wanted = ((n_q + 2 * n_kv) * lanes + kAppendThreads - 1) / kAppendThreads;
+  const int room = (int)((2ll * sms + T - 1) / T);
+  const dim3 grid(T, wanted < room ? wanted : room);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto launch = lanes == 8 ? launch_append<8> : lanes == 16 ? launch_append<16> : launch_append<32>;
+  return launch(vec, grid, st, src[0], src[1], src[2], src[3], q_out, seq_of_token, pos_of_token, B, n_q, n_kv, dk, dv,
+                rope_dim, s_max, codes_k, scale_k, codes_v, scale_v, freq);
+}
+
+int32_t sb_cache_read_fp8(const void *codes_k, const void *scale_k, const void *codes_v, const void *scale_v, int32_t B,
+                          int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max, int32_t begin, int32_t count,
+                          int32_t shared_len, void *out_k, void *out_v, void *stream) {
+  if (B < 0 || B > 65535 || n_kv < 1 || n_kv > 65535 || !head_ok(dk) || !head_ok(dv) || s_max < 1 || begin < 0 ||
+      count < 0 || count > s_max - begin || shared_len < 0 || shared_len > s_max)
+    return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: bad shape (B=%d n_kv=%d widths %d/%d positions %d+%d of %d, shared %d)",
+                B, n_kv, dk, dv, begin, count, s_max, shared_len);
+  if (B == 0 || count == 0) return SB_OK;
+  if (!codes_k || !scale_k || !codes_v || !scale_v || !out_k || !out_v)
+    return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: null pointer");
+  if (!aligned(codes_k, 16) || !aligned(codes_v, 16) || !aligned(out_k, 16) || !aligned(out_v, 16))
+    return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: codes and outputs must be 16-byte aligned");
+  const int step = kReadThreads / ((dk + dv) >> 4);
+  const int wanted = (count + step - 1) / step;
+  const int sms = sb_device_sm_count() > 0 ? sb_device_sm_count() : 148;
+  const long long heads = (long long)B * n_kv;
+  const long long room = (64ll * sms + heads - 1) / heads;
+  const dim3 grid((unsigned)(wanted < room ? wanted : room), n_kv, B);
+  SB_CUDA_CHECK(launch_pdl(cache_read_fp8_kernel, grid, dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream),
+                           static_cast<const uint8_t *>(codes_k), static_cast<const uint8_t *>(scale_k),
+                           static_cast<const uint8_t *>(codes_v), static_cast<const uint8_t *>(scale_v), n_kv, dk, dv,
+                           s_max, begin, count, shared_len, static_cast<__nv_bfloat16 *>(out_k),
+                           static_cast<__nv_bfloat16 *>(out_v)));
+  SB_LAUNCH_CHECK();
+  return SB_OK;
+}
+
+}  // extern "C"

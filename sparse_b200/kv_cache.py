@@ -1,0 +1,43 @@
+"""A key/value cache in 8-bit floating point.
+
+Half the bytes of the bf16 cache: what a decode step's attention reads, and what a
+context of a given length takes of HBM.  Written by `ops.rope_append_quantized`, read by
+`ops.attn_decode_quantized` and, as bf16, by `ops.cache_read`.
+
+The row of a (sequence, head, position) is e4m3 codes and one power of two, the least
+one (2^-127 or more) by which the row's largest magnitude is at most 448.  Heads come
+before positions, unlike in the bf16 cache: a head's codes are then one run of bytes, and
+so are its scales, of which a position has only one byte per head.
+"""
+from __future__ import annotations
+
+import torch
+
+CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+class QuantizedCache:
+    """k [B, n_kv, S, dk] and v [B, n_kv, S, dv] codes, k_scale and v_scale [B, n_kv, S]."""
+    __slots__ = ("k", "k_scale", "v", "v_scale")
+
+    def __init__(self, k: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor, v_scale: torch.Tensor):
+        if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k_scale.shape != k.shape[:3] or (
+                v_scale.shape != k.shape[:3]):
+            raise RuntimeError("QuantizedCache: codes [B, n_kv, S, d] and scales [B, n_kv, S] do not fit: %s" % (
+                [tuple(t.shape) for t in (k, k_scale, v, v_scale)],))
+        for t, dtype in ((k, CODES), (k_scale, SCALES), (v, CODES), (v_scale, SCALES)):
+            if t.dtype != dtype or t.device != k.device or not t.is_contiguous():
+                raise RuntimeError("QuantizedCache needs contiguous %s codes and %s scales on one device" % (CODES, SCALES))
+        self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
+
+    @classmethod
+    def zeros(cls, batch: int, max_seq: int, n_kv: int, dk: int, dv: int, device) -> "QuantizedCache":
+        """A cache whose every position reads back as zero."""
+        def z(*shape, dtype):
+            return torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype)
+        return cls(z(batch, n_kv, max_seq, dk, dtype=CODES), z(batch, n_kv, max_seq, dtype=SCALES),
+                   z(batch, n_kv, max_seq, dv, dtype=CODES), z(batch, n_kv, max_seq, dtype=SCALES))
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device

@@ -6,12 +6,14 @@ of the tensors' device and never synchronise.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from ._lib import lib, check
+from .kv_cache import QuantizedCache
 
 _DT = {torch.bfloat16: _lib.SB_DTYPE_BF16, torch.float32: _lib.SB_DTYPE_F32}
 
@@ -195,6 +197,144 @@ def combine(rows_out: torch.Tensor, slot_of_item: torch.Tensor, idx: torch.Tenso
             check(lib.sb_combine_gated(_ptr(rows_out), _ptr(slot_of_item), _ptr(idx), _ptr(shared_out),
                                        _ptr(shared_scale), tokens, h, k, _ptr(out), _stream(rows_out)),
                   "sb_combine_gated")
+    return out
+
+
+def _rows3(t: torch.Tensor, what: str, like: torch.Tensor, heads, width: int) -> Tuple[int, int, int]:
+    """Address, token stride and head stride of a bf16 [T, heads, width] view (one head: shared)."""
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.device != like.device or t.shape[0] != like.shape[0] or (
+            t.shape[1] not in heads or t.shape[2] != width):
+        raise RuntimeError("rope_append_quantized: %s must be bf16 [%d, %s, %d] on %s, got %s %s on %s" % (
+            what, like.shape[0], " or ".join(map(str, heads)), width, like.device, t.dtype, tuple(t.shape), t.device))
+    if t.stride(2) != 1 and t.shape[2] > 1 and t.shape[0] > 0:
+        raise RuntimeError("rope_append_quantized: the elements of a head of %s must lie side by side" % what)
+    return t.data_ptr(), t.stride(0), t.stride(1) if t.shape[1] > 1 else 0
+
+
+def _index(t: torch.Tensor, n: int, device: torch.device, what: str) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+        raise RuntimeError("%s must be a contiguous int32 tensor of %d elements on %s" % (what, n, device))
+    return t.data_ptr()
+
+
+def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest: Optional[torch.Tensor],
+                          v: torch.Tensor, seq_of_token: torch.Tensor, pos_of_token: torch.Tensor,
+                          cache: QuantizedCache, theta: float) -> torch.Tensor:
+    """Rotary embedding of q and k, and k and v quantised into the cache; returns the rotated
+    queries [T, n_q, dk].
+
+    q [T, n_q, dk]; the first part of a key head, the rotated one, is k_rot [T, n_kv or 1, r]
+    (one head: shared by all), the rest k_rest [T, n_kv or 1, dk - r] (None where nothing is
+    left, as k_rot where nothing is rotated); v [T, n_kv or 1, dv].  All are bf16 views with any
+    token and head strides.  Token t goes to row (seq_of_token[t], pos_of_token[t]), int32; one
+    outside the cache is not stored."""
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.device != cache.device or not q.is_cuda:
+        raise RuntimeError("rope_append_quantized: q must be bf16 [T, n_q, dk] on the cache's CUDA device")
+    t, n_q, dk = q.shape
+    b, n_kv, s_max, dk_cache = cache.k.shape
+    dv = cache.v.shape[3]
+    rope = k_rot.shape[-1] if k_rot is not None else 0
+    if dk != dk_cache or rope > dk or n_q < 1:
+        raise RuntimeError("rope_append_quantized: heads of %d and a cache of heads of %d" % (dk, dk_cache))
+    if (k_rest is None) != (rope == dk):
+        raise RuntimeError("rope_append_quantized: k_rest holds the %d unrotated elements of a key head" % (dk - rope))
+    strides, ptrs = [], []
+    for view, what, heads, width in ((q, "q", (n_q,), dk), (k_rot, "k_rot", (n_kv, 1), rope),
+                                     (k_rest, "k_rest", (n_kv, 1), dk - rope), (v, "v", (n_kv, 1), dv)):
+        ptr, token, head = _rows3(view, what, q, heads, width) if view is not None else (None, 0, 0)
+        ptrs.append(ptr)
+        strides += [token, head]
+    seq, pos = (_index(x, t, q.device, "rope_append_quantized: " + n) for x, n in
+                ((seq_of_token, "seq_of_token"), (pos_of_token, "pos_of_token")))
+    out = torch.empty((t, n_q, dk), dtype=torch.bfloat16, device=q.device)
+    with torch.cuda.device(q.device):
+        check(lib.sb_rope_append_fp8(*ptrs, seq, pos, t, b, n_q, n_kv, dk, dv, rope, theta, s_max,
+                                     (ctypes.c_int64 * 8)(*strides), out.data_ptr(), cache.k.data_ptr(),
+                                     cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), _stream(q)),
+              "sb_rope_append_fp8")
+    return out
+
+
+def cache_read(cache: QuantizedCache, begin: int, count: int, shared_len: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Positions begin .. begin+count-1 of every sequence as bf16: (k [B, n_kv, count, dk],
+    v [B, n_kv, count, dv]), exactly the values the codes stand for.  Positions below
+    `shared_len` are sequence 0's."""
+    b, n_kv, s_max, dk = cache.k.shape
+    dv = cache.v.shape[3]
+    if not cache.k.is_cuda:
+        raise RuntimeError("sparse_b200 ops need CUDA tensors (there is no CPU path)")
+    if begin < 0 or count < 0 or begin + count > s_max or not 0 <= shared_len <= s_max:
+        raise RuntimeError("cache_read: positions %d .. %d, %d of them shared, of a cache of %d" % (
+            begin, begin + count, shared_len, s_max))
+    k = torch.empty((b, n_kv, count, dk), dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty((b, n_kv, count, dv), dtype=torch.bfloat16, device=cache.device)
+    with torch.cuda.device(cache.device):
+        check(lib.sb_cache_read_fp8(_ptr(cache.k), _ptr(cache.k_scale), _ptr(cache.v), _ptr(cache.v_scale), b, n_kv, dk, dv,
+                                    s_max, begin, count, shared_len, k.data_ptr(), v.data_ptr(), _stream(k)),
+              "sb_cache_read_fp8")
+    return k, v
+
+
+def _attn_operands(name: str, q: torch.Tensor, seq_lens: torch.Tensor, batch: int, n_kv: int, dk: int, dv: int, s_max: int,
+                   shared_len: int, device: torch.device, status: Optional[torch.Tensor]):
+    """Checks; -> (seq_lens, status, output, workspace) of a decode attention call."""
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.device != device or not q.is_cuda or q.shape[0] != batch or (
+            q.shape[2] != dk or q.shape[1] < 1):
+        raise RuntimeError("%s: q must be bf16 [%d, n_q, %d] on the cache's CUDA device, got %s %s on %s" % (
+            name, batch, dk, q.dtype, tuple(q.shape), q.device))
+    if batch > 0 and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != dk)) or (
+            batch > 1 and q.stride(0) < q.shape[1] * dk):
+        raise RuntimeError("%s: the heads of a sequence's query must lie side by side, sequences apart" % name)
+    if not 0 <= shared_len <= s_max:
+        raise RuntimeError("%s: %d shared positions of a cache of %d" % (name, shared_len, s_max))
+    if status is not None and (status.dtype != torch.int32 or status.device != device):
+        raise RuntimeError("%s: status must be int32 on %s" % (name, device))
+    lens = _index(seq_lens, batch, device, name + ": seq_lens")
+    n_q = q.shape[1]
+    out = torch.empty((batch, n_q, dv), dtype=torch.bfloat16, device=device)
+    ws_bytes = lib.sb_attn_cached_workspace_bytes(batch, n_q, n_kv, dv, s_max, shared_len)
+    return lens, _ptr(status), out, torch.empty((max(ws_bytes, 16),), dtype=torch.uint8, device=device)
+
+
+def attn_decode_quantized(q: torch.Tensor, cache: QuantizedCache, seq_lens: torch.Tensor, shared_len: int = 0,
+                          scale: Optional[float] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query per sequence, q [B, n_q, dk] bf16, against the first seq_lens[b] (int32)
+    positions of its quantised cache -> [B, n_q, dv]; zeros where there are none.
+
+    n_q is a multiple of the cache's heads.  `shared_len`: as many first positions are the
+    same for the whole batch and stand in sequence 0's rows; they are read once.  `scale`
+    defaults to dk ** -0.5; `status` as in `grouped_swiglu`."""
+    b, n_kv, s_max, dk = cache.k.shape
+    dv = cache.v.shape[3]
+    lens, st, out, ws = _attn_operands("attn_decode_quantized", q, seq_lens, b, n_kv, dk, dv, s_max, shared_len, cache.device,
+                                       status)
+    with torch.cuda.device(q.device):
+        check(lib.sb_attn_decode_fp8(q.data_ptr(), q.stride(0) if b > 1 else 0, _ptr(cache.k), _ptr(cache.k_scale),
+                                     _ptr(cache.v), _ptr(cache.v_scale), lens, b, q.shape[1], n_kv, dk, dv, s_max,
+                                     shared_len, dk ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(),
+                                     out.data_ptr(), st, _stream(q)), "sb_attn_decode_fp8")
+    return out
+
+
+def attn_decode_shared(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, seq_lens: torch.Tensor,
+                       shared_len: int, scale: Optional[float] = None,
+                       status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`attn_decode_quantized` over a bf16 cache, cache_k [B, S, n_kv, dk] and cache_v
+    [B, S, n_kv, dv]: the first `shared_len` positions of the batch stand in sequence 0's
+    rows and are read once for all sequences."""
+    if cache_k.dim() != 4 or cache_v.dim() != 4 or cache_k.shape[:3] != cache_v.shape[:3]:
+        raise RuntimeError("attn_decode_shared: caches [B, S, n_kv, d] do not fit: %s and %s" % (
+            tuple(cache_k.shape), tuple(cache_v.shape)))
+    if any(c.dtype != torch.bfloat16 or c.device != cache_k.device for c in (cache_k, cache_v)):
+        raise RuntimeError("attn_decode_shared needs bf16 caches on one device")
+    b, s_max, n_kv, dk = cache_k.shape
+    dv = cache_v.shape[3]
+    lens, st, out, ws = _attn_operands("attn_decode_shared", q, seq_lens, b, n_kv, dk, dv, s_max, shared_len, cache_k.device,
+                                       status)
+    with torch.cuda.device(q.device):
+        check(lib.sb_attn_decode_shared(q.data_ptr(), q.stride(0) if b > 1 else 0, _ptr(cache_k), _ptr(cache_v), lens, b,
+                                        q.shape[1], n_kv, dk, dv, s_max, shared_len, dk ** -0.5 if scale is None else scale,
+                                        ws.data_ptr(), ws.numel(), out.data_ptr(), st, _stream(q)), "sb_attn_decode_shared")
     return out
 
 
