@@ -649,7 +649,8 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  *                  positions of its quantised cache; softmax in fp32; out [B,n_q,dv] bf16,
  *                  zeros for a sequence without positions.  Query head h reads key head
  *                  h / (n_q / n_kv).  With shared_len > 0 positions below it are read from
- *                  sequence 0's rows, once for all sequences that are longer than it.  ws:
+ *                  sequence 0's rows, once for all sequences that reach over them.
+ *                  scale >= 0.  ws:
  *                  sb_attn_cached_workspace_bytes(), 16-byte aligned, not shared by calls
  *                  that may overlap on the GPU.  status: device int32 (may be NULL), set
  *                  non-zero if a bounded wait gave up.  (dk,dv) = (128,128), (192,128),

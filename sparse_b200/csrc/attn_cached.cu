@@ -17,7 +17,7 @@
 // or reaches over several leaves a partial result for each, and attn_join_kernel joins those.
 #include <math.h>
 
-#include "kv_fp8.cuh"
+#include "attn_cached.cuh"
 
 namespace sb {
 namespace {
@@ -25,20 +25,6 @@ namespace {
 constexpr int kThreads = 128;                 // four warps, 16 positions of a tile each
 constexpr int kTile = 64;
 constexpr int kMaxCtas = 592;                 // 148 SMs, four CTAs each
-
-struct Cache {                        // bf16: [B, s_max, n_kv, d]; quantised: codes [B, n_kv, s_max, d], scales [B, n_kv, s_max]
-  const void *k, *v;
-  const uint8_t *ks, *vs;
-};
-
-struct Shape {
-  int B, n_q, n_kv, group;            // group = query heads per key head
-  int s_max, shared_len;
-  int rows;                           // query rows of a segment (at most 8 * NT)
-  int row_tiles, pre_row_tiles;       // segments per key head: of a sequence, and of the shared positions
-  int64_t q_stride;
-  float scale_log2;                   // scale * log2(e)
-};
 
 // The line of tiles: first the shared positions (per key head and row tile), then
 // sequence by sequence, key head by key head, row tile by row tile.
@@ -63,11 +49,6 @@ __device__ __forceinline__ uint2 ldg_stream8(const void *p) {
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
   return r;
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -86,10 +67,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t *>(&v);
 }
-
-// A weight below this multiple of the running maximum's does not move the maximum: sums and
-// weights stay below 2^8 times their usual size, and most steps have nothing to rescale.
-constexpr float kLazy = 8.f;
 
 // The state of one warp over a run of positions, NT * 8 query rows (row 8 nt + 2c + r in
 // registers [nt][.][r] of lanes with lane % 4 == c).
@@ -489,7 +466,8 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
 template <int DV>
 __global__ void __launch_bounds__(DV)
 attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, const float *__restrict__ part,
-                 const float *__restrict__ part_lse, __nv_bfloat16 *__restrict__ out) {
+                 const float *__restrict__ part_lse, const float *__restrict__ pre_part, const float *__restrict__ pre_lse,
+                 __nv_bfloat16 *__restrict__ out) {
   __shared__ int s_sum[2][DV / 32];
   pdl_launch_dependents();
   pdl_wait();
@@ -511,8 +489,8 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
   const int total = pre_line + own_heads * all, share = (total + n_ctas - 1) / n_ctas;
   const int len = seq_len(s, seq_lens, b);
   float top = -INFINITY, sum = 0.f, acc = 0.f;
-  const auto take = [&](size_t slot, int row) {
-    const float lse = part_lse[slot * s.rows + row], o = part[(slot * s.rows + row) * DV + threadIdx.x];
+  const auto take = [&](const float *from, const float *from_lse, size_t slot_row) {
+    const float lse = from_lse[slot_row], o = from[slot_row * DV + threadIdx.x];
     const float m = fmaxf(top, lse), ref = m == -INFINITY ? 0.f : m;
     const float f = exp2_approx(top - ref), w = exp2_approx(lse - ref);
     sum = sum * f + w;
@@ -520,9 +498,13 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
     top = m;
   };
   const auto pieces = [&](int first, int tiles, int segment, int row) {
-    for (int cta = first / share; cta <= (first + tiles - 1) / share; ++cta) take((size_t)cta + segment, row);
+    for (int cta = first / share; cta <= (first + tiles - 1) / share; ++cta) take(part, part_lse, ((size_t)cta + segment) * s.rows + row);
   };
-  if (pre_line > 0 && len >= s.shared_len) {
+  if (s.pre_splits > 0 && len >= s.shared_len) {
+    const int r = b * s.group + hg, rt = r / kPrefixRows, rows = prefix_rows(s);
+    const size_t slot = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * 2;
+    for (int i = 0; i < 2 * s.pre_splits; ++i) take(pre_part, pre_lse, (slot + i) * rows + r - rt * kPrefixRows);
+  } else if (pre_line > 0 && len >= s.shared_len) {
     const int r = b * s.group + hg, rt = r / s.rows, n = pre_tiles(s);
     const int seg = hk * s.pre_row_tiles + rt;
     pieces(seg * n, n, seg, r - rt * s.rows);
@@ -537,21 +519,29 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
 
 constexpr int kMaxRows = 16;
 
-// Rows, row tiles and segments of a call; the rest of the shape is the caller's.
+// How a call is cut; the rest of the shape is the caller's.  Up to sixteen rows share one
+// pass of the streamed line over the prefix, more go through the tensor-core tiles.
 void plan(Shape &s) {
-  const int widest = s.shared_len > 0 ? (s.B * (int64_t)s.group > kMaxRows ? kMaxRows : s.B * s.group) : s.group;
-  s.rows = widest > s.group ? widest : s.group;
-  if (s.rows > kMaxRows) s.rows = kMaxRows;
+  const int64_t pre_rows = s.shared_len > 0 ? (int64_t)s.B * s.group : 0;
+  s.pre_splits = pre_rows > kMaxRows ? prefix_splits(s) : 0;
+  s.rows = s.group > kMaxRows ? kMaxRows : s.group;
+  if (pre_rows > s.rows && s.pre_splits == 0) s.rows = (int)pre_rows;
   s.row_tiles = (s.group + s.rows - 1) / s.rows;
-  s.pre_row_tiles = s.shared_len > 0 ? (int)(((int64_t)s.B * s.group + s.rows - 1) / s.rows) : 0;
+  s.pre_row_tiles = pre_rows > 0 && s.pre_splits == 0 ? 1 : 0;
 }
-int64_t slots(const Shape &s) { return kMaxCtas + (int64_t)s.n_kv * (s.pre_row_tiles + (int64_t)s.B * s.row_tiles); }
+// Partial results: of the streamed line, then of the shared positions' tiles; outputs first,
+// then logarithms.
+int64_t slot_rows(const Shape &s) { return (kMaxCtas + (int64_t)s.n_kv * (s.pre_row_tiles + (int64_t)s.B * s.row_tiles)) * s.rows; }
+int64_t pre_slot_rows(const Shape &s) { return prefix_slots(s) * prefix_rows(s); }
 
 template <int DK, int DV, bool FP8>
 int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_lens, const Shape &s, float *part,
-               __nv_bfloat16 *out, cudaStream_t st) {
-  const int64_t slot_rows = slots(s) * s.rows;
-  float *lse = part + slot_rows * DV;
+               __nv_bfloat16 *out, int32_t *status, cudaStream_t st) {
+  float *pre_part = part + slot_rows(s) * DV, *lse = pre_part + pre_slot_rows(s) * DV, *pre_lse = lse + slot_rows(s);
+  if (s.pre_splits > 0) {
+    const int32_t rc = launch_attn_prefix(FP8, DK, DV, q, cache, s, pre_part, pre_lse, status, st);
+    if (rc != SB_OK) return rc;
+  }
   const int sms = sb_device_sm_count() > 0 ? sb_device_sm_count() : 148;
   // a CTA for every tile there can be, up to four per SM
   const int64_t tiles = (int64_t)s.n_kv * ((int64_t)s.pre_row_tiles * ((s.shared_len + kTile - 1) / kTile) +
@@ -562,7 +552,8 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
   SB_CUDA_CHECK(launch_pdl(kern, dim3(ctas), dim3(kThreads), 0, st, q, cache, seq_lens, s, part, lse));
   SB_LAUNCH_CHECK();
   SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV>, dim3(s.B * s.n_q), dim3(DV), 0, st, seq_lens, s, ctas,
-                           static_cast<const float *>(part), static_cast<const float *>(lse), out));
+                           static_cast<const float *>(part), static_cast<const float *>(lse),
+                           static_cast<const float *>(pre_part), static_cast<const float *>(pre_lse), out));
   SB_LAUNCH_CHECK();
   return SB_OK;
 }
@@ -570,11 +561,12 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
 template <bool FP8>
 int32_t attend(const char *name, const void *q, int64_t q_stride, Cache cache, const int32_t *seq_lens, int B, int n_q,
                int n_kv, int dk, int dv, int s_max, int shared_len, float scale, void *ws, size_t ws_bytes, void *out,
-               void *stream) {
+               int32_t *status, void *stream) {
   // (the line's tiles are counted in 32 bits)
-  if (B < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || s_max < 1 || shared_len < 0 || shared_len > s_max ||
+  if (B < 0 || n_q < 1 || n_kv < 1 || n_kv > 65535 || n_q % n_kv != 0 || s_max < 1 || shared_len < 0 || shared_len > s_max ||
       (int64_t)B * n_q > (1 << 22) || (int64_t)B * n_q * (s_max / kTile + 2) > (1ll << 30))
     return fail(SB_E_INVALID_ARG, "%s: bad shape (B=%d heads %d/%d s_max=%d shared %d)", name, B, n_q, n_kv, s_max, shared_len);
+  if (!(scale >= 0.f) || !isfinite(scale)) return fail(SB_E_INVALID_ARG, "%s: scale must be finite and not negative", name);
   if (q_stride == 0) q_stride = (int64_t)n_q * dk;
   if (q_stride < (int64_t)n_q * dk) return fail(SB_E_INVALID_ARG, "%s: q_stride smaller than a token's heads", name);
   if (!((dk == 128 && dv == 128) || (dk == 192 && dv == 128) || (dk == 64 && dv == 64)))
@@ -586,15 +578,15 @@ int32_t attend(const char *name, const void *q, int64_t q_stride, Cache cache, c
     return fail(SB_E_INVALID_ARG, "%s: cache and workspace must be 16-byte aligned", name);
   if (ws_bytes < sb_attn_cached_workspace_bytes(B, n_q, n_kv, dv, s_max, shared_len))
     return fail(SB_E_WORKSPACE, "%s: workspace too small", name);
-  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, q_stride, scale * 1.4426950408889634f};
+  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, q_stride, scale * 1.4426950408889634f};
   plan(s);
   const __nv_bfloat16 *qq = static_cast<const __nv_bfloat16 *>(q);
   float *part = static_cast<float *>(ws);
   __nv_bfloat16 *oo = static_cast<__nv_bfloat16 *>(out);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dk == 128 ? launch<128, 128, FP8>(qq, cache, seq_lens, s, part, oo, st)
-         : dk == 192 ? launch<192, 128, FP8>(qq, cache, seq_lens, s, part, oo, st)
-                     : launch<64, 64, FP8>(qq, cache, seq_lens, s, part, oo, st);
+  return dk == 128 ? launch<128, 128, FP8>(qq, cache, seq_lens, s, part, oo, status, st)
+         : dk == 192 ? launch<192, 128, FP8>(qq, cache, seq_lens, s, part, oo, status, st)
+                     : launch<64, 64, FP8>(qq, cache, seq_lens, s, part, oo, status, st);
 }
 
 }  // namespace
@@ -607,28 +599,26 @@ extern "C" {
 size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t dv, int32_t s_max, int32_t shared_len) {
   if (B < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || dv < 1 || s_max < 1 || shared_len < 0 || (int64_t)B * n_q > (1 << 22))
     return 0;
-  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0.f};
+  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, 0.f};
   plan(s);
-  return (size_t)slots(s) * s.rows * (dv + 1) * sizeof(float);
+  return (size_t)(slot_rows(s) + pre_slot_rows(s)) * (dv + 1) * sizeof(float);
 }
 
 int32_t sb_attn_decode_shared(const void *q, int64_t q_stride, const void *cache_k, const void *cache_v,
                               const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk, int32_t dv,
                               int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
                               int32_t *status, void *stream) {
-  (void)status;
   return attend<false>("sb_attn_decode_shared", q, q_stride, Cache{cache_k, cache_v, nullptr, nullptr}, seq_lens, B, n_q,
-                       n_kv, dk, dv, s_max, shared_len, scale, ws, ws_bytes, out, stream);
+                       n_kv, dk, dv, s_max, shared_len, scale, ws, ws_bytes, out, status, stream);
 }
 
 int32_t sb_attn_decode_fp8(const void *q, int64_t q_stride, const void *codes_k, const void *scale_k, const void *codes_v,
                            const void *scale_v, const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk,
                            int32_t dv, int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
                            int32_t *status, void *stream) {
-  (void)status;
   return attend<true>("sb_attn_decode_fp8", q, q_stride,
                       Cache{codes_k, codes_v, static_cast<const uint8_t *>(scale_k), static_cast<const uint8_t *>(scale_v)},
-                      seq_lens, B, n_q, n_kv, dk, dv, s_max, shared_len, scale, ws, ws_bytes, out, stream);
+                      seq_lens, B, n_q, n_kv, dk, dv, s_max, shared_len, scale, ws, ws_bytes, out, status, stream);
 }
 
 }  // extern "C"

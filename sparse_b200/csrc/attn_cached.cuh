@@ -1,0 +1,49 @@
+// Decode attention over cached positions: what its kernels share.
+#pragma once
+
+#include "kv_fp8.cuh"
+
+namespace sb {
+
+struct Cache {                        // bf16: [B, s_max, n_kv, d]; quantised: codes [B, n_kv, s_max, d], scales [B, n_kv, s_max]
+  const void *k, *v;
+  const uint8_t *ks, *vs;
+};
+
+struct Shape {
+  int B, n_q, n_kv, group;            // group = query heads per key head
+  int s_max, shared_len;
+  int rows;                           // query rows of a segment of the streamed line (at most 16)
+  int row_tiles, pre_row_tiles;       // its segments per key head: of a sequence, and of the shared positions
+  int pre_splits;                     // > 0: the shared positions go through attn_prefix_kernel, cut in so many
+  int64_t q_stride;
+  float scale_log2;                   // scale * log2(e), >= 0
+};
+
+// Query rows of one tile of attn_prefix_kernel.  The rows of a key head are numbered
+// sequence by sequence: row = b * group + h.
+constexpr int kPrefixRows = 128;
+__host__ __device__ inline int prefix_row_tiles(const Shape &s) { return (int)(((int64_t)s.B * s.group + kPrefixRows - 1) / kPrefixRows); }
+// Partial results of that kernel: two per CTA, of `prefix_rows` rows.
+__host__ __device__ inline int prefix_rows(const Shape &s) { return s.B * (int64_t)s.group < kPrefixRows ? s.B * s.group : kPrefixRows; }
+inline int64_t prefix_slots(const Shape &s) { return (int64_t)s.n_kv * prefix_row_tiles(s) * s.pre_splits * 2; }
+
+// Sizes for which the shared positions of a call are cut `splits` ways by attn_prefix_kernel.
+int prefix_splits(const Shape &s);
+
+// softmax(q k) v of every row of the batch over the shared positions, as partial results:
+// part [slot][row][dv] attention over the slot's positions, lse [slot][row] log2 of their sum of exponentials.
+int32_t launch_attn_prefix(bool fp8, int dk, int dv, const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float *part,
+                           float *lse, int32_t *status, cudaStream_t stream);
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A weight below this power of two of the running maximum's does not move the maximum: sums
+// and weights stay below 2^8 times their usual size, and most steps have nothing to rescale.
+constexpr float kLazy = 8.f;
+
+}  // namespace sb

@@ -1,0 +1,465 @@
+// Attention of a whole batch's queries over the positions that its sequences share: for
+// every key head one matrix product of the batch's rows (sequences x query heads of the
+// group, tiles of 128) with the shared keys, a softmax along the keys, and a second product
+// with the values, on the tensor cores.
+//
+// Bound by the bytes of the prefix while the rows fit one tile (bf16, heads of 128: 64 KB
+// per 128 positions are 2.8 K clocks of an SM's share of HBM, the two products 1 K, the
+// exponentials 1 K), by the exponentials and the conversion of codes beyond.  One CTA per
+// SM; the positions are cut into as many runs as fill the machine.
+//
+// Roles: warp 0 loads tiles of 128 keys and values (TMA: bf16 boxes into the swizzled operand
+// layout; codes as one run of bytes each), warp 1 issues the products, two groups of four
+// warps do the softmax, one thread per row, on alternating tiles.  Each group has its own
+// scores, its own running maximum and its own output accumulator in TMEM (2 x 128 + 2 x DV
+// columns), so the groups exchange nothing and one group's products run under the other's
+// exponentials; probabilities go back into TMEM (bf16, over their scores), where the second
+// product takes its left operand from.  Quantised: four more warps turn a row of codes per
+// thread into bf16 operands, scale applied (exact), so the products are the bf16 ones.
+//
+// Probabilities are rounded to bf16 (2^-8), the type of the values that they are multiplied
+// with, and their sum is taken over the rounded ones; scores, sums and accumulators are fp32.
+//
+// All mbarrier waits are bounded; when one runs out the CTA raises its abort flag, reports
+// through `status`, waits for its copies and frees its TMEM.
+#include <math.h>
+
+#include "attn_cached.cuh"
+#include "sb_tc.cuh"
+
+namespace sb {
+namespace {
+
+constexpr int kKeys = 128;                       // positions of a tile
+constexpr uint32_t kBox = kKeys * 128;           // 64 bf16 columns of 128 rows: 16 KB
+constexpr int kSoftmaxWarp = 4, kConvertWarp = 12;
+
+template <int DK, int DV, bool FP8>
+struct Layout {
+  static constexpr uint32_t kQ = DK / 64 * kBox, kK = DK / 64 * kBox, kV = DV / 64 * kBox;
+  // operand buffers: filled by TMA (bf16), or by the converting warps from two stages of codes
+  static constexpr int kStages = FP8 ? (DK > 128 ? 1 : 2) : (DK > 128 ? 2 : DK > 64 ? 3 : 4);
+  static constexpr int kRaw = FP8 ? 2 : 0;
+  static constexpr uint32_t kRawK = kKeys * DK, kRawV = kKeys * DV;
+  static constexpr uint32_t kBytes = kQ + kStages * (kK + kV) + kRaw * (kRawK + kRawV);
+  static constexpr uint32_t kSmem = kBytes + 1024 + 256;
+  static constexpr int kThreads = FP8 ? 512 : 384;
+  static_assert(kSmem <= 232448, "shared memory of a CTA");
+};
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *tm, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D (TMEM) = or += A (shared memory) * B (shared memory)
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// D (TMEM) = or += A (TMEM, two bf16 a column) * B (shared memory)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// fp32 accumulator, bf16 operands, M = 128; b_mn: B lies along N instead of along K
+constexpr uint32_t idesc_m128(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// The values as the right operand of the second product: a row per position (the product's
+// K), 64-column boxes of 128-byte rows under the 128-byte swizzle; 16 KB from box to box along
+// N, 1 KB from eight rows to the next eight along K.
+__device__ __forceinline__ uint64_t desc_values(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(kBox >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// byte offset of 16-byte chunk `chunk` of row `row` in 64-column boxes under the 128-byte swizzle
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
+  return (uint32_t)(chunk >> 3) * kBox + (uint32_t)row * 128 + (uint32_t)(((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// sixteen codes (one 16-byte chunk) times a power of two -> two chunks of bf16, exact
+__device__ __forceinline__ void convert16(const uint4 &c, float scale, uint4 &lo, uint4 &hi) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = f16x2_to_float2(e4m3x2_to_f16x2(w[i])), b = f16x2_to_float2(e4m3x2_to_f16x2(w[i] >> 16));
+    o[2 * i] = pack_bf16x2(a.x * scale, a.y * scale);
+    o[2 * i + 1] = pack_bf16x2(b.x * scale, b.y * scale);
+  }
+  lo = make_uint4(o[0], o[1], o[2], o[3]);
+  hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// grid = (runs of positions, row tiles, key heads)
+template <int DK, int DV, bool FP8>
+__global__ void __launch_bounds__(Layout<DK, DV, FP8>::kThreads, 1)
+attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                   const __nv_bfloat16 *__restrict__ q, Cache cache, Shape s, float *__restrict__ part,
+                   float *__restrict__ part_lse, int32_t *__restrict__ status) {
+  using L = Layout<DK, DV, FP8>;
+  constexpr int NS = L::kStages, NR = L::kRaw;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char *aligned_base = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t q_smem = base, k_smem = q_smem + L::kQ, v_smem = k_smem + NS * L::kK, raw_smem = v_smem + NS * L::kV;
+  const uint32_t bars = base + L::kBytes;
+  const uint32_t k_full = bars, k_empty = k_full + 8 * 4, v_full = k_empty + 8 * 4, v_empty = v_full + 8 * 4;
+  const uint32_t s_full = v_empty + 8 * 4, p_full = s_full + 16, o_full = p_full + 16;
+  const uint32_t rk_full = o_full + 16, rv_full = rk_full + 16, r_empty = rv_full + 16;       // two each
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(aligned_base + L::kBytes + 8 * 16 + 16 * 6);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.z, rt = blockIdx.y;
+  const int all_tiles = (s.shared_len + kKeys - 1) / kKeys;
+  const int tile0 = (int)((int64_t)blockIdx.x * all_tiles / gridDim.x), tile1 = (int)((int64_t)(blockIdx.x + 1) * all_tiles / gridDim.x);
+  const int n = tile1 - tile0;
+  const int rows = min(kPrefixRows, s.B * s.group - rt * kPrefixRows);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(k_full + 8 * i, FP8 ? 4 : 1); mbar_init(k_empty + 8 * i, 1);
+      mbar_init(v_full + 8 * i, FP8 ? 4 : 1); mbar_init(v_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); mbar_init(o_full + 8 * i, 1);
+      mbar_init(rk_full + 8 * i, 1); mbar_init(rv_full + 8 * i, 1); mbar_init(r_empty + 8 * i, 4);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  // the tile's query rows, zeros behind the last one
+  const bool q_vec = s.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  for (int i = threadIdx.x; i < kPrefixRows * (DK / 8); i += L::kThreads) {
+    const int row = i / (DK / 8), chunk = i - row * (DK / 8);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (row < rows) {
+      const int r = rt * kPrefixRows + row, b = r / s.group, h = hk * s.group + r - b * s.group;
+      const __nv_bfloat16 *src = q + b * s.q_stride + (size_t)h * DK + chunk * 8;
+      if (q_vec) {
+        x = __ldg(reinterpret_cast<const uint4 *>(src));
+      } else {
+        const unsigned short *e = reinterpret_cast<const unsigned short *>(src);
+        x = make_uint4(e[0] | ((uint32_t)e[1] << 16), e[2] | ((uint32_t)e[3] << 16), e[4] | ((uint32_t)e[5] << 16),
+                       e[6] | ((uint32_t)e[7] << 16));
+      }
+    }
+    *reinterpret_cast<uint4 *>(aligned_base + swizzled(row, chunk)) = x;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t s_tmem = tmem, o_tmem = tmem + 2 * kKeys;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      if constexpr (FP8) {
+        const size_t row0 = (size_t)hk * s.s_max;
+        for (int i = 0; i < n; ++i) {
+          const int st = i & 1, key = (tile0 + i) * kKeys;
+          const uint32_t keys = min(kKeys, s.shared_len - key);
+          if (!mbar_wait(r_empty + 8 * st, ((i >> 1) & 1) ^ 1u, abort_flag)) break;
+          const uint32_t dst = raw_smem + st * (L::kRawK + L::kRawV);
+          mbar_expect_tx(rk_full + 8 * st, keys * DK);
+          bulk_load(dst, static_cast<const uint8_t *>(cache.k) + (row0 + key) * DK, keys * DK, rk_full + 8 * st);
+          mbar_expect_tx(rv_full + 8 * st, keys * DV);
+          bulk_load(dst + L::kRawK, static_cast<const uint8_t *>(cache.v) + (row0 + key) * DV, keys * DV, rv_full + 8 * st);
+        }
+      } else {
+        // (positions behind the last shared one lie outside the tensor map: zeros)
+        for (int i = 0; i < n; ++i) {
+          const int st = i % NS, key = (tile0 + i) * kKeys;
+          const uint32_t ph = ((i / NS) & 1) ^ 1u;
+          if (!mbar_wait(k_empty + 8 * st, ph, abort_flag)) break;
+          mbar_expect_tx(k_full + 8 * st, L::kK);
+#pragma unroll
+          for (int x = 0; x < DK / 64; ++x) tma_load_3d(k_smem + st * L::kK + x * kBox, &tm_k, k_full + 8 * st, x * 64, hk, key);
+          if (!mbar_wait(v_empty + 8 * st, ph, abort_flag)) break;
+          mbar_expect_tx(v_full + 8 * st, L::kV);
+#pragma unroll
+          for (int x = 0; x < DV / 64; ++x) tma_load_3d(v_smem + st * L::kV + x * kBox, &tm_v, v_full + 8 * st, x * 64, hk, key);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_m128(kKeys, false), id_o = idesc_m128(DV, true);
+      bool ok = true;
+      const auto scores = [&](int i) {
+        const int st = i % NS;
+        if (!mbar_wait(k_full + 8 * st, (i / NS) & 1, abort_flag)) return false;
+        tc_fence_after();
+        const uint64_t a = umma_desc_sw128(q_smem), b = umma_desc_sw128(k_smem + st * L::kK);
+#pragma unroll
+        for (int x = 0; x < DK / 16; ++x) {
+          const uint64_t off = (uint64_t)((x >> 2) * (kBox >> 4) + (x & 3) * 2);
+          tc_mma_ss(s_tmem + (i & 1) * kKeys, a + off, b + off, id_s, x > 0);
+        }
+        tc_commit(s_full + 8 * (i & 1));
+        tc_commit(k_empty + 8 * st);
+        return true;
+      };
+      if (n > 0) ok = scores(0);
+      for (int i = 0; ok && i < n; ++i) {
+        // (the scores of tile i + 1 go where those of i - 1 were: their second product is issued)
+        if (i + 1 < n && !scores(i + 1)) break;
+        const int st = i % NS, w = i & 1;
+        if (!mbar_wait(v_full + 8 * st, (i / NS) & 1, abort_flag)) break;
+        if (!mbar_wait(p_full + 8 * w, (i >> 1) & 1, abort_flag)) break;
+        tc_fence_after();
+        const uint64_t b = desc_values(v_smem + st * L::kV);
+#pragma unroll
+        for (int x = 0; x < kKeys / 16; ++x)
+          tc_mma_ts(o_tmem + w * DV, s_tmem + w * kKeys + x * 8, b + (uint64_t)(x * (2048 >> 4)), id_o, i > 1 || x > 0);
+        tc_commit(v_empty + 8 * st);
+        if (i + 2 >= n) tc_commit(o_full + 8 * w);
+      }
+    }
+  } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
+    const int w = (warp - kSoftmaxWarp) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
+    const uint32_t st_at = s_tmem + w * kKeys + lane_at, ot_at = o_tmem + w * DV + lane_at;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int i = w; i < n; i += 2) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * w, (i >> 1) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      const int keys = min(kKeys, s.shared_len - (tile0 + i) * kKeys);
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kKeys; x += 32) {
+        uint32_t r[32];
+        tc_ld32(st_at + x, r);
+        tc_wait_ld();
+        if (x + 32 <= keys) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = x + e < keys ? fmaxf(top, __uint_as_float(r[e])) : top;
+        }
+      }
+      top *= s.scale_log2;
+      if (__any_sync(0xffffffffu, top > m + kLazy)) {
+        const float up = fmaxf(m, top), f = m == -INFINITY ? 0.f : exp2_approx(m - up);
+        l *= f;
+        m = up;
+        if (i >= 2) {                  // (the tile's scores are behind all earlier products: the accumulator is still)
+#pragma unroll
+          for (int x = 0; x < DV; x += 32) {
+            uint32_t r[32], h[16];
+            tc_ld32(ot_at + x, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) h[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+            tc_st16(ot_at + x, h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) h[e] = __float_as_uint(__uint_as_float(r[16 + e]) * f);
+            tc_st16(ot_at + x + 16, h);
+          }
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int x = 0; x < kKeys; x += 32) {
+        uint32_t r[32], p[16];
+        tc_ld32(st_at + x, r);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float a = exp2_approx(fmaf(__uint_as_float(r[2 * e]), s.scale_log2, -ref));
+          float b = exp2_approx(fmaf(__uint_as_float(r[2 * e + 1]), s.scale_log2, -ref));
+          if (x + 32 > keys) {
+            if (x + 2 * e >= keys) a = 0.f;
+            if (x + 2 * e + 1 >= keys) b = 0.f;
+          }
+          p[e] = pack_bf16x2(a, b);
+          l += bf16_lo(p[e]) + bf16_hi(p[e]);
+        }
+        tc_st16(st_at + x / 2, p);
+      }
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + 8 * w);
+    }
+    // this group's partial result; without a tile, or with an empty row, nothing that weighs
+    const size_t slot = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * 2 + w;
+    const int slot_rows = prefix_rows(s);
+    const bool any = w < n;
+    if (ok && any) {
+      ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * w, 0, abort_flag));
+      tc_fence_after();
+    }
+    if (ok) {
+      const float f = l == 0.f ? 0.f : 1.f / l;
+      float *dst = part + (slot * slot_rows + row) * DV;
+#pragma unroll
+      for (int x = 0; x < DV; x += 32) {
+        uint32_t r[32];
+        tc_ld32(ot_at + x, r);
+        tc_wait_ld();
+        if (row < rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4 *>(dst + x + e) =
+                any && l != 0.f ? make_float4(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f,
+                                              __uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      if (row < rows) part_lse[slot * slot_rows + row] = l == 0.f ? -INFINITY : m + log2f(l);
+      tc_fence_before();
+    }
+  } else if (FP8 && warp >= kConvertWarp) {
+    // one row of codes per thread, its chunks in an order that keeps eight neighbouring rows
+    // on different banks, in the codes and in the swizzled operand
+    const int row = (warp - kConvertWarp) * 32 + lane;
+    const size_t row0 = (size_t)hk * s.s_max;
+    const auto convert = [&](uint32_t src, uint32_t dst, int d, float scale, bool in) {
+      const int chunks = d / 16;
+      int chunk = row % chunks;
+      for (int x = 0; x < chunks; ++x, chunk = chunk + 1 == chunks ? 0 : chunk + 1) {
+        uint4 c = make_uint4(0, 0, 0, 0), lo, hi;
+        if (in) c = *reinterpret_cast<const uint4 *>(aligned_base + (src - base) + row * d + chunk * 16);
+        convert16(c, in ? scale : 0.f, lo, hi);
+        *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk)) = lo;
+        *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk + 1)) = hi;
+      }
+    };
+    const auto scale_at = [&](const uint8_t *scales, int i) {
+      const int key = (tile0 + i) * kKeys + row;
+      return i < n && key < s.shared_len ? (uint32_t)__ldg(scales + row0 + key) : 0u;
+    };
+    uint32_t ks = scale_at(cache.ks, 0), vs = scale_at(cache.vs, 0);
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1, op = i % NS;
+      const uint32_t raw = raw_smem + st * (L::kRawK + L::kRawV), ph = (i >> 1) & 1, op_ph = ((i / NS) & 1) ^ 1u;
+      const bool in = (tile0 + i) * kKeys + row < s.shared_len;
+      const uint32_t ks_next = scale_at(cache.ks, i + 1), vs_next = scale_at(cache.vs, i + 1);
+      bool ok = mbar_wait(rk_full + 8 * st, ph, abort_flag) && mbar_wait(k_empty + 8 * op, op_ph, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      convert(raw, k_smem + op * L::kK, DK, e8m0_value(ks), in);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(k_full + 8 * op);
+      ok = mbar_wait(rv_full + 8 * st, ph, abort_flag) && mbar_wait(v_empty + 8 * op, op_ph, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      convert(raw + L::kRawK, v_smem + op * L::kV, DV, e8m0_value(vs), in);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(v_full + 8 * op); mbar_arrive(r_empty + 8 * st); }
+      ks = ks_next;
+      vs = vs_next;
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && status) atomicExch(status, 1);
+    const unsigned long long t0 = gtime_ns();
+    while (gtime_ns() - t0 < 2000000ull) __nanosleep(1000);       // copies in flight
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// The shared rows of a bf16 cache as [shared_len][n_kv][d], boxes of 64 columns, one head, 128 positions.
+int32_t encode_rows(CUtensorMap *tm, const void *base, int d, int n_kv, int shared_len) {
+  // A map depends on these values only: the last ones of a thread are kept, as for the grouped GEMM.
+  struct Entry { const void *base; int d, n_kv, len; CUtensorMap map; };
+  static thread_local Entry kept[64];
+  static thread_local int used = 0, next = 0;
+  for (int i = 0; i < used; ++i)
+    if (kept[i].base == base && kept[i].d == d && kept[i].n_kv == n_kv && kept[i].len == shared_len) { *tm = kept[i].map; return SB_OK; }
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(SB_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)n_kv, (cuuint64_t)shared_len};
+  cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)d * n_kv * 2};
+  cuuint32_t box[3] = {64, 1, kKeys}, step[3] = {1, 1, 1};
+  const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SB_E_CUDA, "cuTensorMapEncodeTiled of the shared rows failed with CUresult %d", (int)r);
+  const int slot = used < 64 ? used++ : next++ % 64;
+  kept[slot] = Entry{base, d, n_kv, shared_len, *tm};
+  return SB_OK;
+}
+
+template <int DK, int DV, bool FP8>
+int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float *part, float *lse, int32_t *status,
+               cudaStream_t stream) {
+  using L = Layout<DK, DV, FP8>;
+  CUtensorMap tm_k = {}, tm_v = {};
+  if (!FP8) {
+    int32_t rc = encode_rows(&tm_k, cache.k, DK, s.n_kv, s.shared_len);
+    if (rc == SB_OK) rc = encode_rows(&tm_v, cache.v, DV, s.n_kv, s.shared_len);
+    if (rc != SB_OK) return rc;
+  }
+  auto kern = attn_prefix_kernel<DK, DV, FP8>;
+  SB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
+  const dim3 grid(s.pre_splits, prefix_row_tiles(s), s.n_kv);
+  SB_CUDA_CHECK(launch_pdl(kern, grid, dim3(L::kThreads), L::kSmem, stream, tm_k, tm_v, q, cache, s, part, lse, status));
+  SB_LAUNCH_CHECK();
+  return SB_OK;
+}
+
+}  // namespace
+
+int prefix_splits(const Shape &s) {
+  const int64_t tiles = (s.shared_len + kKeys - 1) / kKeys, heads = (int64_t)s.n_kv * prefix_row_tiles(s);
+  const int64_t fit = 148 / heads;
+  return (int)(fit < 1 ? 1 : fit < tiles ? fit : tiles);
+}
+
+int32_t launch_attn_prefix(bool fp8, int dk, int dv, const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float *part,
+                           float *lse, int32_t *status, cudaStream_t stream) {
+  if (dk == 128) return (fp8 ? launch<128, 128, true> : launch<128, 128, false>)(q, cache, s, part, lse, status, stream);
+  if (dk == 192) return (fp8 ? launch<192, 128, true> : launch<192, 128, false>)(q, cache, s, part, lse, status, stream);
+  return (fp8 ? launch<64, 64, true> : launch<64, 64, false>)(q, cache, s, part, lse, status, stream);
+}
+
+}  // namespace sb

@@ -485,3 +485,22 @@ def test_wrappers_refuse_operands_that_do_not_fit():
     with pytest.raises(RuntimeError):
         ops.attn_decode_shared(q, _rand(2, 2, 2, 64).transpose(1, 2), _rand(2, 2, 2, 64), lens, 0)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("b,n_q,n_kv,dk,dv,shared", [(18, 37, 37, 128, 128, 4500), (18, 37, 37, 64, 64, 4517),
+                                                     (18, 37, 37, 192, 128, 2305), (150, 74, 74, 64, 64, 1281)])
+@pytest.mark.parametrize("slope", [0.0, 0.02, -0.02])
+def test_long_shared_prefix(kind, b, n_q, n_kv, dk, dv, shared, slope):
+    """Many tiles per run of the tensor-core pass, with scores that keep rising (the accumulator is rescaled again and
+    again), that keep falling, or that do neither."""
+    s_max = shared + 20
+    q, v = _rand(b, n_q, dk, seed=b), _rand(b, n_kv, s_max, dv, seed=7)
+    k = _rand(b, n_kv, s_max, dk, seed=3) / 4
+    if slope:
+        q[:, :, 0], k[..., 0] = 1.0, (slope * torch.arange(s_max, device=DEV)).to(BF)
+    lens = [shared + i % 21 for i in range(b)]
+    got, kk, vv = _attend(kind, q, k, v, lens, shared, scale=1.0)
+    want, tol = _want(q, kk, vv, lens, shared, 1.0)
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() - tol).max())
+    assert float((got.double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
