@@ -22,9 +22,11 @@
 namespace sb {
 namespace {
 
-constexpr int kThreads = 128;                 // four warps, 16 positions of a tile each
-constexpr int kTile = 64;
-constexpr int kMaxCtas = 592;                 // 148 SMs, four CTAs each
+constexpr int kThreads = 128;                 // four warps, a quarter of a tile's positions each
+// Positions of a tile: a step of a warp is 32 quantised or 16 bf16 positions, 8 KB of heads of 128 either way.
+template <bool FP8> constexpr int kTile = FP8 ? 128 : 64;
+constexpr int kLeastTile = 64;
+constexpr int kMaxCtas = 444;                 // 148 SMs, three CTAs each
 
 // The line of tiles: first the shared positions (per key head and row tile), then
 // sequence by sequence, key head by key head, row tile by row tile.
@@ -32,8 +34,12 @@ __device__ __forceinline__ int seq_len(const Shape &s, const int32_t *seq_lens, 
 // A sequence that ends inside the shared positions does not take part in their common pass:
 // its own tiles are those positions, up to its end.
 __device__ __forceinline__ int own_begin(const Shape &s, int len) { return len >= s.shared_len ? s.shared_len : 0; }
-__device__ __forceinline__ int own_tiles(const Shape &s, int len) { return (len - own_begin(s, len) + kTile - 1) / kTile; }
-__device__ __forceinline__ int pre_tiles(const Shape &s) { return s.pre_row_tiles > 0 ? (s.shared_len + kTile - 1) / kTile : 0; }
+template <bool FP8> __device__ __forceinline__ int own_tiles(const Shape &s, int len) {
+  return (len - own_begin(s, len) + kTile<FP8> - 1) / kTile<FP8>;
+}
+template <bool FP8> __device__ __forceinline__ int pre_tiles(const Shape &s) {
+  return s.pre_row_tiles > 0 ? (s.shared_len + kTile<FP8> - 1) / kTile<FP8> : 0;
+}
 
 __device__ __forceinline__ int warp_sum_int(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
@@ -69,7 +75,7 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 
 // The state of one warp over a run of positions, NT * 8 query rows (row 8 nt + 2c + r in
-// registers [nt][.][r] of lanes with lane % 4 == c).
+// registers [nt][r] of lanes with lane % 4 == c), U * 16 positions a step.
 //
 // Quantised: the keys' codes become fp16 (exact) and so do the queries, each row scaled by a
 // power of two to a largest value in [1, 2) (bf16's eight bits fit; what falls below 2^-24 of the
@@ -82,54 +88,82 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 template <int DK, int DV, bool FP8, int NT>
 struct Stream {
   static constexpr int kBytes = FP8 ? 1 : 2;
+  static constexpr int U = FP8 ? 2 : 1;
   static constexpr int KP = DK * kBytes / 64;          // 16-byte pieces a lane holds of a key
   static constexpr int CPL = DV / 8;                   // value columns of a lane
   static constexpr int VW = CPL * kBytes / 4;          // 4-byte words a lane holds of a value
   static constexpr int MT = DV / 16;
+  static constexpr float kNone = -3.0e38f;             // the maximum of no score, or of scores of -inf alone
 
-  uint4 k[2][KP];
-  uint32_t v[4][VW];
-  uint32_t scale_bytes[4];                             // of keys g, g + 8, of values g, g + 8
+  uint4 k[U][2][KP];
+  uint32_t v[U][4][VW];
+  uint32_t k_scale, v_scale;                           // bytes of position `lane` of the step
   uint32_t q[NT][DK / 16][2];
   float q_factor[NT][2];
-  float m[NT][2], mv[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2];                            // running maximum (log2 units) and sum
+  float mv[NT][2], r_v[NT][2];                         // quantised: maximum of the weights, 2^(m - mv)
   float acc[MT][NT][4];
 
   // the value columns of a lane: column(e), e < CPL
   static __device__ __forceinline__ int column(int g, int e) { return FP8 ? g * CPL + e : (e >> 3) * 64 + g * 8 + (e & 7); }
 
-  __device__ __forceinline__ void load_k(const Cache &cache, size_t row0, size_t row_step, int key, int end, int g, int c) {
-    const unsigned char *base = static_cast<const unsigned char *>(cache.k);
+  // Where a lane reads: `kp` the first piece of its key of the step, `vp` the first word of its value.
+  struct Place {
+    const unsigned char *kp, *vp;
+    const uint8_t *ks, *vs;
+    size_t k_step, v_step;                             // bytes from a position to the next
+    int left;                                          // positions from the step's first one to the segment's end
+  };
+  __device__ __forceinline__ void load_k(const Place &at, int g, int c, int lane) {
+    if (at.left >= 16 * U) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int j = key + g + 8 * r;
-      const unsigned char *p = base + (row0 + (size_t)j * row_step) * (DK * kBytes) + c * 16;
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < KP; ++i) k[r][i] = j < end ? ldg_stream(p + i * 64) : make_uint4(0, 0, 0, 0);
-      if constexpr (FP8) {
-        scale_bytes[r] = j < end ? __ldg(cache.ks + row0 + j) : 0u;
-        scale_bytes[2 + r] = j < end ? __ldg(cache.vs + row0 + j) : 0u;
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int i = 0; i < KP; ++i) k[u][r][i] = ldg_stream(at.kp + (16 * u + 8 * r) * at.k_step + i * 64);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int i = 0; i < KP; ++i)
+            k[u][r][i] = 16 * u + 8 * r + g < at.left ? ldg_stream(at.kp + (16 * u + 8 * r) * at.k_step + i * 64)
+                                                      : make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (FP8) {
+      const bool in = lane < at.left;
+      k_scale = in ? __ldg(at.ks + lane) : 0u;
+      v_scale = in ? __ldg(at.vs + lane) : 0u;
+    }
+  }
+  __device__ __forceinline__ void load_v_row(const unsigned char *p, uint32_t (&x)[VW]) {
+    if constexpr (VW == 2) {
+      const uint2 y = ldg_stream8(p);
+      x[0] = y.x; x[1] = y.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < VW / 4; ++i) {
+        const uint4 y = ldg_stream(p + i * 128);
+        x[4 * i] = y.x; x[4 * i + 1] = y.y; x[4 * i + 2] = y.z; x[4 * i + 3] = y.w;
       }
     }
   }
   // positions behind the end give zeros, whatever stands there
-  __device__ __forceinline__ void load_v(const Cache &cache, size_t row0, size_t row_step, int key, int end, int g, int c) {
-    const unsigned char *base = static_cast<const unsigned char *>(cache.v);
+  __device__ __forceinline__ void load_v(const Place &at, int c) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = key + 2 * c + (r & 1) + 8 * (r >> 1);
-      const unsigned char *p = base + (row0 + (size_t)j * row_step) * (DV * kBytes) + g * (VW <= 4 ? VW * 4 : 16);
-      if constexpr (VW == 2) {
-        const uint2 x = j < end ? ldg_stream8(p) : make_uint2(0, 0);
-        v[r][0] = x.x; v[r][1] = x.y;
-      } else {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < VW / 4; ++i) {
-          const uint4 x = j < end ? ldg_stream(p + i * 128) : make_uint4(0, 0, 0, 0);
-          v[r][4 * i] = x.x; v[r][4 * i + 1] = x.y; v[r][4 * i + 2] = x.z; v[r][4 * i + 3] = x.w;
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * u + (r & 1) + 8 * (r >> 1);
+        if (at.left >= 16 * U || j + 2 * c < at.left) {
+          load_v_row(at.vp + j * at.v_step, v[u][r]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VW; ++i) v[u][r][i] = 0;
         }
       }
-    }
   }
 
   // Query rows g (+ 8) of a segment: `row(r)` is the address of row r, or null.
@@ -168,7 +202,8 @@ struct Stream {
       for (int r = 0; r < 2; ++r) {
         // (row 2c + r is held by lanes of group 2c + r)
         q_factor[nt][r] = __shfl_sync(0xffffffffu, factor, (2 * c + r) * 4) * scale_log2;
-        m[nt][r] = mv[nt][r] = -INFINITY;
+        m[nt][r] = mv[nt][r] = kNone;
+        r_v[nt][r] = 1.f;
         l[nt][r] = 0.f;
       }
     }
@@ -180,135 +215,176 @@ struct Stream {
         for (int i = 0; i < 4; ++i) acc[t][nt][i] = 0.f;
   }
 
-  __device__ __forceinline__ void scores(float (&s)[NT][4]) const {
+  // s[u][nt]: scores of keys 16u + g (elements 0, 1: rows 2c, 2c + 1) and 16u + g + 8 (2, 3)
+  __device__ __forceinline__ void scores(float (&s)[U][NT][4]) const {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int i = 0; i < KP; ++i) {
-      const uint32_t a[4] = {k[0][i].x, k[0][i].y, k[0][i].z, k[0][i].w}, b[4] = {k[1][i].x, k[1][i].y, k[1][i].z, k[1][i].w};
-      if constexpr (FP8) {
+        for (int i = 0; i < 4; ++i) s[u][nt][i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t a0 = e4m3x2_to_f16x2(a[w]), a2 = e4m3x2_to_f16x2(a[w] >> 16);
-          const uint32_t a1 = e4m3x2_to_f16x2(b[w]), a3 = e4m3x2_to_f16x2(b[w] >> 16);
+      for (int i = 0; i < KP; ++i) {
+        const uint32_t a[4] = {k[u][0][i].x, k[u][0][i].y, k[u][0][i].z, k[u][0][i].w};
+        const uint32_t b[4] = {k[u][1][i].x, k[u][1][i].y, k[u][1][i].z, k[u][1][i].w};
+        if constexpr (FP8) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<true>(s[nt], a0, a1, a2, a3, q[nt][i * 4 + w][0], q[nt][i * 4 + w][1]);
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a0 = e4m3x2_to_f16x2(a[w]), a2 = e4m3x2_to_f16x2(a[w] >> 16);
+            const uint32_t a1 = e4m3x2_to_f16x2(b[w]), a3 = e4m3x2_to_f16x2(b[w] >> 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<true>(s[u][nt], a0, a1, a2, a3, q[nt][i * 4 + w][0], q[nt][i * 4 + w][1]);
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<false>(s[u][nt], a[2 * w], b[2 * w], a[2 * w + 1], b[2 * w + 1], q[nt][i * 2 + w][0], q[nt][i * 2 + w][1]);
         }
-      } else {
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816<false>(s[nt], a[2 * w], b[2 * w], a[2 * w + 1], b[2 * w + 1], q[nt][i * 2 + w][0], q[nt][i * 2 + w][1]);
       }
     }
   }
 
-  // s: scores of keys g (elements 0, 1: rows 2c, 2c + 1) and g + 8 (2, 3) -> weights as the
-  // right-hand operand of the second product
-  __device__ __forceinline__ void weights(float (&s)[NT][4], const uint32_t (&bytes)[4], bool in0, bool in1, uint32_t (&w)[NT][2]) {
-    float u[NT][4];
-    bool over = false;
+  // Scores -> weights as the right-hand operand of the second product.  `left`: positions of
+  // the step that count.  Weights are worked out against the maxima as they stand; where one
+  // comes out above 2^kLazy (and in the first step) the maxima move and they are worked out again.
+  __device__ __forceinline__ void weights(float (&s)[U][NT][4], uint32_t k_byte, uint32_t v_byte, int left, int g,
+                                          uint32_t (&w)[U][NT][2]) {
+    float vs[U][2];
+    if constexpr (FP8) {
+      const float mine_k = e8m0_value(k_byte), mine_v = e8m0_value(v_byte);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = i < 2 ? in0 : in1;
-        float t = s[nt][i];
-        if constexpr (FP8) t *= e8m0_value(bytes[i >> 1]);
-        t *= q_factor[nt][i & 1];
-        s[nt][i] = in ? t : -INFINITY;
-        over |= s[nt][i] > m[nt][i & 1] + kLazy;
-        if constexpr (FP8) {
-          u[nt][i] = s[nt][i] + (bytes[2 + (i >> 1)] == kScaleNan ? NAN : (float)((int)bytes[2 + (i >> 1)] - 127));
-          if (!in) u[nt][i] = -INFINITY;
-          over |= u[nt][i] > mv[nt][i & 1] + kLazy;
+        for (int h = 0; h < 2; ++h) {
+          const float ks = __shfl_sync(0xffffffffu, mine_k, 16 * u + 8 * h + g);
+          vs[u][h] = __shfl_sync(0xffffffffu, mine_v, 16 * u + 8 * h + g);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) { s[u][nt][2 * h] *= ks; s[u][nt][2 * h + 1] *= ks; }
         }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][nt][i] *= q_factor[nt][i & 1];
+    if (left < 16 * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * u + 8 * (i >> 1) + g >= left) s[u][nt][i] = -INFINITY;
+    }
+    float p[U][NT][4], x[U][NT][4];
+    const auto exponentials = [&] {
+      bool over = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top[2] = {0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[u][nt][i] = exp2_approx(s[u][nt][i] - m[nt][i & 1]);
+            top[i & 1] = fmaxf(top[i & 1], p[u][nt][i]);
+            if constexpr (FP8) {
+              x[u][nt][i] = p[u][nt][i] * vs[u][i >> 1] * r_v[nt][i & 1];
+              top[i & 1] = fmaxf(top[i & 1], x[u][nt][i]);
+            }
+          }
+        over |= fmaxf(top[0], top[1]) > (float)(1 << (int)kLazy);
       }
-    if (__any_sync(0xffffffffu, over)) {
+      return over;
+    };
+    if (__any_sync(0xffffffffu, exponentials())) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float top = fmaxf(s[nt][r], s[nt][2 + r]), topv = FP8 ? fmaxf(u[nt][r], u[nt][2 + r]) : 0.f;
+          float top = kNone, topv = kNone;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              top = fmaxf(top, s[u][nt][2 * h + r]);
+              if constexpr (FP8) topv = fmaxf(topv, s[u][nt][2 * h + r] + log2f(vs[u][h]));
+            }
 #pragma unroll
           for (int off = 4; off <= 16; off <<= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
             if constexpr (FP8) topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, off));
           }
           top = fmaxf(top, m[nt][r]);
-          const float fl = m[nt][r] == -INFINITY ? 0.f : exp2_approx(m[nt][r] - top);
-          l[nt][r] *= fl;
+          float f = exp2_approx(m[nt][r] - top);
+          l[nt][r] *= f;
           m[nt][r] = top;
-          float fa = fl;
           if constexpr (FP8) {
             topv = fmaxf(topv, mv[nt][r]);
-            fa = mv[nt][r] == -INFINITY ? 0.f : exp2_approx(mv[nt][r] - topv);
+            f = exp2_approx(mv[nt][r] - topv);
             mv[nt][r] = topv;
+            r_v[nt][r] = exp2_approx(fminf(top - topv, 126.f));
           }
 #pragma unroll
-          for (int t = 0; t < MT; ++t) { acc[t][nt][r] *= fa; acc[t][nt][2 + r] *= fa; }
+          for (int t = 0; t < MT; ++t) { acc[t][nt][r] *= f; acc[t][nt][2 + r] *= f; }
         }
+      exponentials();
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // only scores of -inf so far: they weigh exp(-inf - 0) = 0
-        const float ref = m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1];
-        p[i] = exp2_approx(s[nt][i] - ref);
-        if constexpr (FP8) {
-          l[nt][i & 1] += p[i];
-          p[i] = exp2_approx(u[nt][i] - (mv[nt][i & 1] == -INFINITY ? 0.f : mv[nt][i & 1]));
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pair;
+          if constexpr (FP8) {
+            pair = pack_f16x2(x[u][nt][2 * h], x[u][nt][2 * h + 1]);
+            l[nt][0] += p[u][nt][2 * h];
+            l[nt][1] += p[u][nt][2 * h + 1];
+          } else {
+            pair = pack_bf16x2(p[u][nt][2 * h], p[u][nt][2 * h + 1]);
+            l[nt][0] += bf16_lo(pair);
+            l[nt][1] += bf16_hi(pair);
+          }
+          w[u][nt][h] = transpose8x8(pair);
         }
-      }
-      uint32_t w0, w1;
-      if constexpr (FP8) {
-        w0 = pack_f16x2(p[0], p[1]);
-        w1 = pack_f16x2(p[2], p[3]);
-      } else {
-        w0 = pack_bf16x2(p[0], p[1]);
-        w1 = pack_bf16x2(p[2], p[3]);
-        l[nt][0] += bf16_lo(w0) + bf16_lo(w1);
-        l[nt][1] += bf16_hi(w0) + bf16_hi(w1);
-      }
-      w[nt][0] = transpose8x8(w0);
-      w[nt][1] = transpose8x8(w1);
-    }
   }
 
-  __device__ __forceinline__ void values(const uint32_t (&w)[NT][2]) {
+  __device__ __forceinline__ void values(const uint32_t (&w)[U][NT][2]) {
 #pragma unroll
-    for (int i = 0; i < VW; ++i) {
-      if constexpr (FP8) {
-        // bytes of two neighbouring positions side by side, then both to fp16 at once
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362u : 0x5140u;
-          const uint32_t lo = __byte_perm(v[0][i], v[1][i], sel), hi = __byte_perm(v[2][i], v[3][i], sel);
-          const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
-          const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+      for (int i = 0; i < VW; ++i) {
+        if constexpr (FP8) {
+          // bytes of two neighbouring positions side by side, then both to fp16 at once
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<true>(acc[2 * i + half][nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362u : 0x5140u;
+            const uint32_t lo = __byte_perm(v[u][0][i], v[u][1][i], sel), hi = __byte_perm(v[u][2][i], v[u][3][i], sel);
+            const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(lo >> 16);
+            const uint32_t a2 = e4m3x2_to_f16x2(hi), a3 = e4m3x2_to_f16x2(hi >> 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<true>(acc[2 * i + half][nt], a0, a1, a2, a3, w[u][nt][0], w[u][nt][1]);
+          }
+        } else {
+          const uint32_t a0 = __byte_perm(v[u][0][i], v[u][1][i], 0x5410), a1 = __byte_perm(v[u][0][i], v[u][1][i], 0x7632);
+          const uint32_t a2 = __byte_perm(v[u][2][i], v[u][3][i], 0x5410), a3 = __byte_perm(v[u][2][i], v[u][3][i], 0x7632);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<false>(acc[i][nt], a0, a1, a2, a3, w[u][nt][0], w[u][nt][1]);
         }
-      } else {
-        const uint32_t a0 = __byte_perm(v[0][i], v[1][i], 0x5410), a1 = __byte_perm(v[0][i], v[1][i], 0x7632);
-        const uint32_t a2 = __byte_perm(v[2][i], v[3][i], 0x5410), a3 = __byte_perm(v[2][i], v[3][i], 0x7632);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<false>(acc[i][nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
       }
-    }
   }
 };
 
-// A run's place in the line of tiles.
+// A piece's place in the line of tiles.
+template <bool FP8>
 struct Cursor {
   int b;                              // sequence, -1: the shared positions
   int w;                              // key head * row tiles + row tile
-  int tile, tiles;                    // tile of the segment
+  int tile, tiles;                    // first tile of the piece in its segment, tiles of the segment
   int begin, end;                     // positions of the segment
   int row_tiles;
 
@@ -319,17 +395,14 @@ struct Cursor {
     const int len = b < 0 ? s.shared_len : seq_len(s, seq_lens, b);
     begin = b < 0 ? 0 : own_begin(s, len);
     end = len;
-    tiles = b < 0 ? pre_tiles(s) : own_tiles(s, len);
+    tiles = b < 0 ? pre_tiles<FP8>(s) : own_tiles<FP8>(s, len);
   }
-  // false: the next tile belongs to another segment
-  __device__ __forceinline__ bool next(const Shape &s, const int32_t *seq_lens) {
-    if (++tile < tiles) return true;
+  __device__ __forceinline__ void next_segment(const Shape &s, const int32_t *seq_lens) {
     tile = 0;
     if (++w == s.n_kv * row_tiles) {
       int n = b;
       do { enter(s, seq_lens, ++n); } while (tiles == 0 && n < s.B - 1);
     }
-    return false;
   }
   __device__ __forceinline__ int segment(const Shape &s) const {
     return b < 0 ? w : s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + w;
@@ -342,23 +415,26 @@ struct Cursor {
 // of the two grows), `rows` rows each: the row's attention over the piece, and the logarithm
 // (base 2) of its sum of exponentials.
 template <int DK, int DV, bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? (FP8 ? 4 : 3) : (FP8 ? 3 : 2))
+__global__ void __launch_bounds__(kThreads, NT == 1 && DK <= 128 ? 3 : 2)
 attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32_t *__restrict__ seq_lens, Shape s,
                    float *__restrict__ part, float *__restrict__ part_lse) {
+  using St = Stream<DK, DV, FP8, NT>;
+  constexpr int kStep = 16 * St::U;
+  static_assert(4 * kStep == kTile<FP8>, "four warps cover a tile");
   __shared__ float s_out[4][NT * 8][DV];
   __shared__ float s_lse[4][NT * 8];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   // this CTA's run: tiles first .. last-1 of the line
-  const int own_heads = s.n_kv * s.row_tiles, pre_line = s.n_kv * s.pre_row_tiles * pre_tiles(s);
+  const int own_heads = s.n_kv * s.row_tiles, pre_line = s.n_kv * s.pre_row_tiles * pre_tiles<FP8>(s);
   int sum = 0;
-  for (int b = lane; b < s.B; b += 32) sum += own_tiles(s, seq_len(s, seq_lens, b));
+  for (int b = lane; b < s.B; b += 32) sum += own_tiles<FP8>(s, seq_len(s, seq_lens, b));
   const int total = pre_line + own_heads * warp_sum_int(sum);
   const int share = (total + gridDim.x - 1) / gridDim.x;
   const int first = blockIdx.x * share, last = min(total, first + share);
   if (first >= last) return;
-  Cursor at;
+  Cursor<FP8> at;
   if (first < pre_line) {
     at.enter(s, seq_lens, -1);
     at.w = first / at.tiles;
@@ -366,12 +442,12 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
   } else {
     int before = pre_line, b0 = 0;
     for (; b0 + 32 < s.B; b0 += 32) {               // the 32 sequences among whose tiles the first one is
-      const int n = own_heads * warp_sum_int(b0 + lane < s.B ? own_tiles(s, seq_len(s, seq_lens, b0 + lane)) : 0);
+      const int n = own_heads * warp_sum_int(own_tiles<FP8>(s, seq_len(s, seq_lens, b0 + lane)));
       if (before + n > first) break;
       before += n;
     }
     for (; b0 + 1 < s.B; ++b0) {
-      const int n = own_heads * own_tiles(s, seq_len(s, seq_lens, b0));
+      const int n = own_heads * own_tiles<FP8>(s, seq_len(s, seq_lens, b0));
       if (before + n > first) break;
       before += n;
     }
@@ -380,15 +456,21 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
     at.tile = first - before - at.w * at.tiles;
   }
 
-  Stream<DK, DV, FP8, NT> st;
-  // row of position j in the cache: row0 + j * row_step
-  const size_t row_step = FP8 ? 1 : (size_t)s.n_kv;
-  const auto row0_of = [&](const Cursor &a) {
-    const int hk = a.w / a.row_tiles, home = a.home(s);
-    return FP8 ? ((size_t)home * s.n_kv + hk) * s.s_max : (size_t)home * s.s_max * s.n_kv + hk;
+  St st;
+  typename St::Place place;
+  place.k_step = (FP8 ? 1 : (size_t)s.n_kv) * (DK * St::kBytes);
+  place.v_step = (FP8 ? 1 : (size_t)s.n_kv) * (DV * St::kBytes);
+  const auto enter = [&](const Cursor<FP8> &a) {
+    const int hk = a.w / a.row_tiles, home = a.home(s), key = a.begin + a.tile * kTile<FP8> + warp * kStep;
+    // row of the step's first position in the cache
+    const size_t row = FP8 ? ((size_t)home * s.n_kv + hk) * s.s_max + key : ((size_t)home * s.s_max + key) * s.n_kv + hk;
+    place.kp = static_cast<const unsigned char *>(cache.k) + row * (DK * St::kBytes) + g * place.k_step + c * 16;
+    place.vp = static_cast<const unsigned char *>(cache.v) + row * (DV * St::kBytes) + 2 * c * place.v_step + g * (St::VW <= 4 ? St::VW * 4 : 16);
+    if constexpr (FP8) { place.ks = cache.ks + row; place.vs = cache.vs + row; }
+    place.left = a.end - key;
   };
   // query row r of the segment
-  const auto begin = [&](const Cursor &a) {
+  const auto begin = [&](const Cursor<FP8> &a) {
     const int hk = a.w / a.row_tiles, rt = a.w - hk * a.row_tiles;
     const int rows = a.b < 0 ? s.B * s.group : s.group;
     st.begin([&](int r) -> const __nv_bfloat16 * {
@@ -398,30 +480,35 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
       return q + b * s.q_stride + (size_t)(hk * s.group + h) * DK;
     }, s.scale_log2, g, c);
   };
-  size_t row0 = row0_of(at);
-  int key = at.begin + at.tile * kTile + warp * 16;
-  st.load_k(cache, row0, row_step, key, at.end, g, c);
-  st.load_v(cache, row0, row_step, key, at.end, g, c);
-  begin(at);
-  for (int t = first; t < last; ++t) {
-    float sc[NT][4];
-    uint32_t w[NT][2];
-    st.scores(sc);
-    const uint32_t bytes[4] = {st.scale_bytes[0], st.scale_bytes[1], st.scale_bytes[2], st.scale_bytes[3]};
-    const bool in0 = key + g < at.end, in1 = key + g + 8 < at.end;
-    const Cursor now = at;
-    const bool more = t + 1 < last;
-    bool same = false;
-    if (more) {
-      same = at.next(s, seq_lens);
-      if (!same) row0 = row0_of(at);
-      key = at.begin + at.tile * kTile + warp * 16;
-      st.load_k(cache, row0, row_step, key, at.end, g, c);
+  enter(at);
+  st.load_k(place, g, c, lane);
+  st.load_v(place, c);
+  for (int t = first; t < last;) {
+    // one piece: tiles of one segment
+    const Cursor<FP8> now = at;
+    const int piece_end = min(last, t + now.tiles - now.tile);
+    begin(now);
+    for (; t < piece_end; ++t) {
+      float sc[St::U][NT][4];
+      uint32_t w[St::U][NT][2];
+      st.scores(sc);
+      const uint32_t k_byte = st.k_scale, v_byte = st.v_scale;
+      const int left = place.left;
+      // the next step's keys are on their way during the rest of this one, its values during the next's first half
+      if (t + 1 < piece_end) {
+        place.kp += kTile<FP8> * place.k_step;
+        place.vp += kTile<FP8> * place.v_step;
+        if constexpr (FP8) { place.ks += kTile<FP8>; place.vs += kTile<FP8>; }
+        place.left -= kTile<FP8>;
+      } else if (t + 1 < last) {
+        at.next_segment(s, seq_lens);
+        enter(at);
+      }
+      if (t + 1 < last) st.load_k(place, g, c, lane);
+      st.weights(sc, k_byte, v_byte, left, g, w);
+      st.values(w);
+      if (t + 1 < last) st.load_v(place, c);
     }
-    st.weights(sc, bytes, in0, in1, w);
-    st.values(w);
-    if (more) st.load_v(cache, row0, row_step, key, at.end, g, c);
-    if (same) continue;
     // the end of a piece: the four warps' results joined, one partial result
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -439,7 +526,7 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
         for (int e = 0; e < DV / 8; ++e) s_out[warp][row][st.column(g, e)] = st.acc[e >> 1][nt][2 * (e & 1) + r] * f;
       }
     __syncthreads();
-    const int hk = now.w / now.row_tiles, rt = now.w - hk * now.row_tiles;
+    const int rt = now.w % now.row_tiles;
     const int rows = min(s.rows, (now.b < 0 ? s.B * s.group : s.group) - rt * s.rows);
     const size_t slot = (size_t)blockIdx.x + now.segment(s);
     for (int i = threadIdx.x; i < rows * DV; i += kThreads) {
@@ -457,59 +544,100 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
       if (col == 0) part_lse[slot * s.rows + row] = sum_w == 0.f ? -INFINITY : top + log2f(sum_w);
     }
     __syncthreads();
-    if (more) begin(at);
   }
 }
 
 // One CTA per (sequence, query head): its pieces of the shared positions and of its own,
-// weighted by their sums of exponentials.
-template <int DV>
+// weighted by their sums of exponentials.  The pieces' weights are worked out side by side
+// (kJoin of them a round), then every thread sums its column over loads that do not wait for
+// one another.
+constexpr int kJoin = 128;
+template <int DV, bool FP8>
 __global__ void __launch_bounds__(DV)
 attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, const float *__restrict__ part,
                  const float *__restrict__ part_lse, const float *__restrict__ pre_part, const float *__restrict__ pre_lse,
                  __nv_bfloat16 *__restrict__ out) {
   __shared__ int s_sum[2][DV / 32];
+  __shared__ float s_weight[kJoin], s_red[2][DV / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.x / s.n_q, h = blockIdx.x - b * s.n_q, hk = h / s.group, hg = h - hk * s.group;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int before = 0, all = 0;
   for (int i = threadIdx.x; i < s.B; i += DV) {
-    const int n = own_tiles(s, seq_len(s, seq_lens, i));
+    const int n = own_tiles<FP8>(s, seq_len(s, seq_lens, i));
     all += n;
     if (i < b) before += n;
   }
   before = warp_sum_int(before);
   all = warp_sum_int(all);
-  if ((threadIdx.x & 31) == 0) { s_sum[0][threadIdx.x >> 5] = before; s_sum[1][threadIdx.x >> 5] = all; }
+  if (lane == 0) { s_sum[0][warp] = before; s_sum[1][warp] = all; }
   __syncthreads();
   before = all = 0;
 #pragma unroll
   for (int w = 0; w < DV / 32; ++w) { before += s_sum[0][w]; all += s_sum[1][w]; }
-  const int own_heads = s.n_kv * s.row_tiles, pre_line = s.n_kv * s.pre_row_tiles * pre_tiles(s);
+  const int own_heads = s.n_kv * s.row_tiles, pre_line = s.n_kv * s.pre_row_tiles * pre_tiles<FP8>(s);
   const int total = pre_line + own_heads * all, share = (total + n_ctas - 1) / n_ctas;
   const int len = seq_len(s, seq_lens, b);
+  const bool prefix = s.shared_len > 0 && len >= s.shared_len;
   float top = -INFINITY, sum = 0.f, acc = 0.f;
-  const auto take = [&](const float *from, const float *from_lse, size_t slot_row) {
-    const float lse = from_lse[slot_row], o = from[slot_row * DV + threadIdx.x];
-    const float m = fmaxf(top, lse), ref = m == -INFINITY ? 0.f : m;
-    const float f = exp2_approx(top - ref), w = exp2_approx(lse - ref);
-    sum = sum * f + w;
-    acc = acc * f + w * o;
-    top = m;
+  // n pieces whose row i is first + i * step in `from`
+  const auto take = [&](const float *from, const float *from_lse, size_t first, size_t step, int n) {
+    for (int i0 = 0; i0 < n; i0 += kJoin) {
+      const int here = min(kJoin, n - i0);
+      float lse[kJoin / DV > 0 ? kJoin / DV : 1], most = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < (int)(sizeof(lse) / sizeof(float)); ++x) {
+        const int i = threadIdx.x + x * DV;
+        lse[x] = i < here ? from_lse[first + (i0 + i) * step] : -INFINITY;
+        most = fmaxf(most, lse[x]);
+      }
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+      if (lane == 0) s_red[0][warp] = most;
+      __syncthreads();
+      float up = top;
+#pragma unroll
+      for (int w = 0; w < DV / 32; ++w) up = fmaxf(up, s_red[0][w]);
+      const float ref = up == -INFINITY ? 0.f : up;
+      float part_sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < (int)(sizeof(lse) / sizeof(float)); ++x) {
+        const float w = exp2_approx(lse[x] - ref);
+        s_weight[threadIdx.x + x * DV] = w;
+        part_sum += w;
+      }
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, off);
+      if (lane == 0) s_red[1][warp] = part_sum;
+      __syncthreads();
+      const float f = exp2_approx(top - ref);
+      sum *= f;
+      acc *= f;
+#pragma unroll
+      for (int w = 0; w < DV / 32; ++w) sum += s_red[1][w];
+      const float *src = from + (first + i0 * step) * DV + threadIdx.x;
+#pragma unroll 8
+      for (int i = 0; i < here; ++i) acc += s_weight[i] * src[i * step * DV];
+      top = up;
+      __syncthreads();
+    }
   };
+  // (a segment's slots follow one another: CTA + segment)
   const auto pieces = [&](int first, int tiles, int segment, int row) {
-    for (int cta = first / share; cta <= (first + tiles - 1) / share; ++cta) take(part, part_lse, ((size_t)cta + segment) * s.rows + row);
+    const int cta = first / share;
+    take(part, part_lse, ((size_t)cta + segment) * s.rows + row, s.rows, (first + tiles - 1) / share - cta + 1);
   };
-  if (s.pre_splits > 0 && len >= s.shared_len) {
+  if (s.pre_splits > 0 && prefix) {
     const int r = b * s.group + hg, rt = r / kPrefixRows, rows = prefix_rows(s);
     const size_t slot = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * 2;
-    for (int i = 0; i < 2 * s.pre_splits; ++i) take(pre_part, pre_lse, (slot + i) * rows + r - rt * kPrefixRows);
-  } else if (pre_line > 0 && len >= s.shared_len) {
-    const int r = b * s.group + hg, rt = r / s.rows, n = pre_tiles(s);
+    take(pre_part, pre_lse, slot * rows + r - rt * kPrefixRows, rows, 2 * s.pre_splits);
+  } else if (pre_line > 0 && prefix) {
+    const int r = b * s.group + hg, rt = r / s.rows, n = pre_tiles<FP8>(s);
     const int seg = hk * s.pre_row_tiles + rt;
     pieces(seg * n, n, seg, r - rt * s.rows);
   }
-  const int n = own_tiles(s, len);
+  const int n = own_tiles<FP8>(s, len);
   if (n > 0) {
     const int rt = hg / s.rows, w = hk * s.row_tiles + rt;
     pieces(pre_line + own_heads * before + w * n, n, s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + w, hg - rt * s.rows);
@@ -543,15 +671,15 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
     if (rc != SB_OK) return rc;
   }
   const int sms = sb_device_sm_count() > 0 ? sb_device_sm_count() : 148;
-  // a CTA for every tile there can be, up to four per SM
-  const int64_t tiles = (int64_t)s.n_kv * ((int64_t)s.pre_row_tiles * ((s.shared_len + kTile - 1) / kTile) +
-                                           (int64_t)s.B * s.row_tiles * ((s.s_max + kTile - 1) / kTile));
-  const int most = 4 * sms < kMaxCtas ? 4 * sms : kMaxCtas;
+  // a CTA for every tile there can be, up to what the SMs hold at once
+  const int64_t tiles = (int64_t)s.n_kv * ((int64_t)s.pre_row_tiles * ((s.shared_len + kTile<FP8> - 1) / kTile<FP8>) +
+                                           (int64_t)s.B * s.row_tiles * ((s.s_max + kTile<FP8> - 1) / kTile<FP8>));
+  const int per_sm = s.rows <= 8 && DK <= 128 ? 3 : 2, most = per_sm * sms < kMaxCtas ? per_sm * sms : kMaxCtas;
   const int ctas = tiles < most ? (int)tiles : most;
   auto kern = s.rows <= 8 ? attn_stream_kernel<DK, DV, FP8, 1> : attn_stream_kernel<DK, DV, FP8, 2>;
   SB_CUDA_CHECK(launch_pdl(kern, dim3(ctas), dim3(kThreads), 0, st, q, cache, seq_lens, s, part, lse));
   SB_LAUNCH_CHECK();
-  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV>, dim3(s.B * s.n_q), dim3(DV), 0, st, seq_lens, s, ctas,
+  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3(s.B * s.n_q), dim3(DV), 0, st, seq_lens, s, ctas,
                            static_cast<const float *>(part), static_cast<const float *>(lse),
                            static_cast<const float *>(pre_part), static_cast<const float *>(pre_lse), out));
   SB_LAUNCH_CHECK();
@@ -564,7 +692,7 @@ int32_t attend(const char *name, const void *q, int64_t q_stride, Cache cache, c
                int32_t *status, void *stream) {
   // (the line's tiles are counted in 32 bits)
   if (B < 0 || n_q < 1 || n_kv < 1 || n_kv > 65535 || n_q % n_kv != 0 || s_max < 1 || shared_len < 0 || shared_len > s_max ||
-      (int64_t)B * n_q > (1 << 22) || (int64_t)B * n_q * (s_max / kTile + 2) > (1ll << 30))
+      (int64_t)B * n_q > (1 << 22) || (int64_t)B * n_q * (s_max / kLeastTile + 2) > (1ll << 30))
     return fail(SB_E_INVALID_ARG, "%s: bad shape (B=%d heads %d/%d s_max=%d shared %d)", name, B, n_q, n_kv, s_max, shared_len);
   if (!(scale >= 0.f) || !isfinite(scale)) return fail(SB_E_INVALID_ARG, "%s: scale must be finite and not negative", name);
   if (q_stride == 0) q_stride = (int64_t)n_q * dk;

@@ -16,8 +16,8 @@
 namespace sb {
 namespace {
 
-constexpr int kAppendThreads = 256;
-constexpr int kMaxHead = 256;                    // a row is at most one warp of 8-value vectors
+constexpr int kAppendThreads = 128;
+constexpr int kMaxHead = 256;                    // angles are kept for one CTA's threads
 constexpr int kMaxHalf = kMaxHead / 2;
 
 // theta^(-2j / rope_dim) / (2 pi), turns per position, as the sum of two floats
@@ -43,45 +43,62 @@ __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8]) {
   }
 }
 
-// Values e .. e+7 of a row whose first `rope` values are rotated: a vector of the first
-// half needs its partner of the second half and the other way round.
-template <bool VEC>
-__device__ __forceinline__ void load_rotated(const __nv_bfloat16 *rot, int e, int half, const float2 *table,
-                                             float (&x)[8]) {
-  float y[8];
-  const bool first = e < half;
-  const int j = first ? e : e - half;
-  load8<VEC>(rot + e, x);
-  load8<VEC>(rot + (first ? e + half : j), y);
+// A row is held by L lanes, two vectors of eight values each: a lane of the rotated part has
+// the two that are turned into one another, so both are loaded once and share their angles.
+struct RowPlace {
+  int e0, e1;                         // first elements of the two vectors
+  bool turned;
+};
+__device__ __forceinline__ RowPlace row_place(int lane, int half) {
+  const int pairs = half >> 3;
+  if (lane < pairs) return RowPlace{8 * lane, half + 8 * lane, true};
+  return RowPlace{16 * lane, 16 * lane + 8, false};
+}
+
+__device__ __forceinline__ void turn(float (&x)[8], float (&y)[8], const float2 *table, int pairs, int lane) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float2 cs = table[j + i];
-    x[i] = first ? x[i] * cs.x - y[i] * cs.y : x[i] * cs.x + y[i] * cs.y;
+    const float2 cs = table[i * pairs + lane];        // neighbouring lanes on neighbouring banks
+    const float a = x[i], b = y[i];
+    x[i] = a * cs.x - b * cs.y;
+    y[i] = b * cs.x + a * cs.y;
   }
 }
 
-// One row per group of L lanes, eight values a lane: codes and scale byte of the row.
-template <int L>
-__device__ __forceinline__ void store_codes(float (&x)[8], int e, int d, uint8_t *codes, uint8_t *scale) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-#pragma unroll
-  for (int off = L / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-  const uint32_t byte = e8m0_of_amax(top);
-  const float inv = e8m0_inverse(byte);
+__device__ __forceinline__ uint2 codes8(float (&x)[8], uint32_t byte, float inv) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= inv;
   if (byte == kScaleTop) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -kCodeTop), kCodeTop);
   }
-  uint2 c = make_uint2(0, 0);
-  if (byte != kScaleNan) c = make_uint2(e4m3x4(x[0], x[1], x[2], x[3]), e4m3x4(x[4], x[5], x[6], x[7]));
-  if (e < d && codes != nullptr) {
-    *reinterpret_cast<uint2 *>(codes + e) = c;
-    if (e == 0) *scale = (uint8_t)byte;
+  return make_uint2(e4m3x4(x[0], x[1], x[2], x[3]), e4m3x4(x[4], x[5], x[6], x[7]));
+}
+
+// Codes and scale byte of the row that L lanes hold; `scale` null: no row.
+template <int L>
+__device__ __forceinline__ void store_codes(float (&x)[8], float (&y)[8], RowPlace at, bool in, int lane, uint8_t *codes,
+                                            uint8_t *scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    top = max(top, max(__float_as_uint(x[i]) & 0x7fffffffu, __float_as_uint(y[i]) & 0x7fffffffu));
+#pragma unroll
+  for (int off = L / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const uint32_t byte = e8m0_of_amax(top);
+  const float inv = e8m0_inverse(byte);
+  uint2 c0 = codes8(x, byte, inv), c1 = codes8(y, byte, inv);
+  if (byte == kScaleNan) c0 = c1 = make_uint2(0, 0);
+  if (scale != nullptr && in) {
+    *reinterpret_cast<uint2 *>(codes + at.e0) = c0;
+    *reinterpret_cast<uint2 *>(codes + at.e1) = c1;
+    if (lane == 0) *scale = (uint8_t)byte;
   }
+}
+
+__device__ __forceinline__ void store_bf16(__nv_bfloat16 *p, const float (&x)[8]) {
+  *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                             pack_bf16x2(x[6], x[7]));
 }
 
 // grid = (tokens, shares of a token's rows).  A token's angles are worked out once per CTA:
@@ -99,53 +116,56 @@ rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource
   pdl_wait();
   const int t = blockIdx.x;
   const int pos = pos_of_token[t], seq = seq_of_token[t];
-  const int half = rope >> 1;
+  const int half = rope >> 1, pairs = half >> 3;
   if (threadIdx.x < half) {
     const float p = (float)pos, hi = freq.turns[threadIdx.x].x, lo = freq.turns[threadIdx.x].y;
     const float a = p * hi;
     const float turn = (a - rintf(a)) + (fmaf(p, hi, -a) + p * lo);
     float sn, cs;
     sincospif(2.f * turn, &sn, &cs);
-    table[threadIdx.x] = make_float2(cs, sn);
+    table[(threadIdx.x & 7) * pairs + (threadIdx.x >> 3)] = make_float2(cs, sn);
   }
   __syncthreads();
   const bool cached = pos >= 0 && pos < s_max && seq >= 0 && seq < B;
   const int rows = n_q + (cached ? 2 * n_kv : 0);
-  const int e = (threadIdx.x % L) * 8;
+  const int lane = threadIdx.x % L;
+  const RowPlace key_at = row_place(lane, half), value_at = row_place(lane, 0);
+  const bool in_key = lane * 16 < dk, in_value = lane * 16 < dv;
   constexpr int kRows = kAppendThreads / L;              // rows of a CTA in one turn
   // (all lanes of a warp take the same turns: the scale's reduction shuffles across a row)
   for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
     const int r = r0 + threadIdx.x / L;
-    float x[8];
+    float x[8], y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
     uint8_t *codes = nullptr, *scale = nullptr;
-    int d = dk;
-    if (r < n_q) {
-      if (e < rope) load_rotated<VEC>(q.at(t, r), e, half, table, x);
-      else if (e < dk) load8<VEC>(q.at(t, r) + e, x);
-      if (e < dk) {
-        uint32_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-        *reinterpret_cast<uint4 *>(q_out + ((size_t)t * n_q + r) * dk + e) = make_uint4(o[0], o[1], o[2], o[3]);
+    const bool value = r >= n_q + n_kv;
+    if (r < n_q + n_kv) {
+      if (in_key) {
+        const bool query = r < n_q;
+        // (an unrotated vector of a key stands in k_rest, rope elements further on than there)
+        const __nv_bfloat16 *src = query ? q.at(t, r) : key_at.turned ? k_rot.at(t, r - n_q) : k_rest.at(t, r - n_q) - rope;
+        load8<VEC>(src + key_at.e0, x);
+        load8<VEC>(src + key_at.e1, y);
+        if (key_at.turned) turn(x, y, table, pairs, lane);
+        if (query) {
+          __nv_bfloat16 *dst = q_out + ((size_t)t * n_q + r) * dk;
+          store_bf16(dst + key_at.e0, x);
+          store_bf16(dst + key_at.e1, y);
+        }
       }
-    } else if (r < rows) {
-      const int h = r - n_q < n_kv ? r - n_q : r - n_q - n_kv;
-      const size_t row = ((size_t)seq * n_kv + h) * s_max + pos;
-      if (r - n_q < n_kv) {
-        if (e < rope) load_rotated<VEC>(k_rot.at(t, h), e, half, table, x);
-        else if (e < dk) load8<VEC>(k_rest.at(t, h) + (e - rope), x);
-        codes = codes_k + row * dk;
-        scale = scale_k + row;
-      } else {
-        d = dv;
-        if (e < dv) load8<VEC>(v.at(t, h) + e, x);
-        codes = codes_v + row * dv;
-        scale = scale_v + row;
-      }
+    } else if (r < rows && in_value) {
+      const __nv_bfloat16 *src = v.at(t, r - n_q - n_kv);
+      load8<VEC>(src + value_at.e0, x);
+      load8<VEC>(src + value_at.e1, y);
     }
-    if (r0 + kRows > n_q) store_codes<L>(x, e, d, codes, scale);      // (the same for the whole CTA)
+    if (r0 + kRows <= n_q) continue;                     // (queries only; the same for the whole CTA)
+    if (r >= n_q && r < rows) {
+      const size_t row = ((size_t)seq * n_kv + (value ? r - n_q - n_kv : r - n_q)) * s_max + pos;
+      codes = value ? codes_v + row * dv : codes_k + row * dk;
+      scale = value ? scale_v + row : scale_k + row;
+    }
+    store_codes<L>(x, y, value ? value_at : key_at, value ? in_value : in_key, lane, codes, scale);
   }
 }
 
@@ -162,9 +182,10 @@ int32_t launch_append(bool vec, dim3 grid, cudaStream_t st, RowSource q, RowSour
   return SB_OK;
 }
 
-// grid = (shares of the positions, heads, sequences).  A position of a head is dk/16 + dv/16 vectors of
-// sixteen codes; a thread keeps its place in the row and walks over positions.
-constexpr int kReadThreads = 256;
+// grid = (shares of the positions, heads, sequences).  A position of a head is dk/8 + dv/8 vectors of
+// eight codes; a thread keeps its place in the row and walks over positions, kReadAhead of them
+// in flight.  Eight codes a thread, so that a warp's 16-byte stores are one run of bytes.
+constexpr int kReadThreads = 256, kReadAhead = 4;
 __global__ void __launch_bounds__(kReadThreads)
 cache_read_fp8_kernel(const uint8_t *__restrict__ codes_k, const uint8_t *__restrict__ scale_k,
                       const uint8_t *__restrict__ codes_v, const uint8_t *__restrict__ scale_v, int n_kv, int dk, int dv,
@@ -172,31 +193,40 @@ cache_read_fp8_kernel(const uint8_t *__restrict__ codes_k, const uint8_t *__rest
                       __nv_bfloat16 *__restrict__ out_v) {
   pdl_launch_dependents();
   pdl_wait();
-  const int per_row = (dk + dv) >> 4;
+  const int per_row = (dk + dv) >> 3;
   const int lane = threadIdx.x % per_row, step = kReadThreads / per_row;
   const int first = threadIdx.x / per_row;
   if (first >= step) return;                              // (threads left over where per_row does not divide the CTA)
   const int h = blockIdx.y, b = blockIdx.z;
-  const bool key = lane < (dk >> 4);
-  const int d = key ? dk : dv, e = (key ? lane : lane - (dk >> 4)) * 16;
+  const bool key = lane < (dk >> 3);
+  const int d = key ? dk : dv, e = (key ? lane : lane - (dk >> 3)) * 8;
   const uint8_t *codes = key ? codes_k : codes_v, *scales = key ? scale_k : scale_v;
   __nv_bfloat16 *dst = (key ? out_k : out_v) + ((size_t)b * n_kv + h) * count * d + e;
-  for (int i = blockIdx.x * step + first; i < count; i += gridDim.x * step) {
-    const int pos = begin + i;
-    const size_t row = ((size_t)(pos < shared_len ? 0 : b) * n_kv + h) * s_max + pos;
-    const uint4 c = __ldg(reinterpret_cast<const uint4 *>(codes + row * d + e));
-    const float scale = e8m0_value(__ldg(scales + row));
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    uint32_t o[8];
+  for (int i0 = blockIdx.x * step * kReadAhead + first; i0 < count; i0 += gridDim.x * step * kReadAhead) {
+    uint2 c[kReadAhead];
+    uint32_t byte[kReadAhead];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 lo = f16x2_to_float2(e4m3x2_to_f16x2(w[k])), hi = f16x2_to_float2(e4m3x2_to_f16x2(w[k] >> 16));
-      o[2 * k] = pack_bf16x2(lo.x * scale, lo.y * scale);
-      o[2 * k + 1] = pack_bf16x2(hi.x * scale, hi.y * scale);
+    for (int a = 0; a < kReadAhead; ++a) {
+      const int i = i0 + a * step, pos = begin + i;
+      c[a] = make_uint2(0, 0);
+      byte[a] = 0;
+      if (i < count) {
+        const size_t row = ((size_t)(pos < shared_len ? 0 : b) * n_kv + h) * s_max + pos;
+        c[a] = __ldg(reinterpret_cast<const uint2 *>(codes + row * d + e));
+        byte[a] = __ldg(scales + row);
+      }
     }
-    uint4 *p = reinterpret_cast<uint4 *>(dst + (size_t)i * d);
-    p[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+    for (int a = 0; a < kReadAhead; ++a) {
+      const int i = i0 + a * step;
+      const float scale = e8m0_value(byte[a]);
+      const float2 v0 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].x)), v1 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].x >> 16));
+      const float2 v2 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].y)), v3 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].y >> 16));
+      if (i < count)
+        *reinterpret_cast<uint4 *>(dst + (size_t)i * d) =
+            make_uint4(pack_bf16x2(v0.x * scale, v0.y * scale), pack_bf16x2(v1.x * scale, v1.y * scale),
+                       pack_bf16x2(v2.x * scale, v2.y * scale), pack_bf16x2(v3.x * scale, v3.y * scale));
+    }
   }
 }
 
@@ -238,14 +268,14 @@ int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest,
     freq.turns[j].y = (float)(turns - (double)freq.turns[j].x);
   }
   const int widest = dk > dv ? dk : dv;
-  const int lanes = widest <= 64 ? 8 : widest <= 128 ? 16 : 32;
+  const int lanes = widest <= 64 ? 4 : widest <= 128 ? 8 : 16;
   // at most two waves of CTAs: more would only repeat the angle table
   const int sms = sb_device_sm_count() > 0 ? sb_device_sm_count() : 148;
   const int wanted = ((n_q + 2 * n_kv) * lanes + kAppendThreads - 1) / kAppendThreads;
   const int room = (int)((2ll * sms + T - 1) / T);
   const dim3 grid(T, wanted < room ? wanted : room);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto launch = lanes == 8 ? launch_append<8> : lanes == 16 ? launch_append<16> : launch_append<32>;
+  auto launch = lanes == 4 ? launch_append<4> : lanes == 8 ? launch_append<8> : launch_append<16>;
   return launch(vec, grid, st, src[0], src[1], src[2], src[3], q_out, seq_of_token, pos_of_token, B, n_q, n_kv, dk, dv,
                 rope_dim, s_max, codes_k, scale_k, codes_v, scale_v, freq);
 }
@@ -262,11 +292,11 @@ int32_t sb_cache_read_fp8(const void *codes_k, const void *scale_k, const void *
     return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: null pointer");
   if (!aligned(codes_k, 16) || !aligned(codes_v, 16) || !aligned(out_k, 16) || !aligned(out_v, 16))
     return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: codes and outputs must be 16-byte aligned");
-  const int step = kReadThreads / ((dk + dv) >> 4);
+  const int step = kReadThreads / ((dk + dv) >> 3) * kReadAhead;
   const int wanted = (count + step - 1) / step;
   const int sms = sb_device_sm_count() > 0 ? sb_device_sm_count() : 148;
   const long long heads = (long long)B * n_kv;
-  const long long room = (64ll * sms + heads - 1) / heads;
+  const long long room = (32ll * sms + heads - 1) / heads;
   const dim3 grid((unsigned)(wanted < room ? wanted : room), n_kv, B);
   SB_CUDA_CHECK(launch_pdl(cache_read_fp8_kernel, grid, dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream),
                            static_cast<const uint8_t *>(codes_k), static_cast<const uint8_t *>(scale_k),
