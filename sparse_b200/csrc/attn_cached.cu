@@ -519,7 +519,7 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
         for (int off = 4; off <= 16; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
         const int row = nt * 8 + 2 * c + r;
         float f = 1.f / l;
-        if constexpr (FP8) f *= exp2_approx(st.mv[nt][r] - st.m[nt][r]);
+        if constexpr (FP8) f *= exp2f(st.mv[nt][r] - st.m[nt][r]);
         if (l == 0.f) f = 0.f;
         if (g == 0) s_lse[warp][row] = l == 0.f ? -INFINITY : st.m[nt][r] + log2f(l);
 #pragma unroll

@@ -36,9 +36,10 @@ int prefix_splits(const Shape &s);
 int32_t launch_attn_prefix(bool fp8, int dk, int dv, const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float *part,
                            float *lse, int32_t *status, cudaStream_t stream);
 
+// 2^x; results below 2^-126 are zero
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 

@@ -18,7 +18,7 @@
 // thread into bf16 operands, scale applied (exact), so the products are the bf16 ones.
 //
 // Probabilities are rounded to bf16 (2^-8), the type of the values that they are multiplied
-// with, and their sum is taken over the rounded ones; scores, sums and accumulators are fp32.
+// with; scores, their sums and the accumulators are fp32.
 //
 // All mbarrier waits are bounded; when one runs out the CTA raises its abort flag, reports
 // through `status`, waits for its copies and frees its TMEM.
@@ -116,6 +116,56 @@ __device__ __forceinline__ void convert16(const uint4 &c, float scale, uint4 &lo
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+constexpr float kNone = -3.0e38f;                // the maximum of no score, or of scores of -inf alone
+
+// 32 scores of a row from position x of its tile on; in the last tile (TAIL) those behind the last
+// shared position are -inf.
+template <bool TAIL>
+__device__ __forceinline__ void row_scores(uint32_t st_at, int x, int keys, uint32_t (&r)[32]) {
+  tc_ld32(st_at + x, r);
+  tc_wait_ld();
+  if constexpr (TAIL) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) r[e] = x + e < keys ? r[e] : 0xff800000u;
+  }
+}
+
+// The largest score of a row, kNone at least.
+template <bool TAIL>
+__device__ __forceinline__ float row_top(uint32_t st_at, int keys) {
+  float top[4] = {kNone, kNone, kNone, kNone};
+#pragma unroll
+  for (int x = 0; x < kKeys; x += 32) {
+    uint32_t r[32];
+    row_scores<TAIL>(st_at, x, keys, r);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      top[e & 3] = fmaxf(top[e & 3], fmaxf(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])));
+  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// A row's exponentials against the maximum `m` into TMEM, bf16 pairs over the scores (a pair is
+// stored behind the scores it replaces); returns their sum.
+template <bool TAIL>
+__device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float scale_log2, float m) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < kKeys; x += 32) {
+    uint32_t r[32], p[16];
+    row_scores<TAIL>(st_at, x, keys, r);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float a = exp2_approx(fmaf(__uint_as_float(r[2 * e]), scale_log2, -m));
+      const float b = exp2_approx(fmaf(__uint_as_float(r[2 * e + 1]), scale_log2, -m));
+      sum[e & 3] += a + b;
+      p[e] = pack_bf16x2(a, b);
+    }
+    tc_st16(st_at + x / 2, p);
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // grid = (runs of positions, row tiles, key heads)
@@ -256,30 +306,16 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int w = (warp - kSoftmaxWarp) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
     const uint32_t st_at = s_tmem + w * kKeys + lane_at, ot_at = o_tmem + w * DV + lane_at;
-    float m = -INFINITY, l = 0.f;
+    float m = kNone, l = 0.f;
     bool ok = true;
     for (int i = w; i < n; i += 2) {
       ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * w, (i >> 1) & 1, abort_flag));
       if (!ok) break;
       tc_fence_after();
       const int keys = min(kKeys, s.shared_len - (tile0 + i) * kKeys);
-      float top = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < kKeys; x += 32) {
-        uint32_t r[32];
-        tc_ld32(st_at + x, r);
-        tc_wait_ld();
-        if (x + 32 <= keys) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) top = x + e < keys ? fmaxf(top, __uint_as_float(r[e])) : top;
-        }
-      }
-      top *= s.scale_log2;
+      const float top = (keys == kKeys ? row_top<false>(st_at, keys) : row_top<true>(st_at, keys)) * s.scale_log2;
       if (__any_sync(0xffffffffu, top > m + kLazy)) {
-        const float up = fmaxf(m, top), f = m == -INFINITY ? 0.f : exp2_approx(m - up);
+        const float up = fmaxf(m, top), f = exp2_approx(m - up);
         l *= f;
         m = up;
         if (i >= 2) {                  // (the tile's scores are behind all earlier products: the accumulator is still)
@@ -297,25 +333,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           }
         }
       }
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int x = 0; x < kKeys; x += 32) {
-        uint32_t r[32], p[16];
-        tc_ld32(st_at + x, r);
-        tc_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float a = exp2_approx(fmaf(__uint_as_float(r[2 * e]), s.scale_log2, -ref));
-          float b = exp2_approx(fmaf(__uint_as_float(r[2 * e + 1]), s.scale_log2, -ref));
-          if (x + 32 > keys) {
-            if (x + 2 * e >= keys) a = 0.f;
-            if (x + 2 * e + 1 >= keys) b = 0.f;
-          }
-          p[e] = pack_bf16x2(a, b);
-          l += bf16_lo(p[e]) + bf16_hi(p[e]);
-        }
-        tc_st16(st_at + x / 2, p);
-      }
+      l += keys == kKeys ? exponentials<false>(st_at, keys, s.scale_log2, m) : exponentials<true>(st_at, keys, s.scale_log2, m);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -355,14 +373,23 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int row = (warp - kConvertWarp) * 32 + lane;
     const size_t row0 = (size_t)hk * s.s_max;
     const auto convert = [&](uint32_t src, uint32_t dst, int d, float scale, bool in) {
-      const int chunks = d / 16;
-      int chunk = row % chunks;
-      for (int x = 0; x < chunks; ++x, chunk = chunk + 1 == chunks ? 0 : chunk + 1) {
-        uint4 c = make_uint4(0, 0, 0, 0), lo, hi;
-        if (in) c = *reinterpret_cast<const uint4 *>(aligned_base + (src - base) + row * d + chunk * 16);
-        convert16(c, in ? scale : 0.f, lo, hi);
-        *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk)) = lo;
-        *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk + 1)) = hi;
+      const int chunks = d / 16, start = row % chunks;
+#pragma unroll
+      for (int x0 = 0; x0 < chunks; x0 += 4) {
+        uint4 c[4], lo, hi;
+        int chunk[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          chunk[x] = start + x0 + x < chunks ? start + x0 + x : start + x0 + x - chunks;
+          c[x] = in ? *reinterpret_cast<const uint4 *>(aligned_base + (src - base) + row * d + chunk[x] * 16)
+                    : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          convert16(c[x], in ? scale : 0.f, lo, hi);
+          *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk[x])) = lo;
+          *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk[x] + 1)) = hi;
+        }
       }
     };
     const auto scale_at = [&](const uint8_t *scales, int i) {
