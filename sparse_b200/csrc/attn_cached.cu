@@ -166,25 +166,44 @@ struct Stream {
       }
   }
 
-  // Query rows g (+ 8) of a segment: `row(r)` is the address of row r, or null.
+  // Query rows g (+ 8) of a segment into registers: `row(r)` is the address of row r, or null.  MMA
+  // step i takes four elements of a lane, those of its word(s) of the key's piece, so a lane's
+  // elements of a 64-byte key piece stand side by side in the query too.
   template <typename Row>
-  __device__ __forceinline__ void begin(const Row &row, float scale_log2, int g, int c) {
+  __device__ __forceinline__ void fetch(const Row &row, bool vec, int c) {
     constexpr int kPerPiece = 16 / kBytes;             // elements of a 16-byte piece of a key
+    const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const __nv_bfloat16 *src = row(nt * 8 + g);
+#pragma unroll
+      for (int i = 0; i < DK / 16; i += 2) {
+        // eight elements: the words of MMA steps i and i + 1
+        const __nv_bfloat16 *p = src + (i * 4 / kPerPiece) * (4 * kPerPiece) + c * kPerPiece + (i * 4) % kPerPiece;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (src != nullptr) {
+          if (vec) {
+            x = __ldg(reinterpret_cast<const uint4 *>(p));
+          } else {
+            const unsigned short *e = reinterpret_cast<const unsigned short *>(p);
+            x = make_uint4(e[0] | ((uint32_t)e[1] << 16), e[2] | ((uint32_t)e[3] << 16), e[4] | ((uint32_t)e[5] << 16),
+                           e[6] | ((uint32_t)e[7] << 16));
+          }
+        }
+        q[nt][i][0] = x.x; q[nt][i][1] = x.y; q[nt][i + 1][0] = x.z; q[nt][i + 1][1] = x.w;
+      }
+    }
+  }
+  // The rows just fetched, with nothing summed yet.
+  __device__ __forceinline__ void begin(float scale_log2, int c) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       uint32_t top = 0;
 #pragma unroll
-      for (int s = 0; s < DK / 16; ++s) {
+      for (int s = 0; s < DK / 16; ++s)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // MMA step s takes four elements of a lane: those of its word(s) of the key's piece
-          const int first = (s * 4 / kPerPiece) * (4 * kPerPiece) + c * kPerPiece + (s * 4) % kPerPiece + 2 * half;
-          const uint32_t lo = src ? __bfloat16_as_ushort(src[first]) : 0, hi = src ? __bfloat16_as_ushort(src[first + 1]) : 0;
-          q[nt][s][half] = lo | (hi << 16);
-          top = max(top, max(lo & 0x7fffu, hi & 0x7fffu));
-        }
-      }
+        for (int half = 0; half < 2; ++half)
+          top = max(top, max(q[nt][s][half] & 0x7fffu, (q[nt][s][half] >> 16) & 0x7fffu));
       float factor = 1.f;
       if constexpr (FP8) {
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -421,7 +440,7 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
   using St = Stream<DK, DV, FP8, NT>;
   constexpr int kStep = 16 * St::U;
   static_assert(4 * kStep == kTile<FP8>, "four warps cover a tile");
-  __shared__ float s_out[4][NT * 8][DV];
+  __shared__ __align__(16) float s_out[4][NT * 8][DV];
   __shared__ float s_lse[4][NT * 8];
   pdl_launch_dependents();
   pdl_wait();
@@ -470,15 +489,16 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
     place.left = a.end - key;
   };
   // query row r of the segment
-  const auto begin = [&](const Cursor<FP8> &a) {
+  const bool q_vec = s.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+  const auto fetch = [&](const Cursor<FP8> &a) {
     const int hk = a.w / a.row_tiles, rt = a.w - hk * a.row_tiles;
     const int rows = a.b < 0 ? s.B * s.group : s.group;
-    st.begin([&](int r) -> const __nv_bfloat16 * {
+    st.fetch([&](int r) -> const __nv_bfloat16 * {
       r += rt * s.rows;
       if (r >= rows || r >= (rt + 1) * s.rows) return nullptr;
       const int b = a.b < 0 ? r / s.group : a.b, h = a.b < 0 ? r - b * s.group : r;
       return q + b * s.q_stride + (size_t)(hk * s.group + h) * DK;
-    }, s.scale_log2, g, c);
+    }, q_vec, c);
   };
   enter(at);
   st.load_k(place, g, c, lane);
@@ -487,7 +507,8 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
     // one piece: tiles of one segment
     const Cursor<FP8> now = at;
     const int piece_end = min(last, t + now.tiles - now.tile);
-    begin(now);
+    fetch(now);
+    st.begin(s.scale_log2, c);
     for (; t < piece_end; ++t) {
       float sc[St::U][NT][4];
       uint32_t w[St::U][NT][2];
@@ -528,121 +549,128 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
     __syncthreads();
     const int rt = now.w % now.row_tiles;
     const int rows = min(s.rows, (now.b < 0 ? s.B * s.group : s.group) - rt * s.rows);
-    const size_t slot = (size_t)blockIdx.x + now.segment(s);
-    for (int i = threadIdx.x; i < rows * DV; i += kThreads) {
-      const int row = i / DV, col = i - row * DV;
-      float top = -INFINITY, sum_w = 0.f, o = 0.f;
+    const size_t slot_row = ((size_t)blockIdx.x + now.segment(s)) * s.rows;
+    constexpr int kCols = DV / 32;                       // columns of a lane
+    for (int row = warp; row < rows; row += 4) {
+      float lse[4], top = -INFINITY, total_w = 0.f, o[kCols];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) top = fmaxf(top, s_lse[x][row]);
+      for (int x = 0; x < 4; ++x) { lse[x] = s_lse[x][row]; top = fmaxf(top, lse[x]); }
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) o[e] = 0.f;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float lse = s_lse[x][row], f = lse == -INFINITY ? 0.f : exp2_approx(lse - top);
-        sum_w += f;
-        o += f * s_out[x][row][col];
+        const float f = exp2_approx(lse[x] - ref);
+        total_w += f;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) o[e] += f * s_out[x][row][lane * kCols + e];
       }
-      part[(slot * s.rows + row) * DV + col] = sum_w == 0.f ? 0.f : o / sum_w;
-      if (col == 0) part_lse[slot * s.rows + row] = sum_w == 0.f ? -INFINITY : top + log2f(sum_w);
+      const float f = total_w == 0.f ? 0.f : 1.f / total_w;
+      float *dst = part + (slot_row + row) * DV + lane * kCols;
+      if constexpr (kCols == 4) *reinterpret_cast<float4 *>(dst) = make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+      else *reinterpret_cast<float2 *>(dst) = make_float2(o[0] * f, o[1] * f);
+      if (lane == 0) part_lse[slot_row + row] = total_w == 0.f ? -INFINITY : top + log2f(total_w);
     }
     __syncthreads();
   }
 }
 
-// One CTA per (sequence, query head): its pieces of the shared positions and of its own,
-// weighted by their sums of exponentials.  The pieces' weights are worked out side by side
-// (kJoin of them a round), then every thread sums its column over loads that do not wait for
-// one another.
-constexpr int kJoin = 128;
+// One warp per (sequence, query head): its pieces of the shared positions and of its own,
+// weighted by their sums of exponentials.  A lane looks after one piece's weight and, then, after
+// its columns of all pieces, whose loads do not wait for one another.
+constexpr int kJoinWarps = 4;
 template <int DV, bool FP8>
-__global__ void __launch_bounds__(DV)
+__global__ void __launch_bounds__(kJoinWarps * 32)
 attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, const float *__restrict__ part,
                  const float *__restrict__ part_lse, const float *__restrict__ pre_part, const float *__restrict__ pre_lse,
                  __nv_bfloat16 *__restrict__ out) {
-  __shared__ int s_sum[2][DV / 32];
-  __shared__ float s_weight[kJoin], s_red[2][DV / 32];
+  constexpr int kCols = DV / 32;
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.x / s.n_q, h = blockIdx.x - b * s.n_q, hk = h / s.group, hg = h - hk * s.group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  if (row >= s.B * s.n_q) return;
+  const int b = row / s.n_q, h = row - b * s.n_q, hk = h / s.group, hg = h - hk * s.group;
   int before = 0, all = 0;
-  for (int i = threadIdx.x; i < s.B; i += DV) {
+  for (int i = lane; i < s.B; i += 32) {
     const int n = own_tiles<FP8>(s, seq_len(s, seq_lens, i));
     all += n;
     if (i < b) before += n;
   }
   before = warp_sum_int(before);
   all = warp_sum_int(all);
-  if (lane == 0) { s_sum[0][warp] = before; s_sum[1][warp] = all; }
-  __syncthreads();
-  before = all = 0;
-#pragma unroll
-  for (int w = 0; w < DV / 32; ++w) { before += s_sum[0][w]; all += s_sum[1][w]; }
   const int own_heads = s.n_kv * s.row_tiles, pre_line = s.n_kv * s.pre_row_tiles * pre_tiles<FP8>(s);
   const int total = pre_line + own_heads * all, share = (total + n_ctas - 1) / n_ctas;
   const int len = seq_len(s, seq_lens, b);
   const bool prefix = s.shared_len > 0 && len >= s.shared_len;
-  float top = -INFINITY, sum = 0.f, acc = 0.f;
-  // n pieces whose row i is first + i * step in `from`
-  const auto take = [&](const float *from, const float *from_lse, size_t first, size_t step, int n) {
-    for (int i0 = 0; i0 < n; i0 += kJoin) {
-      const int here = min(kJoin, n - i0);
-      float lse[kJoin / DV > 0 ? kJoin / DV : 1], most = -INFINITY;
+  float top = -INFINITY, sum = 0.f, acc[kCols];
 #pragma unroll
-      for (int x = 0; x < (int)(sizeof(lse) / sizeof(float)); ++x) {
-        const int i = threadIdx.x + x * DV;
-        lse[x] = i < here ? from_lse[first + (i0 + i) * step] : -INFINITY;
-        most = fmaxf(most, lse[x]);
-      }
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-      if (lane == 0) s_red[0][warp] = most;
-      __syncthreads();
-      float up = top;
-#pragma unroll
-      for (int w = 0; w < DV / 32; ++w) up = fmaxf(up, s_red[0][w]);
-      const float ref = up == -INFINITY ? 0.f : up;
-      float part_sum = 0.f;
-#pragma unroll
-      for (int x = 0; x < (int)(sizeof(lse) / sizeof(float)); ++x) {
-        const float w = exp2_approx(lse[x] - ref);
-        s_weight[threadIdx.x + x * DV] = w;
-        part_sum += w;
-      }
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, off);
-      if (lane == 0) s_red[1][warp] = part_sum;
-      __syncthreads();
-      const float f = exp2_approx(top - ref);
-      sum *= f;
-      acc *= f;
-#pragma unroll
-      for (int w = 0; w < DV / 32; ++w) sum += s_red[1][w];
-      const float *src = from + (first + i0 * step) * DV + threadIdx.x;
-#pragma unroll 8
-      for (int i = 0; i < here; ++i) acc += s_weight[i] * src[i * step * DV];
-      top = up;
-      __syncthreads();
-    }
-  };
-  // (a segment's slots follow one another: CTA + segment)
-  const auto pieces = [&](int first, int tiles, int segment, int row) {
+  for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
+  // Where the row's pieces are: of the shared positions, then (a segment's slots follow one
+  // another: CTA + segment) of its own.
+  const float *from[2] = {part, part}, *from_lse[2] = {part_lse, part_lse};
+  size_t first_row[2] = {0, 0}, step[2] = {(size_t)s.rows, (size_t)s.rows};
+  int n[2] = {0, 0};
+  const auto line = [&](int x, int first, int tiles, int segment, int r) {
     const int cta = first / share;
-    take(part, part_lse, ((size_t)cta + segment) * s.rows + row, s.rows, (first + tiles - 1) / share - cta + 1);
+    first_row[x] = ((size_t)cta + segment) * s.rows + r;
+    n[x] = (first + tiles - 1) / share - cta + 1;
   };
   if (s.pre_splits > 0 && prefix) {
-    const int r = b * s.group + hg, rt = r / kPrefixRows, rows = prefix_rows(s);
-    const size_t slot = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * 2;
-    take(pre_part, pre_lse, slot * rows + r - rt * kPrefixRows, rows, 2 * s.pre_splits);
+    const int r = b * s.group + hg, rt = r / kPrefixRows;
+    from[0] = pre_part;
+    from_lse[0] = pre_lse;
+    step[0] = prefix_rows(s);
+    first_row[0] = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * 2 * step[0] + r - rt * kPrefixRows;
+    n[0] = 2 * s.pre_splits;
   } else if (pre_line > 0 && prefix) {
-    const int r = b * s.group + hg, rt = r / s.rows, n = pre_tiles<FP8>(s);
-    const int seg = hk * s.pre_row_tiles + rt;
-    pieces(seg * n, n, seg, r - rt * s.rows);
+    const int r = b * s.group + hg, rt = r / s.rows, tiles = pre_tiles<FP8>(s), seg = hk * s.pre_row_tiles + rt;
+    line(0, seg * tiles, tiles, seg, r - rt * s.rows);
   }
-  const int n = own_tiles<FP8>(s, len);
-  if (n > 0) {
+  if (const int tiles = own_tiles<FP8>(s, len); tiles > 0) {
     const int rt = hg / s.rows, w = hk * s.row_tiles + rt;
-    pieces(pre_line + own_heads * before + w * n, n, s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + w, hg - rt * s.rows);
+    line(1, pre_line + own_heads * before + w * tiles, tiles, s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + w, hg - rt * s.rows);
   }
-  out[(size_t)blockIdx.x * DV + threadIdx.x] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
+  for (int i0 = 0; i0 < n[0] + n[1]; i0 += 32) {
+    const int here = min(32, n[0] + n[1] - i0), mine = i0 + lane, x = mine < n[0] ? 0 : 1;
+    const size_t at = first_row[x] + (mine - (x ? n[0] : 0)) * step[x];
+    const float lse = lane < here ? from_lse[x][at] : -INFINITY;
+    const float *mine_at = from[x] + at * DV;
+    float most = lse;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+    most = fmaxf(most, top);
+    const float ref = most == -INFINITY ? 0.f : most, f = exp2_approx(top - ref), w = exp2_approx(lse - ref);
+    float weights = w;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) weights += __shfl_xor_sync(0xffffffffu, weights, off);
+    sum = sum * f + weights;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) acc[e] *= f;
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), i)) + lane * kCols;
+      if constexpr (kCols == 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(src);
+        acc[0] += wi * v.x; acc[1] += wi * v.y; acc[2] += wi * v.z; acc[3] += wi * v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2 *>(src);
+        acc[0] += wi * v.x; acc[1] += wi * v.y;
+      }
+    }
+    top = most;
+  }
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  if (sum == 0.f) {
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
+  }
+  __nv_bfloat16 *dst = out + (size_t)row * DV + lane * kCols;
+#pragma unroll
+  for (int e = 0; e < kCols; e += 2) {
+    const uint32_t pair = pack_bf16x2(acc[e] * f, acc[e + 1] * f);
+    *reinterpret_cast<uint32_t *>(dst + e) = pair;
+  }
 }
 
 constexpr int kMaxRows = 16;
@@ -679,7 +707,7 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
   auto kern = s.rows <= 8 ? attn_stream_kernel<DK, DV, FP8, 1> : attn_stream_kernel<DK, DV, FP8, 2>;
   SB_CUDA_CHECK(launch_pdl(kern, dim3(ctas), dim3(kThreads), 0, st, q, cache, seq_lens, s, part, lse));
   SB_LAUNCH_CHECK();
-  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3(s.B * s.n_q), dim3(DV), 0, st, seq_lens, s, ctas,
+  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3((s.B * s.n_q + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, st, seq_lens, s, ctas,
                            static_cast<const float *>(part), static_cast<const float *>(lse),
                            static_cast<const float *>(pre_part), static_cast<const float *>(pre_lse), out));
   SB_LAUNCH_CHECK();
@@ -702,8 +730,8 @@ int32_t attend(const char *name, const void *q, int64_t q_stride, Cache cache, c
   if (B == 0) return SB_OK;
   if (!q || !cache.k || !cache.v || (FP8 && (!cache.ks || !cache.vs)) || !seq_lens || !ws || !out)
     return fail(SB_E_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(cache.k, 16) || !aligned(cache.v, 16) || !aligned(ws, 16))
-    return fail(SB_E_INVALID_ARG, "%s: cache and workspace must be 16-byte aligned", name);
+  if (!aligned(cache.k, 16) || !aligned(cache.v, 16) || !aligned(ws, 16) || !aligned(out, 4))
+    return fail(SB_E_INVALID_ARG, "%s: cache and workspace must be 16-byte aligned, out 4-byte", name);
   if (ws_bytes < sb_attn_cached_workspace_bytes(B, n_q, n_kv, dv, s_max, shared_len))
     return fail(SB_E_WORKSPACE, "%s: workspace too small", name);
   Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, q_stride, scale * 1.4426950408889634f};

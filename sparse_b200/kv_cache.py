@@ -21,12 +21,13 @@ class QuantizedCache:
     __slots__ = ("k", "k_scale", "v", "v_scale")
 
     def __init__(self, k: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor, v_scale: torch.Tensor):
-        if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or k_scale.shape != k.shape[:3] or (
-                v_scale.shape != k.shape[:3]):
+        rows = k.shape[:3]
+        if k.dim() != 4 or v.dim() != 4 or not rows == v.shape[:3] == k_scale.shape == v_scale.shape:
             raise RuntimeError("QuantizedCache: codes [B, n_kv, S, d] and scales [B, n_kv, S] do not fit: %s" % (
                 [tuple(t.shape) for t in (k, k_scale, v, v_scale)],))
+        device = k.device
         for t, dtype in ((k, CODES), (k_scale, SCALES), (v, CODES), (v_scale, SCALES)):
-            if t.dtype != dtype or t.device != k.device or not t.is_contiguous():
+            if t.dtype != dtype or t.device != device or not t.is_contiguous():
                 raise RuntimeError("QuantizedCache needs contiguous %s codes and %s scales on one device" % (CODES, SCALES))
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
 

@@ -200,21 +200,42 @@ def combine(rows_out: torch.Tensor, slot_of_item: torch.Tensor, idx: torch.Tenso
     return out
 
 
-def _rows3(t: torch.Tensor, what: str, like: torch.Tensor, heads, width: int) -> Tuple[int, int, int]:
-    """Address, token stride and head stride of a bf16 [T, heads, width] view (one head: shared)."""
-    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.device != like.device or t.shape[0] != like.shape[0] or (
-            t.shape[1] not in heads or t.shape[2] != width):
-        raise RuntimeError("rope_append_quantized: %s must be bf16 [%d, %s, %d] on %s, got %s %s on %s" % (
-            what, like.shape[0], " or ".join(map(str, heads)), width, like.device, t.dtype, tuple(t.shape), t.device))
-    if t.stride(2) != 1 and t.shape[2] > 1 and t.shape[0] > 0:
-        raise RuntimeError("rope_append_quantized: the elements of a head of %s must lie side by side" % what)
-    return t.data_ptr(), t.stride(0), t.stride(1) if t.shape[1] > 1 else 0
+# The calls of a decode step, of which a layer makes several and whose kernels take a few
+# microseconds: checks without tensor temporaries, the stream's handle without a Stream object, a
+# device guard only where another device is current.
+_Strides = ctypes.c_int64 * 8
 
 
-def _index(t: torch.Tensor, n: int, device: torch.device, what: str) -> int:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
-        raise RuntimeError("%s must be a contiguous int32 tensor of %d elements on %s" % (what, n, device))
+class _On:
+    """`with _On(index)`: that device is the current one."""
+    __slots__ = ("index", "guard")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        self.guard = None
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _index(t: torch.Tensor, n: int, device: int, what: str) -> int:
+    if t.dtype != torch.int32 or t.get_device() != device or t.shape != (n,) or not t.is_contiguous():
+        raise RuntimeError("%s must be a contiguous int32 tensor of %d elements on CUDA device %d" % (what, n, device))
     return t.data_ptr()
+
+
+def _cache_device(cache: QuantizedCache) -> int:
+    device = cache.k.get_device()
+    if device < 0:
+        raise RuntimeError("sparse_b200 ops need CUDA tensors (there is no CPU path)")
+    return device
 
 
 def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest: Optional[torch.Tensor],
@@ -227,31 +248,38 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
     (one head: shared by all), the rest k_rest [T, n_kv or 1, dk - r] (None where nothing is
     left, as k_rot where nothing is rotated); v [T, n_kv or 1, dv].  All are bf16 views with any
     token and head strides.  Token t goes to row (seq_of_token[t], pos_of_token[t]), int32; one
-    outside the cache is not stored."""
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.device != cache.device or not q.is_cuda:
-        raise RuntimeError("rope_append_quantized: q must be bf16 [T, n_q, dk] on the cache's CUDA device")
-    t, n_q, dk = q.shape
-    b, n_kv, s_max, dk_cache = cache.k.shape
+    outside the cache is not stored.  Two tokens of a call must not name the same row."""
+    device = _cache_device(cache)
+    b, n_kv, s_max, dk = cache.k.shape
     dv = cache.v.shape[3]
-    rope = k_rot.shape[-1] if k_rot is not None else 0
-    if dk != dk_cache or rope > dk or n_q < 1:
-        raise RuntimeError("rope_append_quantized: heads of %d and a cache of heads of %d" % (dk, dk_cache))
-    if (k_rest is None) != (rope == dk):
-        raise RuntimeError("rope_append_quantized: k_rest holds the %d unrotated elements of a key head" % (dk - rope))
-    strides, ptrs = [], []
-    for view, what, heads, width in ((q, "q", (n_q,), dk), (k_rot, "k_rot", (n_kv, 1), rope),
-                                     (k_rest, "k_rest", (n_kv, 1), dk - rope), (v, "v", (n_kv, 1), dv)):
-        ptr, token, head = _rows3(view, what, q, heads, width) if view is not None else (None, 0, 0)
-        ptrs.append(ptr)
-        strides += [token, head]
-    seq, pos = (_index(x, t, q.device, "rope_append_quantized: " + n) for x, n in
-                ((seq_of_token, "seq_of_token"), (pos_of_token, "pos_of_token")))
-    out = torch.empty((t, n_q, dk), dtype=torch.bfloat16, device=q.device)
-    with torch.cuda.device(q.device):
-        check(lib.sb_rope_append_fp8(*ptrs, seq, pos, t, b, n_q, n_kv, dk, dv, rope, theta, s_max,
-                                     (ctypes.c_int64 * 8)(*strides), out.data_ptr(), cache.k.data_ptr(),
-                                     cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), _stream(q)),
-              "sb_rope_append_fp8")
+    rope = 0 if k_rot is None else k_rot.shape[-1]
+    if q.dim() != 3 or q.shape[1] < 1 or q.shape[2] != dk or rope > dk or (k_rest is None) != (rope == dk):
+        raise RuntimeError("rope_append_quantized: q %s and a key of %d rotated and %s other elements for a cache of heads of %d"
+                           % (tuple(q.shape), rope, None if k_rest is None else k_rest.shape[-1], dk))
+    t, n_q, _ = q.shape
+    ptrs, strides = [], []
+    for view, heads, width in ((q, n_q, dk), (k_rot, n_kv, rope), (k_rest, n_kv, dk - rope), (v, n_kv, dv)):
+        if view is None:
+            ptrs.append(None)
+            strides += (0, 0)
+            continue
+        shape = view.shape
+        if (shape != (t, heads, width) and (shape != (t, 1, width) or view is q)) or view.dtype != torch.bfloat16 or (
+                view.get_device() != device):
+            raise RuntimeError("rope_append_quantized: needs bf16 [%d, %d or 1, %d] on the cache's device, got %s %s" % (
+                t, heads, width, view.dtype, tuple(shape)))
+        token, head, element = view.stride()
+        if element != 1 and t > 0:
+            raise RuntimeError("rope_append_quantized: the elements of a head must lie side by side")
+        ptrs.append(view.data_ptr())
+        strides += (token, head if shape[1] > 1 else 0)
+    seq = _index(seq_of_token, t, device, "rope_append_quantized: seq_of_token")
+    pos = _index(pos_of_token, t, device, "rope_append_quantized: pos_of_token")
+    out = q.new_empty((t, n_q, dk))
+    with _On(device) as stream:
+        check(lib.sb_rope_append_fp8(*ptrs, seq, pos, t, b, n_q, n_kv, dk, dv, rope, theta, s_max, _Strides(*strides),
+                                     out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
+                                     cache.v_scale.data_ptr(), stream), "sb_rope_append_fp8")
     return out
 
 
@@ -259,41 +287,46 @@ def cache_read(cache: QuantizedCache, begin: int, count: int, shared_len: int = 
     """Positions begin .. begin+count-1 of every sequence as bf16: (k [B, n_kv, count, dk],
     v [B, n_kv, count, dv]), exactly the values the codes stand for.  Positions below
     `shared_len` are sequence 0's."""
+    device = _cache_device(cache)
     b, n_kv, s_max, dk = cache.k.shape
     dv = cache.v.shape[3]
-    if not cache.k.is_cuda:
-        raise RuntimeError("sparse_b200 ops need CUDA tensors (there is no CPU path)")
     if begin < 0 or count < 0 or begin + count > s_max or not 0 <= shared_len <= s_max:
         raise RuntimeError("cache_read: positions %d .. %d, %d of them shared, of a cache of %d" % (
             begin, begin + count, shared_len, s_max))
-    k = torch.empty((b, n_kv, count, dk), dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty((b, n_kv, count, dv), dtype=torch.bfloat16, device=cache.device)
-    with torch.cuda.device(cache.device):
-        check(lib.sb_cache_read_fp8(_ptr(cache.k), _ptr(cache.k_scale), _ptr(cache.v), _ptr(cache.v_scale), b, n_kv, dk, dv,
-                                    s_max, begin, count, shared_len, k.data_ptr(), v.data_ptr(), _stream(k)),
+    k = cache.k.new_empty((b, n_kv, count, dk), dtype=torch.bfloat16)
+    v = cache.k.new_empty((b, n_kv, count, dv), dtype=torch.bfloat16)
+    with _On(device) as stream:
+        check(lib.sb_cache_read_fp8(cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(),
+                                    b, n_kv, dk, dv, s_max, begin, count, shared_len, k.data_ptr(), v.data_ptr(), stream),
               "sb_cache_read_fp8")
     return k, v
 
 
-def _attn_operands(name: str, q: torch.Tensor, seq_lens: torch.Tensor, batch: int, n_kv: int, dk: int, dv: int, s_max: int,
-                   shared_len: int, device: torch.device, status: Optional[torch.Tensor]):
-    """Checks; -> (seq_lens, status, output, workspace) of a decode attention call."""
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.device != device or not q.is_cuda or q.shape[0] != batch or (
-            q.shape[2] != dk or q.shape[1] < 1):
-        raise RuntimeError("%s: q must be bf16 [%d, n_q, %d] on the cache's CUDA device, got %s %s on %s" % (
-            name, batch, dk, q.dtype, tuple(q.shape), q.device))
-    if batch > 0 and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != dk)) or (
-            batch > 1 and q.stride(0) < q.shape[1] * dk):
+def _decode_attention(name: str, call, q: torch.Tensor, cache_ptrs, seq_lens: torch.Tensor, b: int, n_kv: int, dk: int,
+                      dv: int, s_max: int, shared_len: int, scale: Optional[float], status: Optional[torch.Tensor],
+                      device: int) -> torch.Tensor:
+    """Checks of the operands that both kinds of cache share, output and workspace, the call."""
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.get_device() != device or q.shape[0] != b or q.shape[2] != dk or (
+            q.shape[1] < 1):
+        raise RuntimeError("%s: q must be bf16 [%d, n_q, %d] on the cache's device, got %s %s on %s" % (
+            name, b, dk, q.dtype, tuple(q.shape), q.device))
+    n_q = q.shape[1]
+    seq_stride, head_stride, element = q.stride()
+    if b > 0 and (element != 1 or (n_q > 1 and head_stride != dk) or (b > 1 and seq_stride < n_q * dk)):
         raise RuntimeError("%s: the heads of a sequence's query must lie side by side, sequences apart" % name)
     if not 0 <= shared_len <= s_max:
         raise RuntimeError("%s: %d shared positions of a cache of %d" % (name, shared_len, s_max))
-    if status is not None and (status.dtype != torch.int32 or status.device != device):
-        raise RuntimeError("%s: status must be int32 on %s" % (name, device))
-    lens = _index(seq_lens, batch, device, name + ": seq_lens")
-    n_q = q.shape[1]
-    out = torch.empty((batch, n_q, dv), dtype=torch.bfloat16, device=device)
-    ws_bytes = lib.sb_attn_cached_workspace_bytes(batch, n_q, n_kv, dv, s_max, shared_len)
-    return lens, _ptr(status), out, torch.empty((max(ws_bytes, 16),), dtype=torch.uint8, device=device)
+    if status is not None and (status.dtype != torch.int32 or status.get_device() != device or status.numel() < 1):
+        raise RuntimeError("%s: status must be int32 on the cache's device" % name)
+    lens = _index(seq_lens, b, device, name)
+    out = q.new_empty((b, n_q, dv))
+    ws_bytes = lib.sb_attn_cached_workspace_bytes(b, n_q, n_kv, dv, s_max, shared_len) or 16
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
+    with _On(device) as stream:
+        check(call(q.data_ptr(), seq_stride if b > 1 else 0, *cache_ptrs, lens, b, n_q, n_kv, dk, dv, s_max, shared_len,
+                   dk ** -0.5 if scale is None else scale, ws.data_ptr(), ws_bytes, out.data_ptr(),
+                   None if status is None else status.data_ptr(), stream), name)
+    return out
 
 
 def attn_decode_quantized(q: torch.Tensor, cache: QuantizedCache, seq_lens: torch.Tensor, shared_len: int = 0,
@@ -303,17 +336,11 @@ def attn_decode_quantized(q: torch.Tensor, cache: QuantizedCache, seq_lens: torc
 
     n_q is a multiple of the cache's heads.  `shared_len`: as many first positions are the
     same for the whole batch and stand in sequence 0's rows; they are read once.  `scale`
-    defaults to dk ** -0.5; `status` as in `grouped_swiglu`."""
+    (at least 0) defaults to dk ** -0.5; `status` as in `grouped_swiglu`."""
     b, n_kv, s_max, dk = cache.k.shape
-    dv = cache.v.shape[3]
-    lens, st, out, ws = _attn_operands("attn_decode_quantized", q, seq_lens, b, n_kv, dk, dv, s_max, shared_len, cache.device,
-                                       status)
-    with torch.cuda.device(q.device):
-        check(lib.sb_attn_decode_fp8(q.data_ptr(), q.stride(0) if b > 1 else 0, _ptr(cache.k), _ptr(cache.k_scale),
-                                     _ptr(cache.v), _ptr(cache.v_scale), lens, b, q.shape[1], n_kv, dk, dv, s_max,
-                                     shared_len, dk ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(),
-                                     out.data_ptr(), st, _stream(q)), "sb_attn_decode_fp8")
-    return out
+    ptrs = (cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr())
+    return _decode_attention("attn_decode_quantized", lib.sb_attn_decode_fp8, q, ptrs, seq_lens, b, n_kv, dk, cache.v.shape[3],
+                             s_max, shared_len, scale, status, _cache_device(cache))
 
 
 def attn_decode_shared(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, seq_lens: torch.Tensor,
@@ -325,17 +352,12 @@ def attn_decode_shared(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Te
     if cache_k.dim() != 4 or cache_v.dim() != 4 or cache_k.shape[:3] != cache_v.shape[:3]:
         raise RuntimeError("attn_decode_shared: caches [B, S, n_kv, d] do not fit: %s and %s" % (
             tuple(cache_k.shape), tuple(cache_v.shape)))
-    if any(c.dtype != torch.bfloat16 or c.device != cache_k.device for c in (cache_k, cache_v)):
+    device = cache_k.get_device()
+    if cache_k.dtype != torch.bfloat16 or cache_v.dtype != torch.bfloat16 or cache_v.get_device() != device:
         raise RuntimeError("attn_decode_shared needs bf16 caches on one device")
     b, s_max, n_kv, dk = cache_k.shape
-    dv = cache_v.shape[3]
-    lens, st, out, ws = _attn_operands("attn_decode_shared", q, seq_lens, b, n_kv, dk, dv, s_max, shared_len, cache_k.device,
-                                       status)
-    with torch.cuda.device(q.device):
-        check(lib.sb_attn_decode_shared(q.data_ptr(), q.stride(0) if b > 1 else 0, _ptr(cache_k), _ptr(cache_v), lens, b,
-                                        q.shape[1], n_kv, dk, dv, s_max, shared_len, dk ** -0.5 if scale is None else scale,
-                                        ws.data_ptr(), ws.numel(), out.data_ptr(), st, _stream(q)), "sb_attn_decode_shared")
-    return out
+    return _decode_attention("attn_decode_shared", lib.sb_attn_decode_shared, q, (_ptr(cache_k), _ptr(cache_v)), seq_lens, b,
+                             n_kv, dk, cache_v.shape[3], s_max, shared_len, scale, status, device)
 
 
 def slot_copy_async(dst: torch.Tensor, src: torch.Tensor, stream: torch.cuda.Stream,
