@@ -166,33 +166,21 @@ struct Stream {
       }
   }
 
-  // Query rows g (+ 8) of a segment into registers: `row(r)` is the address of row r, or null.  MMA
-  // step i takes four elements of a lane, those of its word(s) of the key's piece, so a lane's
-  // elements of a 64-byte key piece stand side by side in the query too.
-  template <typename Row>
-  __device__ __forceinline__ void fetch(const Row &row, bool vec, int c) {
+  // Query rows g (+ 8) of `rows` from shared memory ([row][DK]).  MMA step i takes four elements of a
+  // lane, those of its word(s) of the key's piece, so a lane's elements of a 64-byte key piece
+  // stand side by side in the query too.
+  __device__ __forceinline__ void fetch(const __nv_bfloat16 *staged, int rows, int g, int c) {
     constexpr int kPerPiece = 16 / kBytes;             // elements of a 16-byte piece of a key
-    const int g = (threadIdx.x & 31) >> 2;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const __nv_bfloat16 *src = row(nt * 8 + g);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < DK / 16; i += 2) {
         // eight elements: the words of MMA steps i and i + 1
-        const __nv_bfloat16 *p = src + (i * 4 / kPerPiece) * (4 * kPerPiece) + c * kPerPiece + (i * 4) % kPerPiece;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (src != nullptr) {
-          if (vec) {
-            x = __ldg(reinterpret_cast<const uint4 *>(p));
-          } else {
-            const unsigned short *e = reinterpret_cast<const unsigned short *>(p);
-            x = make_uint4(e[0] | ((uint32_t)e[1] << 16), e[2] | ((uint32_t)e[3] << 16), e[4] | ((uint32_t)e[5] << 16),
-                           e[6] | ((uint32_t)e[7] << 16));
-          }
-        }
+        const int first = (i * 4 / kPerPiece) * (4 * kPerPiece) + c * kPerPiece + (i * 4) % kPerPiece;
+        const uint4 x = nt * 8 + g < rows ? *reinterpret_cast<const uint4 *>(staged + (nt * 8 + g) * DK + first)
+                                          : make_uint4(0, 0, 0, 0);
         q[nt][i][0] = x.x; q[nt][i][1] = x.y; q[nt][i + 1][0] = x.z; q[nt][i + 1][1] = x.w;
       }
-    }
   }
   // The rows just fetched, with nothing summed yet.
   __device__ __forceinline__ void begin(float scale_log2, int c) {
@@ -442,6 +430,7 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
   static_assert(4 * kStep == kTile<FP8>, "four warps cover a tile");
   __shared__ __align__(16) float s_out[4][NT * 8][DV];
   __shared__ float s_lse[4][NT * 8];
+  __shared__ __align__(16) __nv_bfloat16 s_q[2][NT * 8 * DK];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -488,26 +477,39 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
     if constexpr (FP8) { place.ks = cache.ks + row; place.vs = cache.vs + row; }
     place.left = a.end - key;
   };
-  // query row r of the segment
+  // The rows of a segment's queries on their way into shared memory, ahead of the piece.  Two
+  // buffers: a warp that runs ahead writes the next piece's while another reads this one's.
   const bool q_vec = s.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-  const auto fetch = [&](const Cursor<FP8> &a) {
-    const int hk = a.w / a.row_tiles, rt = a.w - hk * a.row_tiles;
-    const int rows = a.b < 0 ? s.B * s.group : s.group;
-    st.fetch([&](int r) -> const __nv_bfloat16 * {
-      r += rt * s.rows;
-      if (r >= rows || r >= (rt + 1) * s.rows) return nullptr;
-      const int b = a.b < 0 ? r / s.group : a.b, h = a.b < 0 ? r - b * s.group : r;
-      return q + b * s.q_stride + (size_t)(hk * s.group + h) * DK;
-    }, q_vec, c);
+  const auto rows_of = [&](const Cursor<FP8> &a) {
+    return min(s.rows, (a.b < 0 ? s.B * s.group : s.group) - a.w % a.row_tiles * s.rows);
   };
+  const auto stage = [&](const Cursor<FP8> &a, __nv_bfloat16 *dst) {
+    const int hk = a.w / a.row_tiles, r0 = (a.w - hk * a.row_tiles) * s.rows, rows = rows_of(a);
+    for (int i = threadIdx.x; i < rows * (DK / 8); i += kThreads) {
+      const int row = i / (DK / 8), e = (i - row * (DK / 8)) * 8, r = r0 + row;
+      const int b = a.b < 0 ? r / s.group : a.b, h = a.b < 0 ? r - b * s.group : r;
+      const __nv_bfloat16 *src = q + b * s.q_stride + (size_t)(hk * s.group + h) * DK + e;
+      if (q_vec) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                     ::"r"((uint32_t)__cvta_generic_to_shared(dst + row * DK + e)), "l"(src) : "memory");
+      } else {
+        for (int x = 0; x < 8; ++x) dst[row * DK + e + x] = src[x];
+      }
+    }
+  };
+  int buffer = 0;
+  stage(at, s_q[0]);
   enter(at);
   st.load_k(place, g, c, lane);
   st.load_v(place, c);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
   for (int t = first; t < last;) {
     // one piece: tiles of one segment
     const Cursor<FP8> now = at;
     const int piece_end = min(last, t + now.tiles - now.tile);
-    fetch(now);
+    st.fetch(s_q[buffer], rows_of(now), g, c);
+    buffer ^= 1;
     st.begin(s.scale_log2, c);
     for (; t < piece_end; ++t) {
       float sc[St::U][NT][4];
@@ -524,6 +526,7 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
       } else if (t + 1 < last) {
         at.next_segment(s, seq_lens);
         enter(at);
+        stage(at, s_q[buffer]);
       }
       if (t + 1 < last) st.load_k(place, g, c, lane);
       st.weights(sc, k_byte, v_byte, left, g, w);
@@ -543,12 +546,17 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
         if constexpr (FP8) f *= exp2f(st.mv[nt][r] - st.m[nt][r]);
         if (l == 0.f) f = 0.f;
         if (g == 0) s_lse[warp][row] = l == 0.f ? -INFINITY : st.m[nt][r] + log2f(l);
+        // (four columns at a time; the four rows that a warp writes together go to different banks)
+        float4 *dst = reinterpret_cast<float4 *>(s_out[warp][row]);
 #pragma unroll
-        for (int e = 0; e < DV / 8; ++e) s_out[warp][row][st.column(g, e)] = st.acc[e >> 1][nt][2 * (e & 1) + r] * f;
+        for (int e = 0; e < DV / 8; e += 4)
+          dst[(st.column(g, e) >> 2) ^ ((row >> 1) & 3)] =
+              make_float4(st.acc[e >> 1][nt][r] * f, st.acc[e >> 1][nt][2 + r] * f, st.acc[(e >> 1) + 1][nt][r] * f,
+                          st.acc[(e >> 1) + 1][nt][2 + r] * f);
       }
+    asm volatile("cp.async.wait_all;" ::: "memory");     // the next piece's queries
     __syncthreads();
-    const int rt = now.w % now.row_tiles;
-    const int rows = min(s.rows, (now.b < 0 ? s.B * s.group : s.group) - rt * s.rows);
+    const int rows = rows_of(now);
     const size_t slot_row = ((size_t)blockIdx.x + now.segment(s)) * s.rows;
     constexpr int kCols = DV / 32;                       // columns of a lane
     for (int row = warp; row < rows; row += 4) {
@@ -563,7 +571,8 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
         const float f = exp2_approx(lse[x] - ref);
         total_w += f;
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) o[e] += f * s_out[x][row][lane * kCols + e];
+        for (int e = 0; e < kCols; ++e)
+          o[e] += f * s_out[x][row][(((lane * kCols) >> 2) ^ ((row >> 1) & 3)) * 4 + ((lane * kCols + e) & 3)];
       }
       const float f = total_w == 0.f ? 0.f : 1.f / total_w;
       float *dst = part + (slot_row + row) * DV + lane * kCols;
@@ -575,9 +584,10 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
   }
 }
 
-// One warp per (sequence, query head): its pieces of the shared positions and of its own,
-// weighted by their sums of exponentials.  A lane looks after one piece's weight and, then, after
-// its columns of all pieces, whose loads do not wait for one another.
+// One CTA per (sequence, query head): its pieces of the shared positions and of its own, weighted
+// by their sums of exponentials.  A lane of each warp looks after one piece's weight; then the
+// four warps sum a quarter of the pieces each, a lane its columns, with loads that do not wait
+// for one another.
 constexpr int kJoinWarps = 4;
 template <int DV, bool FP8>
 __global__ void __launch_bounds__(kJoinWarps * 32)
@@ -585,10 +595,10 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
                  const float *__restrict__ part_lse, const float *__restrict__ pre_part, const float *__restrict__ pre_lse,
                  __nv_bfloat16 *__restrict__ out) {
   constexpr int kCols = DV / 32;
+  __shared__ __align__(8) float s_acc[kJoinWarps][DV];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
-  if (row >= s.B * s.n_q) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x;
   const int b = row / s.n_q, h = row - b * s.n_q, hk = h / s.group, hg = h - hk * s.group;
   int before = 0, all = 0;
   for (int i = lane; i < s.B; i += 32) {
@@ -620,8 +630,8 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
     from[0] = pre_part;
     from_lse[0] = pre_lse;
     step[0] = prefix_rows(s);
-    first_row[0] = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * 2 * step[0] + r - rt * kPrefixRows;
-    n[0] = 2 * s.pre_splits;
+    first_row[0] = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * step[0] + r - rt * kPrefixRows;
+    n[0] = s.pre_splits;
   } else if (pre_line > 0 && prefix) {
     const int r = b * s.group + hg, rt = r / s.rows, tiles = pre_tiles<FP8>(s), seg = hk * s.pre_row_tiles + rt;
     line(0, seg * tiles, tiles, seg, r - rt * s.rows);
@@ -647,7 +657,7 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
 #pragma unroll
     for (int e = 0; e < kCols; ++e) acc[e] *= f;
 #pragma unroll 8
-    for (int i = 0; i < here; ++i) {
+    for (int i = warp; i < here; i += kJoinWarps) {
       const float wi = __shfl_sync(0xffffffffu, w, i);
       const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), i)) + lane * kCols;
       if constexpr (kCols == 4) {
@@ -660,16 +670,19 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
     }
     top = most;
   }
-  const float f = sum == 0.f ? 0.f : 1.f / sum;
-  if (sum == 0.f) {
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
-  }
-  __nv_bfloat16 *dst = out + (size_t)row * DV + lane * kCols;
+  for (int e = 0; e < kCols; ++e) s_acc[warp][lane * kCols + e] = acc[e];
+  __syncthreads();
+  if (threadIdx.x < DV / 2) {
+    float2 o = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int e = 0; e < kCols; e += 2) {
-    const uint32_t pair = pack_bf16x2(acc[e] * f, acc[e + 1] * f);
-    *reinterpret_cast<uint32_t *>(dst + e) = pair;
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float2 x = *reinterpret_cast<const float2 *>(&s_acc[w][2 * threadIdx.x]);
+      o.x += x.x; o.y += x.y;
+    }
+    // no piece, or only such without weight: zeros
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint32_t *>(out + (size_t)row * DV + 2 * threadIdx.x) = sum == 0.f ? 0u : pack_bf16x2(o.x * f, o.y * f);
   }
 }
 
@@ -707,7 +720,7 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
   auto kern = s.rows <= 8 ? attn_stream_kernel<DK, DV, FP8, 1> : attn_stream_kernel<DK, DV, FP8, 2>;
   SB_CUDA_CHECK(launch_pdl(kern, dim3(ctas), dim3(kThreads), 0, st, q, cache, seq_lens, s, part, lse));
   SB_LAUNCH_CHECK();
-  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3((s.B * s.n_q + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, st, seq_lens, s, ctas,
+  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3(s.B * s.n_q), dim3(kJoinWarps * 32), 0, st, seq_lens, s, ctas,
                            static_cast<const float *>(part), static_cast<const float *>(lse),
                            static_cast<const float *>(pre_part), static_cast<const float *>(pre_lse), out));
   SB_LAUNCH_CHECK();

@@ -24,9 +24,9 @@ struct Shape {
 // sequence by sequence: row = b * group + h.
 constexpr int kPrefixRows = 128;
 __host__ __device__ inline int prefix_row_tiles(const Shape &s) { return (int)(((int64_t)s.B * s.group + kPrefixRows - 1) / kPrefixRows); }
-// Partial results of that kernel: two per CTA, of `prefix_rows` rows.
+// Partial results of that kernel: one per CTA, of `prefix_rows` rows.
 __host__ __device__ inline int prefix_rows(const Shape &s) { return s.B * (int64_t)s.group < kPrefixRows ? s.B * s.group : kPrefixRows; }
-inline int64_t prefix_slots(const Shape &s) { return (int64_t)s.n_kv * prefix_row_tiles(s) * s.pre_splits * 2; }
+inline int64_t prefix_slots(const Shape &s) { return (int64_t)s.n_kv * prefix_row_tiles(s) * s.pre_splits; }
 
 // Sizes for which the shared positions of a call are cut `splits` ways by attn_prefix_kernel.
 int prefix_splits(const Shape &s);

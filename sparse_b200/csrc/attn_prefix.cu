@@ -339,34 +339,54 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + 8 * w);
     }
-    // this group's partial result; without a tile, or with an empty row, nothing that weighs
-    const size_t slot = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * 2 + w;
-    const int slot_rows = prefix_rows(s);
-    const bool any = w < n;
-    if (ok && any) {
-      ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * w, 0, abort_flag));
-      tc_fence_after();
-    }
-    if (ok) {
-      const float f = l == 0.f ? 0.f : 1.f / l;
-      float *dst = part + (slot * slot_rows + row) * DV;
+    // The two groups' results become one: weights from both sums, this group's rows scaled by its
+    // own, the second group's added to the first's through shared memory (every product is done,
+    // so the operands' place is free), whole rows written.
+    ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full, 0, abort_flag) && (n < 2 || mbar_wait(o_full + 8, 0, abort_flag)));
+    tc_fence_after();
+    float2 *sums = reinterpret_cast<float2 *>(aligned_base);                             // [2][128], over the queries
+    float *rows_at = reinterpret_cast<float *>(aligned_base + L::kQ);                    // [128][DV + 4], over keys and values
+    static_assert(kPrefixRows * (DV + 4) * 4 <= L::kBytes - L::kQ, "room for the accumulators");
+    sums[w * kPrefixRows + row] = make_float2(m, l);
+    const auto groups_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    groups_sync();
+    const float2 other = sums[(w ^ 1) * kPrefixRows + row];
+    const float most = fmaxf(m, other.x), mine = exp2_approx(m - most), sum = l * mine + other.y * exp2_approx(other.x - most);
+    const float f = sum == 0.f ? 0.f : mine / sum;
+    float4 *slot_at = reinterpret_cast<float4 *>(rows_at + row * (DV + 4));
+    for (int turn = 1; turn >= 0; --turn) {
+      if (turn == w) {
 #pragma unroll
-      for (int x = 0; x < DV; x += 32) {
-        uint32_t r[32];
-        tc_ld32(ot_at + x, r);
-        tc_wait_ld();
-        if (row < rows) {
+        for (int x = 0; x < DV; x += 32) {
+          uint32_t r[32];
+          tc_ld32(ot_at + x, r);
+          tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4 *>(dst + x + e) =
-                any && l != 0.f ? make_float4(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f,
-                                              __uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int e = 0; e < 32; e += 4) {
+            // (a group without a tile has nothing in its accumulator)
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (w < n && sum != 0.f)
+              o = make_float4(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f, __uint_as_float(r[e + 2]) * f,
+                              __uint_as_float(r[e + 3]) * f);
+            if (w == 0) {
+              const float4 t = slot_at[(x + e) / 4];
+              o = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
+            }
+            slot_at[(x + e) / 4] = o;
+          }
         }
       }
-      if (row < rows) part_lse[slot * slot_rows + row] = l == 0.f ? -INFINITY : m + log2f(l);
-      tc_fence_before();
+      groups_sync();
     }
+    if (ok) {
+      const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * prefix_rows(s);
+      for (int i = threadIdx.x - kSoftmaxWarp * 32; i < rows * (DV / 4); i += 256) {
+        const int r = i / (DV / 4), col = i - r * (DV / 4);
+        *reinterpret_cast<float4 *>(part + (slot_row + r) * DV + col * 4) = *reinterpret_cast<const float4 *>(rows_at + r * (DV + 4) + col * 4);
+      }
+      if (w == 0 && row < rows) part_lse[slot_row + row] = sum == 0.f ? -INFINITY : most + log2f(sum);
+    }
+    tc_fence_before();
   } else if (FP8 && warp >= kConvertWarp) {
     // one row of codes per thread, its chunks in an order that keeps eight neighbouring rows
     // on different banks, in the codes and in the swizzled operand
