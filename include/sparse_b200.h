@@ -666,7 +666,8 @@ int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest,
 int32_t sb_cache_read_fp8(const void *codes_k, const void *scale_k, const void *codes_v, const void *scale_v, int32_t B,
                           int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max, int32_t begin, int32_t count,
                           int32_t shared_len, void *out_k, void *out_v, void *stream);
-size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t dv, int32_t s_max, int32_t shared_len);
+size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max,
+                                      int32_t shared_len);
 int32_t sb_attn_decode_fp8(const void *q, int64_t q_stride, const void *codes_k, const void *scale_k, const void *codes_v,
                            const void *scale_v, const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk,
                            int32_t dv, int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,

@@ -103,7 +103,7 @@ SIGNATURES: Dict[str, Tuple[object, list]] = {
     "sb_rope_append_fp8": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, i32,
                                  C.POINTER(i64), vp, vp, vp, vp, vp, vp]),
     "sb_cache_read_fp8": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
-    "sb_attn_cached_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+    "sb_attn_cached_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
     "sb_attn_decode_fp8": (i32, [vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, sz, vp, vp,
                                  vp]),
     "sb_attn_decode_shared": (i32, [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, sz, vp, vp, vp]),

@@ -41,6 +41,16 @@ template <bool FP8> __device__ __forceinline__ int pre_tiles(const Shape &s) {
   return s.pre_row_tiles > 0 ? (s.shared_len + kTile<FP8> - 1) / kTile<FP8> : 0;
 }
 
+// The line in equal runs: the first `longer` CTAs have one tile more than the others.
+struct Runs {
+  int least, longer;
+  __device__ __forceinline__ int first(int cta) const { return cta * least + min(cta, longer); }
+  __device__ __forceinline__ int cta_of(int tile) const {
+    const int head = longer * (least + 1);
+    return tile < head ? tile / (least + 1) : longer + (tile - head) / least;
+  }
+};
+
 __device__ __forceinline__ int warp_sum_int(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
 // ---- loads and fragments --------------------------------------------------------------------
@@ -439,8 +449,8 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
   int sum = 0;
   for (int b = lane; b < s.B; b += 32) sum += own_tiles<FP8>(s, seq_len(s, seq_lens, b));
   const int total = pre_line + own_heads * warp_sum_int(sum);
-  const int share = (total + gridDim.x - 1) / gridDim.x;
-  const int first = blockIdx.x * share, last = min(total, first + share);
+  const Runs runs{total / (int)gridDim.x, total % (int)gridDim.x};
+  const int first = runs.first(blockIdx.x), last = runs.first(blockIdx.x + 1);
   if (first >= last) return;
   Cursor<FP8> at;
   if (first < pre_line) {
@@ -609,7 +619,8 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
   before = warp_sum_int(before);
   all = warp_sum_int(all);
   const int own_heads = s.n_kv * s.row_tiles, pre_line = s.n_kv * s.pre_row_tiles * pre_tiles<FP8>(s);
-  const int total = pre_line + own_heads * all, share = (total + n_ctas - 1) / n_ctas;
+  const int total = pre_line + own_heads * all;
+  const Runs runs{total / n_ctas, total % n_ctas};
   const int len = seq_len(s, seq_lens, b);
   const bool prefix = s.shared_len > 0 && len >= s.shared_len;
   float top = -INFINITY, sum = 0.f, acc[kCols];
@@ -621,16 +632,16 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
   size_t first_row[2] = {0, 0}, step[2] = {(size_t)s.rows, (size_t)s.rows};
   int n[2] = {0, 0};
   const auto line = [&](int x, int first, int tiles, int segment, int r) {
-    const int cta = first / share;
+    const int cta = runs.cta_of(first);
     first_row[x] = ((size_t)cta + segment) * s.rows + r;
-    n[x] = (first + tiles - 1) / share - cta + 1;
+    n[x] = runs.cta_of(first + tiles - 1) - cta + 1;
   };
   if (s.pre_splits > 0 && prefix) {
-    const int r = b * s.group + hg, rt = r / kPrefixRows;
+    const int r = b * s.group + hg, rt = r / s.pre_tile_rows;
     from[0] = pre_part;
     from_lse[0] = pre_lse;
     step[0] = prefix_rows(s);
-    first_row[0] = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * step[0] + r - rt * kPrefixRows;
+    first_row[0] = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * step[0] + r - rt * s.pre_tile_rows;
     n[0] = s.pre_splits;
   } else if (pre_line > 0 && prefix) {
     const int r = b * s.group + hg, rt = r / s.rows, tiles = pre_tiles<FP8>(s), seg = hk * s.pre_row_tiles + rt;
@@ -690,9 +701,11 @@ constexpr int kMaxRows = 16;
 
 // How a call is cut; the rest of the shape is the caller's.  Up to sixteen rows share one
 // pass of the streamed line over the prefix, more go through the tensor-core tiles.
-void plan(Shape &s) {
+void plan(Shape &s, int dk) {
   const int64_t pre_rows = s.shared_len > 0 ? (int64_t)s.B * s.group : 0;
-  s.pre_splits = pre_rows > kMaxRows ? prefix_splits(s) : 0;
+  s.pre_splits = 0;
+  s.pre_tile_rows = 1;
+  if (pre_rows > kMaxRows) plan_prefix(s, dk);
   s.rows = s.group > kMaxRows ? kMaxRows : s.group;
   if (pre_rows > s.rows && s.pre_splits == 0) s.rows = (int)pre_rows;
   s.row_tiles = (s.group + s.rows - 1) / s.rows;
@@ -701,7 +714,7 @@ void plan(Shape &s) {
 // Partial results: of the streamed line, then of the shared positions' tiles; outputs first,
 // then logarithms.
 int64_t slot_rows(const Shape &s) { return (kMaxCtas + (int64_t)s.n_kv * (s.pre_row_tiles + (int64_t)s.B * s.row_tiles)) * s.rows; }
-int64_t pre_slot_rows(const Shape &s) { return prefix_slots(s) * prefix_rows(s); }
+int64_t pre_slot_rows(const Shape &s) { return s.pre_splits > 0 ? prefix_slots(s) * prefix_rows(s) : 0; }
 
 template <int DK, int DV, bool FP8>
 int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_lens, const Shape &s, float *part,
@@ -745,10 +758,10 @@ int32_t attend(const char *name, const void *q, int64_t q_stride, Cache cache, c
     return fail(SB_E_INVALID_ARG, "%s: null pointer", name);
   if (!aligned(cache.k, 16) || !aligned(cache.v, 16) || !aligned(ws, 16) || !aligned(out, 4))
     return fail(SB_E_INVALID_ARG, "%s: cache and workspace must be 16-byte aligned, out 4-byte", name);
-  if (ws_bytes < sb_attn_cached_workspace_bytes(B, n_q, n_kv, dv, s_max, shared_len))
+  if (ws_bytes < sb_attn_cached_workspace_bytes(B, n_q, n_kv, dk, dv, s_max, shared_len))
     return fail(SB_E_WORKSPACE, "%s: workspace too small", name);
-  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, q_stride, scale * 1.4426950408889634f};
-  plan(s);
+  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, q_stride, scale * 1.4426950408889634f};
+  plan(s, dk);
   const __nv_bfloat16 *qq = static_cast<const __nv_bfloat16 *>(q);
   float *part = static_cast<float *>(ws);
   __nv_bfloat16 *oo = static_cast<__nv_bfloat16 *>(out);
@@ -765,11 +778,12 @@ using namespace sb;
 
 extern "C" {
 
-size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t dv, int32_t s_max, int32_t shared_len) {
-  if (B < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || dv < 1 || s_max < 1 || shared_len < 0 || (int64_t)B * n_q > (1 << 22))
+size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max,
+                                      int32_t shared_len) {
+  if (B < 0 || dk < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || dv < 1 || s_max < 1 || shared_len < 0 || (int64_t)B * n_q > (1 << 22))
     return 0;
-  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, 0.f};
-  plan(s);
+  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, 0, 0.f};
+  plan(s, dk);
   return (size_t)(slot_rows(s) + pre_slot_rows(s)) * (dv + 1) * sizeof(float);
 }
 

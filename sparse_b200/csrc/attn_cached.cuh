@@ -15,21 +15,23 @@ struct Shape {
   int s_max, shared_len;
   int rows;                           // query rows of a segment of the streamed line (at most 16)
   int row_tiles, pre_row_tiles;       // its segments per key head: of a sequence, and of the shared positions
-  int pre_splits;                     // > 0: the shared positions go through attn_prefix_kernel, cut in so many
+  int pre_splits, pre_tile_rows;      // pre_splits > 0: the shared positions go through attn_prefix_kernel, cut in so many
   int64_t q_stride;
   float scale_log2;                   // scale * log2(e), >= 0
 };
 
-// Query rows of one tile of attn_prefix_kernel.  The rows of a key head are numbered
-// sequence by sequence: row = b * group + h.
+// attn_prefix_kernel takes the rows of a key head, numbered sequence by sequence (row = b * group
+// + h), in tiles of 128, or of two times 128.
 constexpr int kPrefixRows = 128;
-__host__ __device__ inline int prefix_row_tiles(const Shape &s) { return (int)(((int64_t)s.B * s.group + kPrefixRows - 1) / kPrefixRows); }
+__host__ __device__ inline int prefix_row_tiles(const Shape &s) {
+  return (int)(((int64_t)s.B * s.group + s.pre_tile_rows - 1) / s.pre_tile_rows);
+}
 // Partial results of that kernel: one per CTA, of `prefix_rows` rows.
-__host__ __device__ inline int prefix_rows(const Shape &s) { return s.B * (int64_t)s.group < kPrefixRows ? s.B * s.group : kPrefixRows; }
+__host__ __device__ inline int prefix_rows(const Shape &s) { return min(s.B * s.group, s.pre_tile_rows); }
 inline int64_t prefix_slots(const Shape &s) { return (int64_t)s.n_kv * prefix_row_tiles(s) * s.pre_splits; }
 
-// Sizes for which the shared positions of a call are cut `splits` ways by attn_prefix_kernel.
-int prefix_splits(const Shape &s);
+// Sets pre_tile_rows and pre_splits of a call whose shared positions go through attn_prefix_kernel.
+void plan_prefix(Shape &s, int dk);
 
 // softmax(q k) v of every row of the batch over the shared positions, as partial results:
 // part [slot][row][dv] attention over the slot's positions, lse [slot][row] log2 of their sum of exponentials.

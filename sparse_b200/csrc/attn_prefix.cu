@@ -10,12 +10,15 @@
 //
 // Roles: warp 0 loads tiles of 128 keys and values (TMA: bf16 boxes into the swizzled operand
 // layout; codes as one run of bytes each), warp 1 issues the products, two groups of four
-// warps do the softmax, one thread per row, on alternating tiles.  Each group has its own
-// scores, its own running maximum and its own output accumulator in TMEM (2 x 128 + 2 x DV
-// columns), so the groups exchange nothing and one group's products run under the other's
-// exponentials; probabilities go back into TMEM (bf16, over their scores), where the second
-// product takes its left operand from.  Quantised: four more warps turn a row of codes per
-// thread into bf16 operands, scale applied (exact), so the products are the bf16 ones.
+// warps do the softmax of 64-position blocks, one thread per row.  Up to 128 rows the groups
+// take one half of every tile each, above (heads of 128 and less) one of two row tiles each, so
+// that a tile is loaded and converted once for 256 rows.  A group has its own running maximum,
+// its own output accumulator and two score buffers in TMEM (2 x 2 x 64 + 2 x DV columns): the
+// groups exchange nothing until the end, and a block's products run under the exponentials of
+// the block before it.  Probabilities go back into TMEM (bf16, over their scores), where the
+// second product takes its left operand from.  Quantised: four warps turn the keys' codes into
+// bf16 operands and four the values', a row per thread, scale applied (exact), so the products
+// are the bf16 ones.
 //
 // Probabilities are rounded to bf16 (2^-8), the type of the values that they are multiplied
 // with; scores, their sums and the accumulators are fp32.
@@ -32,19 +35,23 @@ namespace {
 
 constexpr int kKeys = 128;                       // positions of a tile
 constexpr uint32_t kBox = kKeys * 128;           // 64 bf16 columns of 128 rows: 16 KB
+constexpr int kBlock = 64;                        // positions of a block: what a group works on at a time
 constexpr int kSoftmaxWarp = 4, kConvertWarp = 12;
 
-template <int DK, int DV, bool FP8>
+// TWO: two row tiles of 128 rows, one for each group
+template <int DK, int DV, bool FP8, bool TWO>
 struct Layout {
   static constexpr uint32_t kQ = DK / 64 * kBox, kK = DK / 64 * kBox, kV = DV / 64 * kBox;
+  static constexpr uint32_t kAllQ = (TWO ? 2 : 1) * kQ;
   // operand buffers: filled by TMA (bf16), or by the converting warps from two stages of codes
-  static constexpr int kStages = FP8 ? (DK > 128 ? 1 : 2) : (DK > 128 ? 2 : DK > 64 ? 3 : 4);
+  static constexpr int kStages = FP8 ? (TWO || DK > 128 ? 1 : 2) : (TWO || DK > 128 ? 2 : DK > 64 ? 3 : 4);
   static constexpr int kRaw = FP8 ? 2 : 0;
   static constexpr uint32_t kRawK = kKeys * DK, kRawV = kKeys * DV;
-  static constexpr uint32_t kBytes = kQ + kStages * (kK + kV) + kRaw * (kRawK + kRawV);
+  static constexpr uint32_t kBytes = kAllQ + kStages * (kK + kV) + kRaw * (kRawK + kRawV);
   static constexpr uint32_t kSmem = kBytes + 1024 + 256;
-  static constexpr int kThreads = FP8 ? 512 : 384;
+  static constexpr int kThreads = FP8 ? 640 : 384;
   static_assert(kSmem <= 232448, "shared memory of a CTA");
+  static_assert(!TWO || DK <= 128, "two row tiles of wider heads leave no room for the keys");
 };
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -120,7 +127,7 @@ __device__ __forceinline__ void convert16(const uint4 &c, float scale, uint4 &lo
 
 constexpr float kNone = -3.0e38f;                // the maximum of no score, or of scores of -inf alone
 
-// 32 scores of a row from position x of its tile on; in the last tile (TAIL) those behind the last
+// 32 scores of a row from position x of its block on; in the last blocks (TAIL) those behind the last
 // shared position are -inf.
 template <bool TAIL>
 __device__ __forceinline__ void row_scores(uint32_t st_at, int x, int keys, uint32_t (&r)[32]) {
@@ -137,7 +144,7 @@ template <bool TAIL>
 __device__ __forceinline__ float row_top(uint32_t st_at, int keys) {
   float top[4] = {kNone, kNone, kNone, kNone};
 #pragma unroll
-  for (int x = 0; x < kKeys; x += 32) {
+  for (int x = 0; x < kBlock; x += 32) {
     uint32_t r[32];
     row_scores<TAIL>(st_at, x, keys, r);
 #pragma unroll
@@ -153,7 +160,7 @@ template <bool TAIL>
 __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float scale_log2, float m) {
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int x = 0; x < kKeys; x += 32) {
+  for (int x = 0; x < kBlock; x += 32) {
     uint32_t r[32], p[16];
     row_scores<TAIL>(st_at, x, keys, r);
 #pragma unroll
@@ -169,39 +176,42 @@ __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float sc
 }
 
 // grid = (runs of positions, row tiles, key heads)
-template <int DK, int DV, bool FP8>
-__global__ void __launch_bounds__(Layout<DK, DV, FP8>::kThreads, 1)
+template <int DK, int DV, bool FP8, bool TWO>
+__global__ void __launch_bounds__(Layout<DK, DV, FP8, TWO>::kThreads, 1)
 attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const __nv_bfloat16 *__restrict__ q, Cache cache, Shape s, float *__restrict__ part,
                    float *__restrict__ part_lse, int32_t *__restrict__ status) {
-  using L = Layout<DK, DV, FP8>;
-  constexpr int NS = L::kStages, NR = L::kRaw;
+  using L = Layout<DK, DV, FP8, TWO>;
+  constexpr int NS = L::kStages, kRows = TWO ? 2 * kPrefixRows : kPrefixRows;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char *aligned_base = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t q_smem = base, k_smem = q_smem + L::kQ, v_smem = k_smem + NS * L::kK, raw_smem = v_smem + NS * L::kV;
+  const uint32_t q_smem = base, k_smem = q_smem + L::kAllQ, v_smem = k_smem + NS * L::kK, raw_smem = v_smem + NS * L::kV;
   const uint32_t bars = base + L::kBytes;
   const uint32_t k_full = bars, k_empty = k_full + 8 * 4, v_full = k_empty + 8 * 4, v_empty = v_full + 8 * 4;
-  const uint32_t s_full = v_empty + 8 * 4, p_full = s_full + 16, o_full = p_full + 16;
-  const uint32_t rk_full = o_full + 16, rv_full = rk_full + 16, r_empty = rv_full + 16;       // two each
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(aligned_base + L::kBytes + 8 * 16 + 16 * 6);
+  const uint32_t s_full = v_empty + 8 * 4, p_full = s_full + 8 * 4;                            // [group][buffer]
+  const uint32_t pv_done = p_full + 8 * 4;                                                    // [group], a phase per block
+  const uint32_t rk_full = pv_done + 16, rv_full = rk_full + 16, r_empty = rv_full + 16;      // two each
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(aligned_base + L::kBytes + 8 * (6 * 4 + 8));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.z, rt = blockIdx.y;
   const int all_tiles = (s.shared_len + kKeys - 1) / kKeys;
   const int tile0 = (int)((int64_t)blockIdx.x * all_tiles / gridDim.x), tile1 = (int)((int64_t)(blockIdx.x + 1) * all_tiles / gridDim.x);
-  const int n = tile1 - tile0;
-  const int rows = min(kPrefixRows, s.B * s.group - rt * kPrefixRows);
+  const int n = tile1 - tile0;                          // tiles of this run, at least one
+  const int blocks = TWO ? 2 * n : n;                   // of each group
+  const int rows = min(kRows, s.B * s.group - rt * kRows);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NS; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(k_full + 8 * i, FP8 ? 4 : 1); mbar_init(k_empty + 8 * i, 1);
       mbar_init(v_full + 8 * i, FP8 ? 4 : 1); mbar_init(v_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); mbar_init(o_full + 8 * i, 1);
-      mbar_init(rk_full + 8 * i, 1); mbar_init(rv_full + 8 * i, 1); mbar_init(r_empty + 8 * i, 4);
+      mbar_init(pv_done + 8 * i, 1);
+      mbar_init(rk_full + 8 * i, 1); mbar_init(rv_full + 8 * i, 1); mbar_init(r_empty + 8 * i, 8);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -215,11 +225,11 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   pdl_wait();
   // the tile's query rows, zeros behind the last one
   const bool q_vec = s.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-  for (int i = threadIdx.x; i < kPrefixRows * (DK / 8); i += L::kThreads) {
+  for (int i = threadIdx.x; i < kRows * (DK / 8); i += L::kThreads) {
     const int row = i / (DK / 8), chunk = i - row * (DK / 8);
     uint4 x = make_uint4(0, 0, 0, 0);
     if (row < rows) {
-      const int r = rt * kPrefixRows + row, b = r / s.group, h = hk * s.group + r - b * s.group;
+      const int r = rt * kRows + row, b = r / s.group, h = hk * s.group + r - b * s.group;
       const __nv_bfloat16 *src = q + b * s.q_stride + (size_t)h * DK + chunk * 8;
       if (q_vec) {
         x = __ldg(reinterpret_cast<const uint4 *>(src));
@@ -229,14 +239,15 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                        e[6] | ((uint32_t)e[7] << 16));
       }
     }
-    *reinterpret_cast<uint4 *>(aligned_base + swizzled(row, chunk)) = x;
+    *reinterpret_cast<uint4 *>(aligned_base + row / kPrefixRows * L::kQ + swizzled(row % kPrefixRows, chunk)) = x;
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t s_tmem = tmem, o_tmem = tmem + 2 * kKeys;
+  // group w: score buffers at s_tmem + (2 w + 0, 1) * 64, accumulator at o_tmem + w * DV
+  const uint32_t s_tmem = tmem, o_tmem = tmem + 4 * kBlock;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -270,56 +281,70 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t id_s = idesc_m128(kKeys, false), id_o = idesc_m128(DV, true);
-      bool ok = true;
-      const auto scores = [&](int i) {
-        const int st = i % NS;
-        if (!mbar_wait(k_full + 8 * st, (i / NS) & 1, abort_flag)) return false;
+      constexpr uint32_t id_s = idesc_m128(kBlock, false), id_o = idesc_m128(DV, true);
+      constexpr uint32_t half_rows = kBlock * 128 >> 4;         // a tile's second half, in descriptor units
+      // block j of a group: tile, and which half of it
+      const auto tile_of = [](int j) { return TWO ? j >> 1 : j; };
+      const auto half_of = [](int j, int w) { return TWO ? j & 1 : w; };
+      const auto scores = [&](int j) {
+        const int i = tile_of(j), st = i % NS;
+        if ((!TWO || !(j & 1)) && !mbar_wait(k_full + 8 * st, (i / NS) & 1, abort_flag)) return false;
         tc_fence_after();
-        const uint64_t a = umma_desc_sw128(q_smem), b = umma_desc_sw128(k_smem + st * L::kK);
+        for (int w = 0; w < 2; ++w) {
+          const uint64_t a = umma_desc_sw128(q_smem + (TWO ? w * L::kQ : 0)), b = umma_desc_sw128(k_smem + st * L::kK) + half_of(j, w) * half_rows;
 #pragma unroll
-        for (int x = 0; x < DK / 16; ++x) {
-          const uint64_t off = (uint64_t)((x >> 2) * (kBox >> 4) + (x & 3) * 2);
-          tc_mma_ss(s_tmem + (i & 1) * kKeys, a + off, b + off, id_s, x > 0);
+          for (int x = 0; x < DK / 16; ++x) {
+            const uint64_t off = (uint64_t)((x >> 2) * (kBox >> 4) + (x & 3) * 2);
+            tc_mma_ss(s_tmem + (2 * w + (j & 1)) * kBlock, a + off, b + off, id_s, x > 0);
+          }
+          tc_commit(s_full + 8 * (2 * w + (j & 1)));
         }
-        tc_commit(s_full + 8 * (i & 1));
-        tc_commit(k_empty + 8 * st);
+        if (!TWO || (j & 1)) tc_commit(k_empty + 8 * st);
         return true;
       };
-      if (n > 0) ok = scores(0);
-      for (int i = 0; ok && i < n; ++i) {
-        // (the scores of tile i + 1 go where those of i - 1 were: their second product is issued)
-        if (i + 1 < n && !scores(i + 1)) break;
-        const int st = i % NS, w = i & 1;
-        if (!mbar_wait(v_full + 8 * st, (i / NS) & 1, abort_flag)) break;
-        if (!mbar_wait(p_full + 8 * w, (i >> 1) & 1, abort_flag)) break;
-        tc_fence_after();
-        const uint64_t b = desc_values(v_smem + st * L::kV);
+      bool ok = scores(0);
+      for (int j = 0; ok && j < blocks; ++j) {
+        // (the scores of block j + 1 go where those of j - 1 were: their second product is issued)
+        if (j + 1 < blocks && !scores(j + 1)) break;
+        const int i = tile_of(j), st = i % NS;
+        if ((!TWO || !(j & 1)) && !mbar_wait(v_full + 8 * st, (i / NS) & 1, abort_flag)) break;
+        for (int w = 0; w < 2; ++w) {
+          ok = mbar_wait(p_full + 8 * (2 * w + (j & 1)), (j >> 1) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t b = desc_values(v_smem + st * L::kV) + half_of(j, w) * half_rows;
 #pragma unroll
-        for (int x = 0; x < kKeys / 16; ++x)
-          tc_mma_ts(o_tmem + w * DV, s_tmem + w * kKeys + x * 8, b + (uint64_t)(x * (2048 >> 4)), id_o, i > 1 || x > 0);
-        tc_commit(v_empty + 8 * st);
-        if (i + 2 >= n) tc_commit(o_full + 8 * w);
+          for (int x = 0; x < kBlock / 16; ++x)
+            tc_mma_ts(o_tmem + w * DV, s_tmem + (2 * w + (j & 1)) * kBlock + x * 8, b + (uint64_t)(x * (2048 >> 4)), id_o, j > 0 || x > 0);
+          tc_commit(pv_done + 8 * w);
+        }
+        if (ok && (!TWO || (j & 1))) tc_commit(v_empty + 8 * st);
       }
     }
   } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
     const int w = (warp - kSoftmaxWarp) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
-    const uint32_t st_at = s_tmem + w * kKeys + lane_at, ot_at = o_tmem + w * DV + lane_at;
+    const uint32_t ot_at = o_tmem + w * DV + lane_at;
     float m = kNone, l = 0.f;
     bool ok = true;
-    for (int i = w; i < n; i += 2) {
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * w, (i >> 1) & 1, abort_flag));
+    for (int j = 0; j < blocks; ++j) {
+      const uint32_t st_at = s_tmem + (2 * w + (j & 1)) * kBlock + lane_at;
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (2 * w + (j & 1)), (j >> 1) & 1, abort_flag));
       if (!ok) break;
       tc_fence_after();
-      const int keys = min(kKeys, s.shared_len - (tile0 + i) * kKeys);
-      const float top = (keys == kKeys ? row_top<false>(st_at, keys) : row_top<true>(st_at, keys)) * s.scale_log2;
+      const int keys = s.shared_len - tile0 * kKeys - (TWO ? j * kBlock : j * kKeys + w * kBlock);
+      const bool whole = keys >= kBlock;
+      const float top = (whole ? row_top<false>(st_at, keys) : row_top<true>(st_at, keys)) * s.scale_log2;
       if (__any_sync(0xffffffffu, top > m + kLazy)) {
         const float up = fmaxf(m, top), f = exp2_approx(m - up);
         l *= f;
         m = up;
-        if (i >= 2) {                  // (the tile's scores are behind all earlier products: the accumulator is still)
-#pragma unroll
+        if (j > 0) {
+          // (the products of the blocks before the last are behind these scores; the last one's may be under way)
+          ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * w, (j - 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
           for (int x = 0; x < DV; x += 32) {
             uint32_t r[32], h[16];
             tc_ld32(ot_at + x, r);
@@ -333,109 +358,110 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           }
         }
       }
-      l += keys == kKeys ? exponentials<false>(st_at, keys, s.scale_log2, m) : exponentials<true>(st_at, keys, s.scale_log2, m);
+      l += whole ? exponentials<false>(st_at, keys, s.scale_log2, m) : exponentials<true>(st_at, keys, s.scale_log2, m);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * w);
+      if (lane == 0) mbar_arrive(p_full + 8 * (2 * w + (j & 1)));
     }
-    // The two groups' results become one: weights from both sums, this group's rows scaled by its
-    // own, the second group's added to the first's through shared memory (every product is done,
-    // so the operands' place is free), whole rows written.
-    ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full, 0, abort_flag) && (n < 2 || mbar_wait(o_full + 8, 0, abort_flag)));
-    tc_fence_after();
-    float2 *sums = reinterpret_cast<float2 *>(aligned_base);                             // [2][128], over the queries
-    float *rows_at = reinterpret_cast<float *>(aligned_base + L::kQ);                    // [128][DV + 4], over keys and values
-    static_assert(kPrefixRows * (DV + 4) * 4 <= L::kBytes - L::kQ, "room for the accumulators");
-    sums[w * kPrefixRows + row] = make_float2(m, l);
+    // A row's result: its accumulator over its sum.  Groups on the two halves of one row tile
+    // first agree on the weights of their sums.  Rows go through shared memory (every product is
+    // done, so the operands' place is free) to be written whole.
     const auto groups_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    if (ok) ok = __all_sync(0xffffffffu, blocks < 2 || mbar_wait(pv_done + 8 * w, (blocks - 2) & 1, abort_flag));
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * w, (blocks - 1) & 1, abort_flag));
+    tc_fence_after();
     groups_sync();
-    const float2 other = sums[(w ^ 1) * kPrefixRows + row];
-    const float most = fmaxf(m, other.x), mine = exp2_approx(m - most), sum = l * mine + other.y * exp2_approx(other.x - most);
-    const float f = sum == 0.f ? 0.f : mine / sum;
-    float4 *slot_at = reinterpret_cast<float4 *>(rows_at + row * (DV + 4));
+    float2 *sums = reinterpret_cast<float2 *>(aligned_base);                             // [2][128], over the queries
+    float *rows_at = reinterpret_cast<float *>(aligned_base + L::kAllQ);                 // [128][DV + 4], over keys and values
+    static_assert(kPrefixRows * (DV + 4) * 4 <= L::kBytes - L::kAllQ, "room for the accumulators");
+    float most = m, sum = l, f = l == 0.f ? 0.f : 1.f / l;
+    if constexpr (!TWO) {
+      sums[w * kPrefixRows + row] = make_float2(m, l);
+      groups_sync();
+      const float2 other = sums[(w ^ 1) * kPrefixRows + row];
+      most = fmaxf(m, other.x);
+      const float mine = exp2_approx(m - most);
+      sum = l * mine + other.y * exp2_approx(other.x - most);
+      f = sum == 0.f ? 0.f : mine / sum;
+    }
+    const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * prefix_rows(s);
+    float4 *row_at = reinterpret_cast<float4 *>(rows_at + row * (DV + 4));
+#pragma unroll 1
     for (int turn = 1; turn >= 0; --turn) {
       if (turn == w) {
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < DV; x += 32) {
           uint32_t r[32];
           tc_ld32(ot_at + x, r);
           tc_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            // (a group without a tile has nothing in its accumulator)
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (w < n && sum != 0.f)
+            if (sum != 0.f)
               o = make_float4(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f, __uint_as_float(r[e + 2]) * f,
                               __uint_as_float(r[e + 3]) * f);
-            if (w == 0) {
-              const float4 t = slot_at[(x + e) / 4];
+            if (!TWO && w == 0) {
+              const float4 t = row_at[(x + e) / 4];
               o = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
             }
-            slot_at[(x + e) / 4] = o;
+            row_at[(x + e) / 4] = o;
           }
         }
       }
       groups_sync();
-    }
-    if (ok) {
-      const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * prefix_rows(s);
-      for (int i = threadIdx.x - kSoftmaxWarp * 32; i < rows * (DV / 4); i += 256) {
-        const int r = i / (DV / 4), col = i - r * (DV / 4);
-        *reinterpret_cast<float4 *>(part + (slot_row + r) * DV + col * 4) = *reinterpret_cast<const float4 *>(rows_at + r * (DV + 4) + col * 4);
+      if (ok && (TWO || turn == 0)) {
+        const int r0 = TWO ? turn * kPrefixRows : 0, here = min(kPrefixRows, rows - r0);
+        for (int i = threadIdx.x - kSoftmaxWarp * 32; i < here * (DV / 4); i += 256) {
+          const int r = i / (DV / 4), col = i - r * (DV / 4);
+          *reinterpret_cast<float4 *>(part + (slot_row + r0 + r) * DV + col * 4) =
+              *reinterpret_cast<const float4 *>(rows_at + r * (DV + 4) + col * 4);
+        }
       }
-      if (w == 0 && row < rows) part_lse[slot_row + row] = sum == 0.f ? -INFINITY : most + log2f(sum);
+      if (TWO) groups_sync();
     }
+    const int r = TWO ? w * kPrefixRows + row : row;
+    if (ok && (TWO || w == 0) && r < rows) part_lse[slot_row + r] = sum == 0.f ? -INFINITY : most + log2f(sum);
     tc_fence_before();
   } else if (FP8 && warp >= kConvertWarp) {
-    // one row of codes per thread, its chunks in an order that keeps eight neighbouring rows
-    // on different banks, in the codes and in the swizzled operand
-    const int row = (warp - kConvertWarp) * 32 + lane;
+    // One row of codes per thread, keys in one group of four warps and values in the other.  The
+    // chunks of a row in an order that keeps eight neighbouring rows on different banks, in the
+    // codes and in the swizzled operand.
+    const bool keys_side = warp < kConvertWarp + 4;
+    const int row = (warp & 3) * 32 + lane;
     const size_t row0 = (size_t)hk * s.s_max;
-    const auto convert = [&](uint32_t src, uint32_t dst, int d, float scale, bool in) {
-      const int chunks = d / 16, start = row % chunks;
-#pragma unroll
-      for (int x0 = 0; x0 < chunks; x0 += 4) {
-        uint4 c[4], lo, hi;
-        int chunk[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          chunk[x] = start + x0 + x < chunks ? start + x0 + x : start + x0 + x - chunks;
-          c[x] = in ? *reinterpret_cast<const uint4 *>(aligned_base + (src - base) + row * d + chunk[x] * 16)
-                    : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          convert16(c[x], in ? scale : 0.f, lo, hi);
-          *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk[x])) = lo;
-          *reinterpret_cast<uint4 *>(aligned_base + (dst - base) + swizzled(row, 2 * chunk[x] + 1)) = hi;
-        }
-      }
-    };
-    const auto scale_at = [&](const uint8_t *scales, int i) {
+    const uint8_t *scales = keys_side ? cache.ks : cache.vs;
+    const uint32_t full = keys_side ? k_full : v_full, empty = keys_side ? k_empty : v_empty, raw_full = keys_side ? rk_full : rv_full;
+    const uint32_t op_smem = keys_side ? k_smem : v_smem, op_bytes = keys_side ? L::kK : L::kV;
+    const int d = keys_side ? DK : DV, chunks = d / 16, start = row % chunks;
+    const auto scale_at = [&](int i) {
       const int key = (tile0 + i) * kKeys + row;
       return i < n && key < s.shared_len ? (uint32_t)__ldg(scales + row0 + key) : 0u;
     };
-    uint32_t ks = scale_at(cache.ks, 0), vs = scale_at(cache.vs, 0);
+    uint32_t byte = scale_at(0);
     for (int i = 0; i < n; ++i) {
       const int st = i & 1, op = i % NS;
-      const uint32_t raw = raw_smem + st * (L::kRawK + L::kRawV), ph = (i >> 1) & 1, op_ph = ((i / NS) & 1) ^ 1u;
       const bool in = (tile0 + i) * kKeys + row < s.shared_len;
-      const uint32_t ks_next = scale_at(cache.ks, i + 1), vs_next = scale_at(cache.vs, i + 1);
-      bool ok = mbar_wait(rk_full + 8 * st, ph, abort_flag) && mbar_wait(k_empty + 8 * op, op_ph, abort_flag);
+      const uint32_t next = scale_at(i + 1);
+      const bool ok = mbar_wait(raw_full + 8 * st, (i >> 1) & 1, abort_flag) && mbar_wait(empty + 8 * op, ((i / NS) & 1) ^ 1u, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) break;
-      convert(raw, k_smem + op * L::kK, DK, e8m0_value(ks), in);
+      const unsigned char *src = aligned_base + (raw_smem - base) + st * (L::kRawK + L::kRawV) + (keys_side ? 0 : L::kRawK) + row * d;
+      unsigned char *dst = aligned_base + (op_smem - base) + op * op_bytes;
+      const float scale = e8m0_value(byte);
+      int chunk = start;
+#pragma unroll 4
+      for (int x = 0; x < chunks; ++x) {
+        uint4 c = make_uint4(0, 0, 0, 0), lo, hi;
+        if (in) c = *reinterpret_cast<const uint4 *>(src + chunk * 16);       // (behind the end stands whatever was there before)
+        convert16(c, in ? scale : 0.f, lo, hi);
+        *reinterpret_cast<uint4 *>(dst + swizzled(row, 2 * chunk)) = lo;
+        *reinterpret_cast<uint4 *>(dst + swizzled(row, 2 * chunk + 1)) = hi;
+        chunk = chunk + 1 == chunks ? 0 : chunk + 1;
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(k_full + 8 * op);
-      ok = mbar_wait(rv_full + 8 * st, ph, abort_flag) && mbar_wait(v_empty + 8 * op, op_ph, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      convert(raw + L::kRawK, v_smem + op * L::kV, DV, e8m0_value(vs), in);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) { mbar_arrive(v_full + 8 * op); mbar_arrive(r_empty + 8 * st); }
-      ks = ks_next;
-      vs = vs_next;
+      if (lane == 0) { mbar_arrive(full + 8 * op); mbar_arrive(r_empty + 8 * st); }
+      byte = next;
     }
   }
 
@@ -476,17 +502,17 @@ int32_t encode_rows(CUtensorMap *tm, const void *base, int d, int n_kv, int shar
   return SB_OK;
 }
 
-template <int DK, int DV, bool FP8>
+template <int DK, int DV, bool FP8, bool TWO>
 int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float *part, float *lse, int32_t *status,
                cudaStream_t stream) {
-  using L = Layout<DK, DV, FP8>;
+  using L = Layout<DK, DV, FP8, TWO>;
   CUtensorMap tm_k = {}, tm_v = {};
   if (!FP8) {
     int32_t rc = encode_rows(&tm_k, cache.k, DK, s.n_kv, s.shared_len);
     if (rc == SB_OK) rc = encode_rows(&tm_v, cache.v, DV, s.n_kv, s.shared_len);
     if (rc != SB_OK) return rc;
   }
-  auto kern = attn_prefix_kernel<DK, DV, FP8>;
+  auto kern = attn_prefix_kernel<DK, DV, FP8, TWO>;
   SB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
   const dim3 grid(s.pre_splits, prefix_row_tiles(s), s.n_kv);
   SB_CUDA_CHECK(launch_pdl(kern, grid, dim3(L::kThreads), L::kSmem, stream, tm_k, tm_v, q, cache, s, part, lse, status));
@@ -496,17 +522,22 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float
 
 }  // namespace
 
-int prefix_splits(const Shape &s) {
+void plan_prefix(Shape &s, int dk) {
+  s.pre_tile_rows = (int64_t)s.B * s.group > kPrefixRows && dk <= 128 ? 2 * kPrefixRows : kPrefixRows;
   const int64_t tiles = (s.shared_len + kKeys - 1) / kKeys, heads = (int64_t)s.n_kv * prefix_row_tiles(s);
   const int64_t fit = 148 / heads;
-  return (int)(fit < 1 ? 1 : fit < tiles ? fit : tiles);
+  s.pre_splits = (int)(fit < 1 ? 1 : fit < tiles ? fit : tiles);
 }
 
 int32_t launch_attn_prefix(bool fp8, int dk, int dv, const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float *part,
                            float *lse, int32_t *status, cudaStream_t stream) {
-  if (dk == 128) return (fp8 ? launch<128, 128, true> : launch<128, 128, false>)(q, cache, s, part, lse, status, stream);
-  if (dk == 192) return (fp8 ? launch<192, 128, true> : launch<192, 128, false>)(q, cache, s, part, lse, status, stream);
-  return (fp8 ? launch<64, 64, true> : launch<64, 64, false>)(q, cache, s, part, lse, status, stream);
+  const bool two = s.pre_tile_rows > kPrefixRows;
+  if (dk == 192) return (fp8 ? launch<192, 128, true, false> : launch<192, 128, false, false>)(q, cache, s, part, lse, status, stream);
+  if (dk == 128)
+    return (fp8 ? two ? launch<128, 128, true, true> : launch<128, 128, true, false>
+                : two ? launch<128, 128, false, true> : launch<128, 128, false, false>)(q, cache, s, part, lse, status, stream);
+  return (fp8 ? two ? launch<64, 64, true, true> : launch<64, 64, true, false>
+              : two ? launch<64, 64, false, true> : launch<64, 64, false, false>)(q, cache, s, part, lse, status, stream);
 }
 
 }  // namespace sb

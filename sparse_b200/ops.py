@@ -320,7 +320,7 @@ def _decode_attention(name: str, call, q: torch.Tensor, cache_ptrs, seq_lens: to
         raise RuntimeError("%s: status must be int32 on the cache's device" % name)
     lens = _index(seq_lens, b, device, name)
     out = q.new_empty((b, n_q, dv))
-    ws_bytes = lib.sb_attn_cached_workspace_bytes(b, n_q, n_kv, dv, s_max, shared_len) or 16
+    ws_bytes = lib.sb_attn_cached_workspace_bytes(b, n_q, n_kv, dk, dv, s_max, shared_len) or 16
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
     with _On(device) as stream:
         check(call(q.data_ptr(), seq_stride if b > 1 else 0, *cache_ptrs, lens, b, n_q, n_kv, dk, dv, s_max, shared_len,
