@@ -54,6 +54,12 @@ struct Layout {
   static_assert(!TWO || DK <= 128, "two row tiles of wider heads leave no room for the keys");
 };
 
+// one lane of a warp that runs together
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -195,7 +201,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(aligned_base + L::kBytes + 8 * (6 * 4 + 8));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (the warp's number and the TMEM address as values that are the same for the whole warp: the
+  // instructions that issue products and copies take uniform registers)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hk = blockIdx.z, rt = blockIdx.y;
   const int all_tiles = (s.shared_len + kKeys - 1) / kKeys;
   const int tile0 = (int)((int64_t)blockIdx.x * all_tiles / gridDim.x), tile1 = (int)((int64_t)(blockIdx.x + 1) * all_tiles / gridDim.x);
@@ -227,52 +235,57 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const bool q_vec = s.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
   for (int i = threadIdx.x; i < kRows * (DK / 8); i += L::kThreads) {
     const int row = i / (DK / 8), chunk = i - row * (DK / 8);
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (row < rows) {
-      const int r = rt * kRows + row, b = r / s.group, h = hk * s.group + r - b * s.group;
-      const __nv_bfloat16 *src = q + b * s.q_stride + (size_t)h * DK + chunk * 8;
-      if (q_vec) {
-        x = __ldg(reinterpret_cast<const uint4 *>(src));
-      } else {
-        const unsigned short *e = reinterpret_cast<const unsigned short *>(src);
+    const uint32_t at = row / kPrefixRows * L::kQ + swizzled(row % kPrefixRows, chunk);
+    const int r = min(rt * kRows + row, s.B * s.group - 1), b = r / s.group, h = hk * s.group + r - b * s.group;
+    const __nv_bfloat16 *src = q + b * s.q_stride + (size_t)h * DK + chunk * 8;
+    if (q_vec) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + at), "l"(src), "r"(row < rows ? 16 : 0) : "memory");
+    } else {
+      const unsigned short *e = reinterpret_cast<const unsigned short *>(src);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row < rows)
         x = make_uint4(e[0] | ((uint32_t)e[1] << 16), e[2] | ((uint32_t)e[3] << 16), e[4] | ((uint32_t)e[5] << 16),
                        e[6] | ((uint32_t)e[7] << 16));
-      }
+      *reinterpret_cast<uint4 *>(aligned_base + at) = x;
     }
-    *reinterpret_cast<uint4 *>(aligned_base + row / kPrefixRows * L::kQ + swizzled(row % kPrefixRows, chunk)) = x;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   // group w: score buffers at s_tmem + (2 w + 0, 1) * 64, accumulator at o_tmem + w * DV
   const uint32_t s_tmem = tmem, o_tmem = tmem + 4 * kBlock;
 
   if (warp == 0) {
-    if (lane == 0) {
-      if constexpr (FP8) {
-        const size_t row0 = (size_t)hk * s.s_max;
-        for (int i = 0; i < n; ++i) {
-          const int st = i & 1, key = (tile0 + i) * kKeys;
-          const uint32_t keys = min(kKeys, s.shared_len - key);
-          if (!mbar_wait(r_empty + 8 * st, ((i >> 1) & 1) ^ 1u, abort_flag)) break;
+    if constexpr (FP8) {
+      const size_t row0 = (size_t)hk * s.s_max;
+      for (int i = 0; i < n; ++i) {
+        const int st = i & 1, key = (tile0 + i) * kKeys;
+        const uint32_t keys = min(kKeys, s.shared_len - key);
+        if (!__all_sync(0xffffffffu, mbar_wait(r_empty + 8 * st, ((i >> 1) & 1) ^ 1u, abort_flag))) break;
+        if (elect_one()) {
           const uint32_t dst = raw_smem + st * (L::kRawK + L::kRawV);
           mbar_expect_tx(rk_full + 8 * st, keys * DK);
           bulk_load(dst, static_cast<const uint8_t *>(cache.k) + (row0 + key) * DK, keys * DK, rk_full + 8 * st);
           mbar_expect_tx(rv_full + 8 * st, keys * DV);
           bulk_load(dst + L::kRawK, static_cast<const uint8_t *>(cache.v) + (row0 + key) * DV, keys * DV, rv_full + 8 * st);
         }
-      } else {
-        // (positions behind the last shared one lie outside the tensor map: zeros)
-        for (int i = 0; i < n; ++i) {
-          const int st = i % NS, key = (tile0 + i) * kKeys;
-          const uint32_t ph = ((i / NS) & 1) ^ 1u;
-          if (!mbar_wait(k_empty + 8 * st, ph, abort_flag)) break;
+      }
+    } else {
+      // (positions behind the last shared one lie outside the tensor map: zeros)
+      for (int i = 0; i < n; ++i) {
+        const int st = i % NS, key = (tile0 + i) * kKeys;
+        const uint32_t ph = ((i / NS) & 1) ^ 1u;
+        if (!__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * st, ph, abort_flag))) break;
+        if (elect_one()) {
           mbar_expect_tx(k_full + 8 * st, L::kK);
 #pragma unroll
           for (int x = 0; x < DK / 64; ++x) tma_load_3d(k_smem + st * L::kK + x * kBox, &tm_k, k_full + 8 * st, x * 64, hk, key);
-          if (!mbar_wait(v_empty + 8 * st, ph, abort_flag)) break;
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * st, ph, abort_flag))) break;
+        if (elect_one()) {
           mbar_expect_tx(v_full + 8 * st, L::kV);
 #pragma unroll
           for (int x = 0; x < DV / 64; ++x) tma_load_3d(v_smem + st * L::kV + x * kBox, &tm_v, v_full + 8 * st, x * 64, hk, key);
@@ -280,18 +293,26 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_m128(kBlock, false), id_o = idesc_m128(DV, true);
-      constexpr uint32_t half_rows = kBlock * 128 >> 4;         // a tile's second half, in descriptor units
-      // block j of a group: tile, and which half of it
-      const auto tile_of = [](int j) { return TWO ? j >> 1 : j; };
-      const auto half_of = [](int j, int w) { return TWO ? j & 1 : w; };
-      const auto scores = [&](int j) {
-        const int i = tile_of(j), st = i % NS;
-        if ((!TWO || !(j & 1)) && !mbar_wait(k_full + 8 * st, (i / NS) & 1, abort_flag)) return false;
-        tc_fence_after();
+    // (one and the same lane issues everything: completion is tracked per thread)
+    const bool leader = elect_one();
+    constexpr uint32_t id_s = idesc_m128(kBlock, false), id_o = idesc_m128(DV, true);
+    constexpr uint32_t half_rows = kBlock * 128 >> 4;         // a tile's second half, in descriptor units
+    const uint64_t q_desc = umma_desc_sw128(q_smem), k_desc = umma_desc_sw128(k_smem), v_desc = desc_values(v_smem);
+    // block j of a group: tile, and which half of it
+    const auto tile_of = [](int j) { return TWO ? j >> 1 : j; };
+    const auto half_of = [](int j, int w) { return TWO ? j & 1 : w; };
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+      tc_fence_after();
+      return ok;
+    };
+    const auto scores = [&](int j) {
+      const int i = tile_of(j), st = i % NS;
+      if ((!TWO || !(j & 1)) && !wait(k_full + 8 * st, (i / NS) & 1)) return false;
+      if (leader) {
+#pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const uint64_t a = umma_desc_sw128(q_smem + (TWO ? w * L::kQ : 0)), b = umma_desc_sw128(k_smem + st * L::kK) + half_of(j, w) * half_rows;
+          const uint64_t a = q_desc + (TWO ? w * (L::kQ >> 4) : 0), b = k_desc + (uint64_t)(st * (L::kK >> 4) + half_of(j, w) * half_rows);
 #pragma unroll
           for (int x = 0; x < DK / 16; ++x) {
             const uint64_t off = (uint64_t)((x >> 2) * (kBox >> 4) + (x & 3) * 2);
@@ -300,25 +321,28 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           tc_commit(s_full + 8 * (2 * w + (j & 1)));
         }
         if (!TWO || (j & 1)) tc_commit(k_empty + 8 * st);
-        return true;
-      };
-      bool ok = scores(0);
-      for (int j = 0; ok && j < blocks; ++j) {
-        // (the scores of block j + 1 go where those of j - 1 were: their second product is issued)
-        if (j + 1 < blocks && !scores(j + 1)) break;
-        const int i = tile_of(j), st = i % NS;
-        if ((!TWO || !(j & 1)) && !mbar_wait(v_full + 8 * st, (i / NS) & 1, abort_flag)) break;
-        for (int w = 0; w < 2; ++w) {
-          ok = mbar_wait(p_full + 8 * (2 * w + (j & 1)), (j >> 1) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t b = desc_values(v_smem + st * L::kV) + half_of(j, w) * half_rows;
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = scores(0);
+    for (int j = 0; ok && j < blocks; ++j) {
+      // (the scores of block j + 1 go where those of j - 1 were: their second product is issued)
+      if (j + 1 < blocks && !scores(j + 1)) break;
+      const int i = tile_of(j), st = i % NS;
+      if ((!TWO || !(j & 1)) && !wait(v_full + 8 * st, (i / NS) & 1)) break;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        ok = ok && wait(p_full + 8 * (2 * w + (j & 1)), (j >> 1) & 1);
+        if (ok && leader) {
+          const uint64_t b = v_desc + (uint64_t)(st * (L::kV >> 4) + half_of(j, w) * half_rows);
 #pragma unroll
           for (int x = 0; x < kBlock / 16; ++x)
             tc_mma_ts(o_tmem + w * DV, s_tmem + (2 * w + (j & 1)) * kBlock + x * 8, b + (uint64_t)(x * (2048 >> 4)), id_o, j > 0 || x > 0);
           tc_commit(pv_done + 8 * w);
+          if (w == 1 && (!TWO || (j & 1))) tc_commit(v_empty + 8 * st);
         }
-        if (ok && (!TWO || (j & 1))) tc_commit(v_empty + 8 * st);
+        __syncwarp();
       }
     }
   } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
@@ -367,14 +391,18 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     // A row's result: its accumulator over its sum.  Groups on the two halves of one row tile
     // first agree on the weights of their sums.  Rows go through shared memory (every product is
     // done, so the operands' place is free) to be written whole.
-    const auto groups_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    const auto groups_sync = [&] {
+      if (TWO) asm volatile("bar.sync %0, 128;" ::"r"(2 + w) : "memory");
+      else asm volatile("bar.sync 1, 256;" ::: "memory");
+    };
     if (ok) ok = __all_sync(0xffffffffu, blocks < 2 || mbar_wait(pv_done + 8 * w, (blocks - 2) & 1, abort_flag));
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * w, (blocks - 1) & 1, abort_flag));
     tc_fence_after();
-    groups_sync();
-    float2 *sums = reinterpret_cast<float2 *>(aligned_base);                             // [2][128], over the queries
-    float *rows_at = reinterpret_cast<float *>(aligned_base + L::kAllQ);                 // [128][DV + 4], over keys and values
-    static_assert(kPrefixRows * (DV + 4) * 4 <= L::kBytes - L::kAllQ, "room for the accumulators");
+    asm volatile("bar.sync 1, 256;" ::: "memory");                                       // both groups' products
+    constexpr int kPitch = DV + 4;
+    float2 *sums = reinterpret_cast<float2 *>(aligned_base);                             // [2][128]
+    float *rows_at = reinterpret_cast<float *>(aligned_base + 4096);                     // [2][128][kPitch]
+    static_assert(4096 + 2 * kPrefixRows * kPitch * 4 <= L::kBytes, "room for the accumulators");
     float most = m, sum = l, f = l == 0.f ? 0.f : 1.f / l;
     if constexpr (!TWO) {
       sums[w * kPrefixRows + row] = make_float2(m, l);
@@ -385,43 +413,34 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       sum = l * mine + other.y * exp2_approx(other.x - most);
       f = sum == 0.f ? 0.f : mine / sum;
     }
-    const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * prefix_rows(s);
-    float4 *row_at = reinterpret_cast<float4 *>(rows_at + row * (DV + 4));
+    float4 *row_at = reinterpret_cast<float4 *>(rows_at + (w * kPrefixRows + row) * kPitch);
 #pragma unroll 1
-    for (int turn = 1; turn >= 0; --turn) {
-      if (turn == w) {
-#pragma unroll 1
-        for (int x = 0; x < DV; x += 32) {
-          uint32_t r[32];
-          tc_ld32(ot_at + x, r);
-          tc_wait_ld();
+    for (int x = 0; x < DV; x += 32) {
+      uint32_t r[32];
+      tc_ld32(ot_at + x, r);
+      tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (sum != 0.f)
-              o = make_float4(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f, __uint_as_float(r[e + 2]) * f,
-                              __uint_as_float(r[e + 3]) * f);
-            if (!TWO && w == 0) {
-              const float4 t = row_at[(x + e) / 4];
-              o = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
-            }
-            row_at[(x + e) / 4] = o;
-          }
-        }
-      }
-      groups_sync();
-      if (ok && (TWO || turn == 0)) {
-        const int r0 = TWO ? turn * kPrefixRows : 0, here = min(kPrefixRows, rows - r0);
-        for (int i = threadIdx.x - kSoftmaxWarp * 32; i < here * (DV / 4); i += 256) {
-          const int r = i / (DV / 4), col = i - r * (DV / 4);
-          *reinterpret_cast<float4 *>(part + (slot_row + r0 + r) * DV + col * 4) =
-              *reinterpret_cast<const float4 *>(rows_at + r * (DV + 4) + col * 4);
-        }
-      }
-      if (TWO) groups_sync();
+      for (int e = 0; e < 32; e += 4)
+        row_at[(x + e) / 4] = sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                         : make_float4(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f,
+                                                       __uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f);
     }
-    const int r = TWO ? w * kPrefixRows + row : row;
-    if (ok && (TWO || w == 0) && r < rows) part_lse[slot_row + r] = sum == 0.f ? -INFINITY : most + log2f(sum);
+    groups_sync();
+    if (ok) {
+      const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * prefix_rows(s);
+      const int r0 = TWO ? w * kPrefixRows : 0, here = min(kPrefixRows, rows - r0), threads = TWO ? 128 : 256;
+#pragma unroll 4
+      for (int i = threadIdx.x - kSoftmaxWarp * 32 - r0; i < here * (DV / 4); i += threads) {
+        const int r = i / (DV / 4), col = i - r * (DV / 4);
+        float4 o = *reinterpret_cast<const float4 *>(rows_at + (r0 + r) * kPitch + col * 4);
+        if constexpr (!TWO) {
+          const float4 t = *reinterpret_cast<const float4 *>(rows_at + (kPrefixRows + r) * kPitch + col * 4);
+          o = make_float4(o.x + t.x, o.y + t.y, o.z + t.z, o.w + t.w);
+        }
+        *reinterpret_cast<float4 *>(part + (slot_row + r0 + r) * DV + col * 4) = o;
+      }
+      if ((TWO || w == 0) && r0 + row < rows) part_lse[slot_row + r0 + row] = sum == 0.f ? -INFINITY : most + log2f(sum);
+    }
     tc_fence_before();
   } else if (FP8 && warp >= kConvertWarp) {
     // One row of codes per thread, keys in one group of four warps and values in the other.  The
