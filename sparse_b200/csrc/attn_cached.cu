@@ -458,16 +458,24 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
     at.w = first / at.tiles;
     at.tile = first - at.w * at.tiles;
   } else {
+    // the sequence among whose tiles the first one is: 32 sequences' tiles summed at a time
     int before = pre_line, b0 = 0;
-    for (; b0 + 32 < s.B; b0 += 32) {               // the 32 sequences among whose tiles the first one is
-      const int n = own_heads * warp_sum_int(own_tiles<FP8>(s, seq_len(s, seq_lens, b0 + lane)));
-      if (before + n > first) break;
-      before += n;
-    }
-    for (; b0 + 1 < s.B; ++b0) {
-      const int n = own_heads * own_tiles<FP8>(s, seq_len(s, seq_lens, b0));
-      if (before + n > first) break;
-      before += n;
+    for (;; b0 += 32) {
+      const int mine = b0 + lane < s.B ? own_heads * own_tiles<FP8>(s, seq_len(s, seq_lens, b0 + lane)) : 0;
+      int upto = mine;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += x;
+      }
+      const uint32_t beyond = __ballot_sync(0xffffffffu, before + upto > first);
+      if (beyond != 0 || b0 + 32 >= s.B) {
+        const int at_lane = beyond != 0 ? __ffs(beyond) - 1 : 0;
+        before += __shfl_sync(0xffffffffu, upto - mine, at_lane);
+        b0 += at_lane;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
     at.enter(s, seq_lens, b0);
     at.w = (first - before) / at.tiles;

@@ -43,12 +43,13 @@ template <int DK, int DV, bool FP8, bool TWO>
 struct Layout {
   static constexpr uint32_t kQ = DK / 64 * kBox, kK = DK / 64 * kBox, kV = DV / 64 * kBox;
   static constexpr uint32_t kAllQ = (TWO ? 2 : 1) * kQ;
-  // operand buffers: filled by TMA (bf16), or by the converting warps from two stages of codes
-  static constexpr int kStages = FP8 ? (TWO || DK > 128 ? 1 : 2) : (TWO || DK > 128 ? 2 : DK > 64 ? 3 : 4);
-  static constexpr int kRaw = FP8 ? 2 : 0;
-  static constexpr uint32_t kRawK = kKeys * DK, kRawV = kKeys * DV;
+  // operand buffers: filled by TMA (bf16), or by the converting warps from stages of codes
+  static constexpr int kStages = FP8 ? (DK > 128 ? 1 : 2) : (TWO || DK > 128 ? 2 : DK > 64 ? 3 : 4);
+  // stages of codes: half a tile each, so that one is loaded while another is converted
+  static constexpr int kRaw = FP8 ? (TWO && DK > 64 ? 2 : 4) : 0;
+  static constexpr uint32_t kRawK = kBlock * DK, kRawV = kBlock * DV;
   static constexpr uint32_t kBytes = kAllQ + kStages * (kK + kV) + kRaw * (kRawK + kRawV);
-  static constexpr uint32_t kSmem = kBytes + 1024 + 256;
+  static constexpr uint32_t kSmem = kBytes + 1024 + 384;
   static constexpr int kThreads = FP8 ? 640 : 384;
   static_assert(kSmem <= 232448, "shared memory of a CTA");
   static_assert(!TWO || DK <= 128, "two row tiles of wider heads leave no room for the keys");
@@ -181,6 +182,10 @@ __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float sc
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+// Warps of a group that have one of its `rows` rows (one at least: a barrier counts them).  What
+// the products hold in the other warps' rows is never read.
+__device__ __forceinline__ int busy_warps(int rows) { return max(1, min(4, (rows + 31) / 32)); }
+
 // grid = (runs of positions, row tiles, key heads)
 template <int DK, int DV, bool FP8, bool TWO>
 __global__ void __launch_bounds__(Layout<DK, DV, FP8, TWO>::kThreads, 1)
@@ -196,9 +201,11 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const uint32_t bars = base + L::kBytes;
   const uint32_t k_full = bars, k_empty = k_full + 8 * 4, v_full = k_empty + 8 * 4, v_empty = v_full + 8 * 4;
   const uint32_t s_full = v_empty + 8 * 4, p_full = s_full + 8 * 4;                            // [group][buffer]
-  const uint32_t pv_done = p_full + 8 * 4;                                                    // [group], a phase per block
-  const uint32_t rk_full = pv_done + 16, rv_full = rk_full + 16, r_empty = rv_full + 16;      // two each
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(aligned_base + L::kBytes + 8 * (6 * 4 + 8));
+  // [group][buffer]; waited for at need only, so the two buffers' barriers are apart: a phase that
+  // is waited for ends before the barrier's next one can, whenever the waiting warp comes by
+  const uint32_t pv_done = p_full + 8 * 4;
+  const uint32_t rk_full = pv_done + 8 * 4, rv_full = rk_full + 8 * 4, r_empty = rv_full + 8 * 4;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(aligned_base + L::kBytes + 8 * (10 * 4));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   // (the warp's number and the TMEM address as values that are the same for the whole warp: the
@@ -210,14 +217,13 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int n = tile1 - tile0;                          // tiles of this run, at least one
   const int blocks = TWO ? 2 * n : n;                   // of each group
   const int rows = min(kRows, s.B * s.group - rt * kRows);
+  const int busy_of[2] = {busy_warps(rows), busy_warps(TWO ? rows - kPrefixRows : rows)};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
       mbar_init(k_full + 8 * i, FP8 ? 4 : 1); mbar_init(k_empty + 8 * i, 1);
       mbar_init(v_full + 8 * i, FP8 ? 4 : 1); mbar_init(v_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4);
-    }
-    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, busy_of[i >> 1]);
       mbar_init(pv_done + 8 * i, 1);
       mbar_init(rk_full + 8 * i, 1); mbar_init(rv_full + 8 * i, 1); mbar_init(r_empty + 8 * i, 8);
     }
@@ -261,16 +267,17 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   if (warp == 0) {
     if constexpr (FP8) {
       const size_t row0 = (size_t)hk * s.s_max;
-      for (int i = 0; i < n; ++i) {
-        const int st = i & 1, key = (tile0 + i) * kKeys;
-        const uint32_t keys = min(kKeys, s.shared_len - key);
-        if (!__all_sync(0xffffffffu, mbar_wait(r_empty + 8 * st, ((i >> 1) & 1) ^ 1u, abort_flag))) break;
+      for (int i = 0; i < 2 * n; ++i) {
+        const int st = i % L::kRaw, key = tile0 * kKeys + i * kBlock;
+        const uint32_t keys = max(0, min(kBlock, s.shared_len - key));       // (none: the barrier completes at once)
+        if (!__all_sync(0xffffffffu, mbar_wait(r_empty + 8 * st, ((i / L::kRaw) & 1) ^ 1u, abort_flag))) break;
         if (elect_one()) {
           const uint32_t dst = raw_smem + st * (L::kRawK + L::kRawV);
           mbar_expect_tx(rk_full + 8 * st, keys * DK);
-          bulk_load(dst, static_cast<const uint8_t *>(cache.k) + (row0 + key) * DK, keys * DK, rk_full + 8 * st);
+          if (keys > 0) bulk_load(dst, static_cast<const uint8_t *>(cache.k) + (row0 + key) * DK, keys * DK, rk_full + 8 * st);
           mbar_expect_tx(rv_full + 8 * st, keys * DV);
-          bulk_load(dst + L::kRawK, static_cast<const uint8_t *>(cache.v) + (row0 + key) * DV, keys * DV, rv_full + 8 * st);
+          if (keys > 0)
+            bulk_load(dst + L::kRawK, static_cast<const uint8_t *>(cache.v) + (row0 + key) * DV, keys * DV, rv_full + 8 * st);
         }
       }
     } else {
@@ -339,7 +346,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
           for (int x = 0; x < kBlock / 16; ++x)
             tc_mma_ts(o_tmem + w * DV, s_tmem + (2 * w + (j & 1)) * kBlock + x * 8, b + (uint64_t)(x * (2048 >> 4)), id_o, j > 0 || x > 0);
-          tc_commit(pv_done + 8 * w);
+          tc_commit(pv_done + 8 * (2 * w + (j & 1)));
           if (w == 1 && (!TWO || (j & 1))) tc_commit(v_empty + 8 * st);
         }
         __syncwarp();
@@ -351,7 +358,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const uint32_t ot_at = o_tmem + w * DV + lane_at;
     float m = kNone, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < blocks; ++j) {
+    const bool busy = (warp & 3) < busy_of[w];
+    for (int j = 0; busy && j < blocks; ++j) {
       const uint32_t st_at = s_tmem + (2 * w + (j & 1)) * kBlock + lane_at;
       ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (2 * w + (j & 1)), (j >> 1) & 1, abort_flag));
       if (!ok) break;
@@ -364,8 +372,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         l *= f;
         m = up;
         if (j > 0) {
-          // (the products of the blocks before the last are behind these scores; the last one's may be under way)
-          ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * w, (j - 1) & 1, abort_flag));
+          // (block j - 2's product into the accumulator is behind these scores; block j - 1's may be under way)
+          ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * (2 * w + ((j - 1) & 1)), ((j - 1) >> 1) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -395,8 +403,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       if (TWO) asm volatile("bar.sync %0, 128;" ::"r"(2 + w) : "memory");
       else asm volatile("bar.sync 1, 256;" ::: "memory");
     };
-    if (ok) ok = __all_sync(0xffffffffu, blocks < 2 || mbar_wait(pv_done + 8 * w, (blocks - 2) & 1, abort_flag));
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * w, (blocks - 1) & 1, abort_flag));
+    // (completion is in order: the last block's product is behind all others)
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 8 * (2 * w + ((blocks - 1) & 1)), ((blocks - 1) >> 1) & 1, abort_flag));
     tc_fence_after();
     asm volatile("bar.sync 1, 256;" ::: "memory");                                       // both groups' products
     constexpr int kPitch = DV + 4;
@@ -415,7 +423,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     float4 *row_at = reinterpret_cast<float4 *>(rows_at + (w * kPrefixRows + row) * kPitch);
 #pragma unroll 1
-    for (int x = 0; x < DV; x += 32) {
+    for (int x = 0; busy && x < DV; x += 32) {
       uint32_t r[32];
       tc_ld32(ot_at + x, r);
       tc_wait_ld();
@@ -443,43 +451,48 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     tc_fence_before();
   } else if (FP8 && warp >= kConvertWarp) {
-    // One row of codes per thread, keys in one group of four warps and values in the other.  The
-    // chunks of a row in an order that keeps eight neighbouring rows on different banks, in the
-    // codes and in the swizzled operand.
+    // Half a row of codes per thread, keys in one group of four warps and values in the other.  A
+    // thread's chunks are every second one from a place that moves with the row: eight
+    // neighbouring rows are on different banks, in the codes and in the swizzled operand.
     const bool keys_side = warp < kConvertWarp + 4;
-    const int row = (warp & 3) * 32 + lane;
+    const int row = threadIdx.x & 63, part = (threadIdx.x >> 6) & 1;
     const size_t row0 = (size_t)hk * s.s_max;
     const uint8_t *scales = keys_side ? cache.ks : cache.vs;
     const uint32_t full = keys_side ? k_full : v_full, empty = keys_side ? k_empty : v_empty, raw_full = keys_side ? rk_full : rv_full;
     const uint32_t op_smem = keys_side ? k_smem : v_smem, op_bytes = keys_side ? L::kK : L::kV;
-    const int d = keys_side ? DK : DV, chunks = d / 16, start = row % chunks;
+    const int d = keys_side ? DK : DV, chunks = d / 16, start = (row + part) % chunks;
     const auto scale_at = [&](int i) {
-      const int key = (tile0 + i) * kKeys + row;
-      return i < n && key < s.shared_len ? (uint32_t)__ldg(scales + row0 + key) : 0u;
+      const int key = tile0 * kKeys + i * kBlock + row;
+      return i < 2 * n && key < s.shared_len ? (uint32_t)__ldg(scales + row0 + key) : 0u;
     };
     uint32_t byte = scale_at(0);
-    for (int i = 0; i < n; ++i) {
-      const int st = i & 1, op = i % NS;
-      const bool in = (tile0 + i) * kKeys + row < s.shared_len;
+    for (int i = 0; i < 2 * n; ++i) {
+      const int st = i % L::kRaw, op = (i >> 1) % NS;
+      const bool in = tile0 * kKeys + i * kBlock + row < s.shared_len;
       const uint32_t next = scale_at(i + 1);
-      const bool ok = mbar_wait(raw_full + 8 * st, (i >> 1) & 1, abort_flag) && mbar_wait(empty + 8 * op, ((i / NS) & 1) ^ 1u, abort_flag);
+      bool ok = mbar_wait(raw_full + 8 * st, (i / L::kRaw) & 1, abort_flag);
+      if (!(i & 1)) ok = ok && mbar_wait(empty + 8 * op, (((i >> 1) / NS) & 1) ^ 1u, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) break;
       const unsigned char *src = aligned_base + (raw_smem - base) + st * (L::kRawK + L::kRawV) + (keys_side ? 0 : L::kRawK) + row * d;
       unsigned char *dst = aligned_base + (op_smem - base) + op * op_bytes;
       const float scale = e8m0_value(byte);
+      const int op_row = (i & 1) * kBlock + row;
       int chunk = start;
 #pragma unroll 4
-      for (int x = 0; x < chunks; ++x) {
+      for (int x = 0; x < chunks / 2; ++x) {
         uint4 c = make_uint4(0, 0, 0, 0), lo, hi;
         if (in) c = *reinterpret_cast<const uint4 *>(src + chunk * 16);       // (behind the end stands whatever was there before)
         convert16(c, in ? scale : 0.f, lo, hi);
-        *reinterpret_cast<uint4 *>(dst + swizzled(row, 2 * chunk)) = lo;
-        *reinterpret_cast<uint4 *>(dst + swizzled(row, 2 * chunk + 1)) = hi;
-        chunk = chunk + 1 == chunks ? 0 : chunk + 1;
+        *reinterpret_cast<uint4 *>(dst + swizzled(op_row, 2 * chunk)) = lo;
+        *reinterpret_cast<uint4 *>(dst + swizzled(op_row, 2 * chunk + 1)) = hi;
+        chunk = chunk + 2 >= chunks ? chunk + 2 - chunks : chunk + 2;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) { mbar_arrive(full + 8 * op); mbar_arrive(r_empty + 8 * st); }
+      if (lane == 0) {
+        mbar_arrive(r_empty + 8 * st);
+        if (i & 1) mbar_arrive(full + 8 * op);
+      }
       byte = next;
     }
   }

@@ -504,3 +504,23 @@ def test_long_shared_prefix(kind, b, n_q, n_kv, dk, dv, shared, slope):
     want, tol = _want(q, kk, vv, lens, shared, 1.0)
     assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() - tol).max())
     assert float((got.double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
+
+
+@pytest.mark.parametrize("kind,b,n_q,n_kv,d,shared", [("fp8", 64, 32, 4, 128, 4096), ("bf16", 40, 16, 16, 128, 2050),
+                                                      ("fp8", 18, 6, 2, 64, 3000), ("bf16", 200, 8, 4, 64, 1500)])
+def test_calls_back_to_back_end_in_time_with_the_same_bits(kind, b, n_q, n_kv, d, shared):
+    """Hundreds of calls with nothing between them: no wait inside runs out, every one gives the same bits."""
+    s_max = shared + 30
+    q, k, v = _rand(b, n_q, d, seed=1), _rand(b, n_kv, s_max, d, seed=2), _rand(b, n_kv, s_max, d, seed=3)
+    lens = torch.tensor([shared + i % 30 for i in range(b)], dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    if kind == "fp8":
+        cache = QuantizedCache(*_quantized(k), *_quantized(v))
+        call = lambda: ops.attn_decode_quantized(q, cache, lens, shared, status=status)      # noqa: E731
+    else:
+        ck, cv = k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
+        call = lambda: ops.attn_decode_shared(q, ck, cv, lens, shared, status=status)        # noqa: E731
+    want, wrong = call(), torch.zeros((), dtype=torch.int64, device=DEV)
+    for _ in range(300):
+        wrong += (call() != want).sum()
+    assert int(status) == 0 and int(wrong) == 0
