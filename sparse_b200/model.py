@@ -23,6 +23,13 @@ and replayed per token; positions and token ids live in device buffers that
 the graph itself advances.  Prefill runs the same layers on chunks of the
 prompt with the library's fused attention over the cache.
 
+`kv_cache="fp8"` keeps keys and values as 8-bit codes (`kv_cache.QuantizedCache`): the
+rotary kernel quantises them as it writes, decode attention reads the codes, prompt
+chunks attend to the codes read back as bf16.  `prefill(ids, shared_len=n)` takes the
+first n ids of every sequence as the same ones (a system prompt): they are computed
+once, stand in the cache of sequence 0 only, and every decode step reads them once for
+the whole batch.  (The reference has neither: its cache is the Transformers one.)
+
 Under expert parallelism every rank holds the whole model except the experts
 it does not own, and its own share of the sequences (data-parallel attention,
 expert-parallel MoE), as the reference's EP group does.
@@ -41,6 +48,7 @@ from . import _lib, ops, synth
 from ._lib import lib, check
 from .block import B200MoeBlock
 from .context import Metrics, SparseContext
+from .kv_cache import QuantizedCache
 from .layer import LayerWeights
 
 
@@ -105,8 +113,11 @@ class ShapedMoeModel:
 
     def __init__(self, cfg: ModelConfig, device: torch.device, batch: int, max_seq: int, seed: int = 0,
                  ep_rank: int = 0, ep_size: int = 1, process_group=None, owner_of: Optional[Sequence[int]] = None,
-                 chunk_tokens: int = 4096):
+                 chunk_tokens: int = 4096, kv_cache: str = "bf16"):
+        if kv_cache not in ("bf16", "fp8"):
+            raise ValueError("kv_cache=%r: a model keeps its keys and values as 'bf16' or 'fp8'" % (kv_cache,))
         self.cfg, self.device, self.batch, self.max_seq = cfg, device, batch, max_seq
+        self.kv_cache, self.shared_len = kv_cache, 0
         self.ep_rank, self.ep_size = ep_rank, ep_size
         h, bf = cfg.hidden, torch.bfloat16
         dev_index = device.index if device.index is not None else torch.cuda.current_device()
@@ -140,8 +151,11 @@ class ShapedMoeModel:
                 ly.wqkv = _normal((nh * dk + nkv * dk + nkv * dv, h), device, s0 + 1)
                 ly.bqkv = _normal((nh * dk + nkv * dk + nkv * dv,), device, s0 + 2) if cfg.qkv_bias else None
             ly.wo = _normal((h, nh * dv), device, s0 + 4)
-            ly.cache_k = torch.zeros((batch, max_seq, nkv, dk), dtype=bf, device=device)
-            ly.cache_v = torch.zeros((batch, max_seq, nkv, dv), dtype=bf, device=device)
+            if kv_cache == "fp8":
+                ly.cache = QuantizedCache.zeros(batch, max_seq, nkv, dk, dv, device)
+            else:
+                ly.cache_k = torch.zeros((batch, max_seq, nkv, dk), dtype=bf, device=device)
+                ly.cache_v = torch.zeros((batch, max_seq, nkv, dv), dtype=bf, device=device)
             if l in cfg.dense_layers:
                 inter = cfg.dense_layers[l]
                 ly.dense_w13 = _normal((1, 2 * inter, h), device, s0 + 5)
@@ -164,6 +178,7 @@ class ShapedMoeModel:
         self.n_split = max(1, min(64, (6 * sms + batch * nh - 1) // (batch * nh), (max_seq + 63) // 64))
         ws = lib.sb_attn_decode_workspace_bytes(batch, nh, dv, self.n_split)
         self.attn_ws = torch.empty((ws,), dtype=torch.uint8, device=device)
+        self.attn_status = torch.zeros((1,), dtype=torch.int32, device=device)
         # decode-step state advanced by the graph itself
         self.cur_ids = torch.zeros((batch,), dtype=torch.int64, device=device)
         self.cur_pos = torch.zeros((batch,), dtype=torch.int32, device=device)
@@ -185,7 +200,7 @@ class ShapedMoeModel:
 
     def _qkv_rope_append(self, ly: _Layer, x: torch.Tensor, seq_of_token, pos_of_token) -> torch.Tensor:
         """Projections of the rows, rotary embedding, keys and values into the cache;
-        returns the rotated queries (a column slice of the projection output)."""
+        returns the rotated queries (bf16 cache: a column slice of the projection output)."""
         cfg = self.cfg
         nh, nkv, dk, dv, t = cfg.n_heads, cfg.n_kv_heads, cfg.qk_dim, cfg.v_dim, x.shape[0]
         if cfg.attention == "mla":
@@ -200,6 +215,11 @@ class ShapedMoeModel:
             check(lib.sb_rmsnorm_rows(latent.data_ptr(), latent.stride(0), ly.kv_norm.data_ptr(), cfg.rms_eps, t, lora,
                                       c_kv.data_ptr(), self._s()), "sb_rmsnorm_rows")
             kv = ops.linear(c_kv, ly.wkv_b)                             # per head: [nope | v]
+            if self.kv_cache == "fp8":
+                heads = kv.view(t, nh, nope + dv)
+                return ops.rope_append_quantized(q.view(t, nh, dk), k_pe.view(t, 1, rope),
+                                                 heads[..., :nope] if nope else None, heads[..., nope:], seq_of_token,
+                                                 pos_of_token, ly.cache, cfg.rope_theta).view(t, nh * dk)
             check(lib.sb_rope_append_mla(q.data_ptr(), k_pe.data_ptr(), kv.data_ptr(), seq_of_token.data_ptr(),
                                          pos_of_token.data_ptr(), t, nh, rope, nope, dv, cfg.rope_theta, self.max_seq,
                                          ly.cache_k.data_ptr(), ly.cache_v.data_ptr(), q.stride(0), k_pe.stride(0),
@@ -208,6 +228,11 @@ class ShapedMoeModel:
         # column slices of the fused projection: the kernels take the token stride
         qkv = ops.linear(x, ly.wqkv, ly.bqkv)
         q, k, v = qkv[:, :nh * dk], qkv[:, nh * dk:nh * dk + nkv * dk], qkv[:, nh * dk + nkv * dk:]
+        if self.kv_cache == "fp8":
+            keys, rope = k.view(t, nkv, dk), cfg.rope_dim
+            return ops.rope_append_quantized(q.view(t, nh, dk), keys[..., :rope] if rope else None,
+                                             keys[..., rope:] if rope < dk else None, v.view(t, nkv, dv), seq_of_token,
+                                             pos_of_token, ly.cache, cfg.rope_theta).view(t, nh * dk)
         check(lib.sb_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), seq_of_token.data_ptr(),
                                  pos_of_token.data_ptr(), t, nh, nkv, dk, dv, cfg.rope_dim, cfg.rope_theta,
                                  self.max_seq, ly.cache_k.data_ptr(), ly.cache_v.data_ptr(), q.stride(0), k.stride(0),
@@ -228,6 +253,19 @@ class ShapedMoeModel:
         return out
 
     # -- prefill -----------------------------------------------------------------------------
+    def _cached(self, ly: _Layer, b: int, kv_len: int):
+        """Keys and values of the first kv_len positions of b sequences, [b, n_kv, kv_len, d] bf16.
+        Positions below `shared_len` stand in sequence 0's rows."""
+        if self.kv_cache == "fp8":
+            c = ly.cache
+            return ops.cache_read(QuantizedCache(c.k[:b], c.k_scale[:b], c.v[:b], c.v_scale[:b]), 0, kv_len,
+                                  min(self.shared_len, kv_len))
+        shared = self.shared_len if b > 1 else 0
+        if shared == 0:
+            return ly.cache_k[:b, :kv_len].transpose(1, 2), ly.cache_v[:b, :kv_len].transpose(1, 2)
+        return tuple(torch.cat([c[:1, :shared].expand(b, -1, -1, -1), c[:b, shared:kv_len]], dim=1).transpose(1, 2)
+                     for c in (ly.cache_k, ly.cache_v))
+
     def _prefill_chunk(self, ids: torch.Tensor, past: int) -> torch.Tensor:
         """ids [B, Tc] at positions past..past+Tc-1 -> hidden state of every token [B*Tc, H] (before the final norm)."""
         cfg, b, tc = self.cfg, ids.shape[0], ids.shape[1]
@@ -247,8 +285,7 @@ class ShapedMoeModel:
             x = self._norm(resid, delta, ly.ln1)
             q = self._qkv_rope_append(ly, x, seq, pos)
             qh = q.reshape(b, tc, nh, dk).transpose(1, 2)
-            kh = ly.cache_k[:b, :kv_len].transpose(1, 2)
-            vh = ly.cache_v[:b, :kv_len].transpose(1, 2)
+            kh, vh = self._cached(ly, b, kv_len)
             if nkv != nh:
                 kh = kh.repeat_interleave(nh // nkv, dim=1)
                 vh = vh.repeat_interleave(nh // nkv, dim=1)
@@ -264,14 +301,27 @@ class ShapedMoeModel:
                                  self._s()), "sb_add_rmsnorm")
         return resid
 
-    def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
-        """input_ids [B, S] -> logits of the last position [B, V] (fp32); fills the cache."""
+    def prefill(self, input_ids: torch.Tensor, shared_len: int = 0) -> torch.Tensor:
+        """input_ids [B, S] -> logits of the last position [B, V] (fp32); fills the cache.
+
+        shared_len < S: as many first ids are the same in every row.  They are computed for
+        sequence 0 and stored in its rows of the cache only; until the next `prefill` the decode
+        steps read them there, once for the whole batch."""
         b, s = input_ids.shape
         if b != self.batch or s >= self.max_seq:
             raise RuntimeError("model was built for batch %d and fewer than %d positions" % (self.batch, self.max_seq))
+        if not 0 <= shared_len < s:
+            raise RuntimeError("%d shared ids of a prompt of %d: at least the last one is a sequence's own" % (shared_len, s))
+        if shared_len > 0 and not bool((input_ids[:, :shared_len] == input_ids[:1, :shared_len]).all()):
+            raise RuntimeError("the first %d ids are not the same in every sequence" % shared_len)
+        if shared_len != self.shared_len:
+            self._graph = None                           # recorded with another shared length
+        self.shared_len = shared_len
+        for p0 in range(0, shared_len, self.chunk_tokens):
+            self._prefill_chunk(input_ids[:1, p0:min(p0 + self.chunk_tokens, shared_len)].contiguous(), p0)
         per_seq = max(1, self.chunk_tokens // b)
         last = None
-        for p0 in range(0, s, per_seq):
+        for p0 in range(shared_len, s, per_seq):
             chunk = input_ids[:, p0:p0 + per_seq].contiguous()
             hidden = self._prefill_chunk(chunk, p0)
             last = hidden.view(b, chunk.shape[1], -1)[:, -1, :].contiguous()
@@ -280,22 +330,33 @@ class ShapedMoeModel:
         return F.linear(normed, self.lm_head).float()
 
     # -- decode ------------------------------------------------------------------------------
+    def _decode_attention(self, ly: _Layer, q: torch.Tensor) -> torch.Tensor:
+        """q [B, n_q * dk] against the cached positions of every sequence -> [B, n_q * dv]."""
+        cfg, b = self.cfg, self.batch
+        nh, nkv, dk, dv, scale = cfg.n_heads, cfg.n_kv_heads, cfg.qk_dim, cfg.v_dim, 1.0 / math.sqrt(cfg.qk_dim)
+        if self.kv_cache == "fp8":
+            return ops.attn_decode_quantized(q.view(b, nh, dk), ly.cache, self.seq_lens, self.shared_len, scale,
+                                             self.attn_status).view(b, nh * dv)
+        if self.shared_len > 0:
+            return ops.attn_decode_shared(q.view(b, nh, dk), ly.cache_k, ly.cache_v, self.seq_lens, self.shared_len, scale,
+                                          self.attn_status).view(b, nh * dv)
+        att = torch.empty((b, nh * dv), dtype=torch.bfloat16, device=self.device)
+        check(lib.sb_attn_decode(q.data_ptr(), q.stride(0), ly.cache_k.data_ptr(), ly.cache_v.data_ptr(),
+                                 self.seq_lens.data_ptr(), b, nh, nkv, dk, dv, self.max_seq, scale, self.n_split,
+                                 self.attn_ws.data_ptr(), self.attn_ws.numel(), att.data_ptr(), self._s()), "sb_attn_decode")
+        return att
+
     def _decode_body(self) -> None:
         """One token per sequence: reads cur_ids/cur_pos, appends to the cache,
         writes the next ids back and advances the positions."""
         cfg, b = self.cfg, self.batch
-        nh, nkv, dk, dv = cfg.n_heads, cfg.n_kv_heads, cfg.qk_dim, cfg.v_dim
         resid = self.embed.index_select(0, self.cur_ids)
         torch.add(self.cur_pos, 1, out=self.seq_lens)
         delta = None
         for ly in self.layers:
             x = self._norm(resid, delta, ly.ln1)
             q = self._qkv_rope_append(ly, x, self.seq_ids, self.cur_pos)
-            att = torch.empty((b, nh * dv), dtype=torch.bfloat16, device=self.device)
-            check(lib.sb_attn_decode(q.data_ptr(), q.stride(0), ly.cache_k.data_ptr(), ly.cache_v.data_ptr(),
-                                     self.seq_lens.data_ptr(), b, nh, nkv, dk, dv, self.max_seq,
-                                     1.0 / math.sqrt(dk), self.n_split, self.attn_ws.data_ptr(),
-                                     self.attn_ws.numel(), att.data_ptr(), self._s()), "sb_attn_decode")
+            att = self._decode_attention(ly, q)
             attn_out = ops.linear(att, ly.wo)
             x2 = self._norm(resid, attn_out, ly.ln2)
             delta = self._mlp(ly, x2)
@@ -332,6 +393,8 @@ class ShapedMoeModel:
         for ly in self.layers:
             if ly.block is not None:
                 ly.block.check_status()
+        if int(self.attn_status.item()) != 0:
+            raise RuntimeError("decode attention: a bounded wait gave up (status %d)" % int(self.attn_status.item()))
 
 
 class RunningStats:
@@ -363,14 +426,15 @@ class RunningStats:
 
 def greedy_decode_profiled(model: ShapedMoeModel, input_ids: torch.Tensor, attention_mask, max_new_tokens: int,
                            env, metrics: Optional[Metrics], measure_ttft: bool, use_graph: bool = True,
-                           per_step_sync: bool = False) -> torch.Tensor:
+                           per_step_sync: bool = False, shared_len: int = 0) -> torch.Tensor:
     """Prefill, then `max_new_tokens - 1` decode steps, greedy; returns
     [B, prompt + max_new_tokens] ids.  Same arguments and the same wall-clock
     bookkeeping as the reference's loop (utils/eval_core.py:18464-18607):
     `metrics.wall_prefill_ms`, `wall_ttft_ms`, `wall_decode_ms`, and one sample
     per step in `metrics.decode_step_stats` when `per_step_sync` asks for the
     reference's per-step synchronisation.  `attention_mask` must be all ones
-    (prompts of equal length), as the launchers produce with `--prompt-len`."""
+    (prompts of equal length), as the launchers produce with `--prompt-len`.
+    `shared_len`: as many first ids are the same in every prompt (`ShapedMoeModel.prefill`)."""
     if attention_mask is not None and not bool(attention_mask.all()):
         raise NotImplementedError("padded prompts are not built; pass prompts of equal length")
     dev = model.device
@@ -379,7 +443,7 @@ def greedy_decode_profiled(model: ShapedMoeModel, input_ids: torch.Tensor, atten
     SparseContext.current_phase = "prefill"
     SparseContext.begin_runtime_call(0)
     t0 = time.perf_counter()
-    logits = model.prefill(input_ids)
+    logits = model.prefill(input_ids, shared_len)
     next_token = torch.argmax(logits, dim=-1)
     model.cur_ids.copy_(next_token)
     torch.cuda.synchronize(dev)
