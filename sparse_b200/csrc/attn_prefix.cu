@@ -27,6 +27,8 @@
 // through `status`, waits for its copies and frees its TMEM.
 #include <math.h>
 
+#include <atomic>
+
 #include "attn_cached.cuh"
 #include "sb_tc.cuh"
 
@@ -545,7 +547,15 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float
     if (rc != SB_OK) return rc;
   }
   auto kern = attn_prefix_kernel<DK, DV, FP8, TWO>;
-  SB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
+  // once per device and instance (setting it twice does no harm)
+  static std::atomic<uint64_t> opted_in{0};
+  int dev = 0;
+  SB_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(opted_in.load(std::memory_order_relaxed) & bit)) {
+    SB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
+    opted_in.fetch_or(bit, std::memory_order_relaxed);
+  }
   const dim3 grid(s.pre_splits, prefix_row_tiles(s), s.n_kv);
   SB_CUDA_CHECK(launch_pdl(kern, grid, dim3(L::kThreads), L::kSmem, stream, tm_k, tm_v, q, cache, s, part, lse, status));
   SB_LAUNCH_CHECK();

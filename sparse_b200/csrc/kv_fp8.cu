@@ -230,6 +230,24 @@ cache_read_fp8_kernel(const uint8_t *__restrict__ codes_k, const uint8_t *__rest
   }
 }
 
+// The frequencies of a model are the same in every call: a thread keeps the last table.
+const RopeFreq &rope_freq(float theta, int rope_dim) {
+  static thread_local RopeFreq kept;
+  static thread_local float kept_theta = 0.f;
+  static thread_local int kept_dim = -1;
+  if (kept_theta != theta || kept_dim != rope_dim) {
+    const double log_theta = log((double)theta);
+    for (int j = 0; j < rope_dim / 2; ++j) {
+      const double turns = exp(-2.0 * j / rope_dim * log_theta) / (2.0 * M_PI);
+      kept.turns[j].x = (float)turns;
+      kept.turns[j].y = (float)(turns - (double)kept.turns[j].x);
+    }
+    kept_theta = theta;
+    kept_dim = rope_dim;
+  }
+  return kept;
+}
+
 bool head_ok(int d) { return d >= 16 && d <= kMaxHead && d % 16 == 0; }
 
 }  // namespace
@@ -261,12 +279,7 @@ int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest,
     src[i] = RowSource{static_cast<const __nv_bfloat16 *>(base[i]), strides[2 * i], strides[2 * i + 1]};
     vec = vec && aligned(base[i], 16) && strides[2 * i] % 8 == 0 && strides[2 * i + 1] % 8 == 0;
   }
-  RopeFreq freq = {};
-  for (int j = 0; j < rope_dim / 2; ++j) {
-    const double turns = exp(-2.0 * j / rope_dim * log((double)theta)) / (2.0 * M_PI);
-    freq.turns[j].x = (float)turns;
-    freq.turns[j].y = (float)(turns - (double)freq.turns[j].x);
-  }
+  const RopeFreq &freq = rope_freq(theta, rope_dim);
   const int widest = dk > dv ? dk : dv;
   const int lanes = widest <= 64 ? 4 : widest <= 128 ? 8 : 16;
   // at most two waves of CTAs: more would only repeat the angle table

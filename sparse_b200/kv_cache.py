@@ -21,14 +21,15 @@ class QuantizedCache:
     __slots__ = ("k", "k_scale", "v", "v_scale")
 
     def __init__(self, k: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor, v_scale: torch.Tensor):
-        rows = k.shape[:3]
-        if k.dim() != 4 or v.dim() != 4 or not rows == v.shape[:3] == k_scale.shape == v_scale.shape:
+        shape = k.shape
+        rows = shape[:3]
+        if len(shape) != 4 or v.dim() != 4 or v.shape[:3] != rows or k_scale.shape != rows or v_scale.shape != rows:
             raise RuntimeError("QuantizedCache: codes [B, n_kv, S, d] and scales [B, n_kv, S] do not fit: %s" % (
                 [tuple(t.shape) for t in (k, k_scale, v, v_scale)],))
-        device = k.device
-        for t, dtype in ((k, CODES), (k_scale, SCALES), (v, CODES), (v_scale, SCALES)):
-            if t.dtype != dtype or t.device != device or not t.is_contiguous():
-                raise RuntimeError("QuantizedCache needs contiguous %s codes and %s scales on one device" % (CODES, SCALES))
+        if k.dtype != CODES or v.dtype != CODES or k_scale.dtype != SCALES or v_scale.dtype != SCALES or not (
+                k.get_device() == v.get_device() == k_scale.get_device() == v_scale.get_device()) or not (
+                k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            raise RuntimeError("QuantizedCache needs contiguous %s codes and %s scales on one device" % (CODES, SCALES))
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
 
     @classmethod

@@ -7,6 +7,7 @@ of the tensors' device and never synchronise.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -206,23 +207,19 @@ def combine(rows_out: torch.Tensor, slot_of_item: torch.Tensor, idx: torch.Tenso
 _Strides = ctypes.c_int64 * 8
 
 
-class _On:
-    """`with _On(index)`: that device is the current one."""
-    __slots__ = ("index", "guard")
+def _call(fn, what: str, device: int, *args) -> None:
+    """fn(*args, stream) with `device` current, its current stream; raises on a status."""
+    if torch._C._cuda_getDevice() == device:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status != 0:
+        check(status, what)
 
-    def __init__(self, index: int):
-        self.index = index
 
-    def __enter__(self) -> int:
-        self.guard = None
-        if torch.cuda.current_device() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+# (the sizes of a serving loop's calls are few: one look-up instead of a call into the library)
+_attn_workspace = functools.lru_cache(maxsize=1024)(lib.sb_attn_cached_workspace_bytes)
 
 
 def _index(t: torch.Tensor, n: int, device: int, what: str) -> int:
@@ -276,10 +273,9 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
     seq = _index(seq_of_token, t, device, "rope_append_quantized: seq_of_token")
     pos = _index(pos_of_token, t, device, "rope_append_quantized: pos_of_token")
     out = q.new_empty((t, n_q, dk))
-    with _On(device) as stream:
-        check(lib.sb_rope_append_fp8(*ptrs, seq, pos, t, b, n_q, n_kv, dk, dv, rope, theta, s_max, _Strides(*strides),
-                                     out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
-                                     cache.v_scale.data_ptr(), stream), "sb_rope_append_fp8")
+    _call(lib.sb_rope_append_fp8, "sb_rope_append_fp8", device, *ptrs, seq, pos, t, b, n_q, n_kv, dk, dv, rope, theta, s_max,
+          _Strides(*strides), out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
+          cache.v_scale.data_ptr())
     return out
 
 
@@ -295,10 +291,8 @@ def cache_read(cache: QuantizedCache, begin: int, count: int, shared_len: int = 
             begin, begin + count, shared_len, s_max))
     k = cache.k.new_empty((b, n_kv, count, dk), dtype=torch.bfloat16)
     v = cache.k.new_empty((b, n_kv, count, dv), dtype=torch.bfloat16)
-    with _On(device) as stream:
-        check(lib.sb_cache_read_fp8(cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(),
-                                    b, n_kv, dk, dv, s_max, begin, count, shared_len, k.data_ptr(), v.data_ptr(), stream),
-              "sb_cache_read_fp8")
+    _call(lib.sb_cache_read_fp8, "sb_cache_read_fp8", device, cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
+          cache.v_scale.data_ptr(), b, n_kv, dk, dv, s_max, begin, count, shared_len, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -306,11 +300,12 @@ def _decode_attention(name: str, call, q: torch.Tensor, cache_ptrs, seq_lens: to
                       dv: int, s_max: int, shared_len: int, scale: Optional[float], status: Optional[torch.Tensor],
                       device: int) -> torch.Tensor:
     """Checks of the operands that both kinds of cache share, output and workspace, the call."""
-    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.get_device() != device or q.shape[0] != b or q.shape[2] != dk or (
-            q.shape[1] < 1):
+    shape = q.shape
+    if len(shape) != 3 or q.dtype != torch.bfloat16 or q.get_device() != device or shape[0] != b or shape[2] != dk or (
+            shape[1] < 1):
         raise RuntimeError("%s: q must be bf16 [%d, n_q, %d] on the cache's device, got %s %s on %s" % (
-            name, b, dk, q.dtype, tuple(q.shape), q.device))
-    n_q = q.shape[1]
+            name, b, dk, q.dtype, tuple(shape), q.device))
+    n_q = shape[1]
     seq_stride, head_stride, element = q.stride()
     if b > 0 and (element != 1 or (n_q > 1 and head_stride != dk) or (b > 1 and seq_stride < n_q * dk)):
         raise RuntimeError("%s: the heads of a sequence's query must lie side by side, sequences apart" % name)
@@ -320,12 +315,11 @@ def _decode_attention(name: str, call, q: torch.Tensor, cache_ptrs, seq_lens: to
         raise RuntimeError("%s: status must be int32 on the cache's device" % name)
     lens = _index(seq_lens, b, device, name)
     out = q.new_empty((b, n_q, dv))
-    ws_bytes = lib.sb_attn_cached_workspace_bytes(b, n_q, n_kv, dk, dv, s_max, shared_len) or 16
+    ws_bytes = _attn_workspace(b, n_q, n_kv, dk, dv, s_max, shared_len) or 16
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
-    with _On(device) as stream:
-        check(call(q.data_ptr(), seq_stride if b > 1 else 0, *cache_ptrs, lens, b, n_q, n_kv, dk, dv, s_max, shared_len,
-                   dk ** -0.5 if scale is None else scale, ws.data_ptr(), ws_bytes, out.data_ptr(),
-                   None if status is None else status.data_ptr(), stream), name)
+    _call(call, name, device, q.data_ptr(), seq_stride if b > 1 else 0, *cache_ptrs, lens, b, n_q, n_kv, dk, dv, s_max,
+          shared_len, dk ** -0.5 if scale is None else scale, ws.data_ptr(), ws_bytes, out.data_ptr(),
+          None if status is None else status.data_ptr())
     return out
 
 
