@@ -238,7 +238,9 @@ HEADS = [(16, 16, 128, 128), (16, 16, 192, 128), (4, 2, 64, 64), (8, 1, 128, 128
 @pytest.mark.parametrize("n_q,n_kv,dk,dv", HEADS)
 @pytest.mark.parametrize("lens,shared,s_max", [
     ([1], 0, 1), ([0, 3, 65, 64, 63, 130], 0, 131), ([700], 0, 701), ([700, 0, 257], 0, 777), ([1025, 5, 1025], 5, 1030),
-    ([300, 301, 200, 0, 299, 333], 300, 340), ([17, 17], 17, 17), ([129] * 9, 128, 140)])
+    ([300, 301, 200, 0, 299, 333], 300, 340), ([17, 17], 17, 17), ([129] * 9, 128, 140),
+    # as many sequences as make the shared positions a pass of their own for all these heads
+    ([130, 70, 0, 127, 128, 129, 131, 257] * 40, 128, 260), ([1000, 77, 0, 999, 1001, 1064, 1066, 1200] * 9, 1000, 1200)])
 def test_attention(kind, n_q, n_kv, dk, dv, lens, shared, s_max):
     b = len(lens)
     q, k, v = _rand(b, n_q, dk, seed=b), _rand(b, n_kv, s_max, dk, seed=s_max), _rand(b, n_kv, s_max, dv, seed=7)
@@ -251,7 +253,9 @@ def test_attention(kind, n_q, n_kv, dk, dv, lens, shared, s_max):
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 @pytest.mark.parametrize("b,n_q,n_kv,dk,dv,shared", [(1, 16, 16, 128, 128, 0), (2, 8, 2, 64, 64, 190), (5, 16, 4, 192, 128, 190),
-                                                     (40, 4, 2, 128, 128, 190), (70, 8, 2, 64, 64, 257)])
+                                                     (40, 4, 2, 128, 128, 190), (70, 8, 2, 64, 64, 257),
+                                                     (90, 8, 8, 128, 128, 190), (150, 16, 16, 64, 64, 257),
+                                                     (40, 48, 16, 128, 128, 190), (90, 16, 8, 192, 128, 193)])
 def test_every_position_is_found(kind, b, n_q, n_kv, dk, dv, shared):
     """A key that answers the query alone: the output is its value, wherever it stands."""
     s_max = 300
@@ -271,11 +275,11 @@ def test_every_position_is_found(kind, b, n_q, n_kv, dk, dv, shared):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
-@pytest.mark.parametrize("b", [2, 40])
-def test_masked_places_may_hold_anything(kind, b):
+@pytest.mark.parametrize("b,n_kv", [(2, 2), (40, 2), (200, 8)])
+def test_masked_places_may_hold_anything(kind, b, n_kv):
     """NaN and infinities behind a sequence's end, and in the shared positions of a sequence that ends inside them,
     change nothing; a sequence that sees one has NaN."""
-    n_q, n_kv, d, s_max, shared = 4, 2, 64, 200, 100
+    n_q, d, s_max, shared = 2 * n_kv, 64, 200, 100
     lens = [150] * (b - 1) + [90]
     q, k, v = _rand(b, n_q, d, seed=1), _rand(b, n_kv, s_max, d, seed=2), _rand(b, n_kv, s_max, d, seed=3)
     clean, _, _ = _attend(kind, q, k, v, lens, shared)
@@ -309,16 +313,16 @@ def test_masked_places_may_hold_anything(kind, b):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
-@pytest.mark.parametrize("b,shared", [(2, 0), (3, 200), (40, 200)])
-def test_scores_far_apart(kind, b, shared):
+@pytest.mark.parametrize("b,shared,n_kv", [(2, 0, 2), (3, 200, 2), (40, 200, 2), (200, 200, 8)])
+def test_scores_far_apart(kind, b, shared, n_kv):
     """Scores over hundreds, rising and falling with the position: the running maximum moves often."""
-    n_q, n_kv, d, s_max = 4, 2, 64, 400
+    n_q, d, s_max = 4 * n_kv, 64, 400
     for sign in (1.0, -1.0):
         k = torch.zeros(b, n_kv, s_max, d, dtype=BF, device=DEV)
         k[..., 0] = (sign * torch.arange(s_max, device=DEV) / 2).to(BF)
         v = _rand(b, n_kv, s_max, d, seed=5)
         q = torch.zeros(b, n_q, d, dtype=BF, device=DEV)
-        q[:, :, 0] = torch.tensor([1.0, -1.0, 0.5, 4.0], device=DEV)
+        q[:, :, 0] = torch.tensor([1.0, -1.0, 0.5, 4.0], device=DEV).repeat(n_kv)
         lens = [s_max - 7 * (i % 5) for i in range(b)]
         got, kk, vv = _attend(kind, q, k, v, lens, shared, scale=1.0)
         want, tol = _want(q, kk, vv, lens, shared, 1.0)
@@ -350,8 +354,9 @@ def test_all_scores_minus_infinity_weigh_nothing(kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
-def test_strided_queries_and_repeats_give_the_same_bits(kind):
-    b, n_q, n_kv, d, s = 40, 8, 4, 128, 333
+@pytest.mark.parametrize("b,n_q,n_kv", [(40, 8, 4), (150, 32, 8)])
+def test_strided_queries_and_repeats_give_the_same_bits(kind, b, n_q, n_kv):
+    d, s = 128, 333
     fused = _rand(b, 3 + n_q * d + 11, seed=1)
     q = fused[:, 3:3 + n_q * d].view(b, n_q, d)
     k, v = _rand(b, n_kv, s, d, seed=2), _rand(b, n_kv, s, d, seed=3)
@@ -364,10 +369,11 @@ def test_strided_queries_and_repeats_give_the_same_bits(kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
-def test_captured_call_follows_its_inputs(kind):
+@pytest.mark.parametrize("b,n_q,n_kv,d", [(24, 4, 2, 64), (150, 16, 8, 128)])
+def test_captured_call_follows_its_inputs(kind, b, n_q, n_kv, d):
     """A recorded call reads queries, lengths and cache as they are when it is replayed; two recordings do not
     share anything."""
-    b, n_q, n_kv, d, s, shared = 24, 4, 2, 64, 200, 64
+    s, shared = 200, 64
     k, v = _rand(b, n_kv, s, d, seed=2), _rand(b, n_kv, s, d, seed=3)
     cache = QuantizedCache(*_quantized(k), *_quantized(v))
     ck, cv = k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
