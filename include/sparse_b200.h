@@ -626,7 +626,9 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  * for code * 2^(scale - 127), scale byte 255 for NaN throughout; the writer takes the least
  * power of two, 2^-127 or more, by which the row's largest magnitude is at most 448 (codes
  * then stop at 240 where 256 would stand for 2^128), and byte 255 with zero codes for a row that holds an infinity or a NaN.  All codes and bf16
- * caches must be 16-byte aligned.
+ * caches must be 16-byte aligned.  A call's operands come as a struct (host memory, not kept);
+ * these calls are a decode step's, and a binding fills one block of bytes faster than it
+ * converts twenty arguments.
  *
  * sb_rope_append_fp8  rotates the first rope_dim elements of every q and k head (pairs
  *                  (i, i + rope_dim/2), angle pos * theta^(-2i/rope_dim)), stores q to
@@ -635,9 +637,8 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  *                  scaled row are fp32, a value is rounded once; angles are those of the
  *                  64-bit formula for positions up to 2^24.  A key head's first rope_dim
  *                  elements come from k_rot and the others from k_rest (NULL where there
- *                  are none).  strides: eight int64 (host), the elements between tokens
- *                  and between heads of q, k_rot, k_rest, v; a head stride of 0 shares one
- *                  row between the heads.  A token whose sequence is outside [0,B) or whose
+ *                  are none).  stride: elements between tokens and between heads of
+ *                  each; a head stride of 0 shares one row between the heads.  A token whose sequence is outside [0,B) or whose
  *                  position is outside [0,s_max) stores nothing but its q; two tokens of one
  *                  call must not name the same row.  dk, dv: multiples of 16 up to 256,
  *                  rope_dim a multiple of 16 up to dk.
@@ -655,27 +656,44 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  *                  that may overlap on the GPU.  status: device int32 (may be NULL), set
  *                  non-zero if a bounded wait gave up.  (dk,dv) = (128,128), (192,128),
  *                  (64,64).
- * sb_attn_decode_shared  the same over a bf16 cache, cache_k [B,s_max,n_kv,dk], cache_v
- *                  [B,s_max,n_kv,dv].
+ * sb_attn_decode_shared  the same over a bf16 cache, k [B,s_max,n_kv,dk] and v [B,s_max,n_kv,dv].
  */
-int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest, const void *v,
-                           const int32_t *seq_of_token, const int32_t *pos_of_token, int32_t T, int32_t B, int32_t n_q,
-                           int32_t n_kv, int32_t dk, int32_t dv, int32_t rope_dim, float theta, int32_t s_max,
-                           const int64_t *strides, void *q_out, void *codes_k, void *scale_k, void *codes_v,
-                           void *scale_v, void *stream);
-int32_t sb_cache_read_fp8(const void *codes_k, const void *scale_k, const void *codes_v, const void *scale_v, int32_t B,
-                          int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max, int32_t begin, int32_t count,
-                          int32_t shared_len, void *out_k, void *out_v, void *stream);
+typedef struct sb_rope_append {
+  const void *q, *k_rot, *k_rest, *v;
+  const int32_t *seq_of_token, *pos_of_token;
+  void *q_out, *codes_k, *scale_k, *codes_v, *scale_v;
+  int64_t stride[8];                  /* between tokens and between heads of q, k_rot, k_rest, v */
+  int32_t T, B, n_q, n_kv, dk, dv, rope_dim, s_max;
+  float theta;
+  int32_t reserved_;
+} sb_rope_append_args;
+
+typedef struct sb_cache_read {
+  const void *codes_k, *scale_k, *codes_v, *scale_v;
+  void *out_k, *out_v;
+  int32_t B, n_kv, dk, dv, s_max, begin, count, shared_len;
+} sb_cache_read_args;
+
+typedef struct sb_attn_cached {
+  const void *q, *k, *scale_k, *v, *scale_v;   /* codes and scales, or bf16 caches (scales unused) */
+  const int32_t *seq_lens;
+  void *ws, *out;
+  int32_t *status;
+  int64_t q_stride;
+  uint64_t ws_bytes;
+  int32_t B, n_q, n_kv, dk, dv, s_max, shared_len;
+  float scale;
+} sb_attn_cached_args;
+
+/* sizeof of the three (0, 1, 2) as this library was compiled; 0 for any other number. */
+size_t sb_cache_struct_bytes(int32_t which);
+
+int32_t sb_rope_append_fp8(const sb_rope_append_args *args, void *stream);
+int32_t sb_cache_read_fp8(const sb_cache_read_args *args, void *stream);
 size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max,
                                       int32_t shared_len);
-int32_t sb_attn_decode_fp8(const void *q, int64_t q_stride, const void *codes_k, const void *scale_k, const void *codes_v,
-                           const void *scale_v, const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk,
-                           int32_t dv, int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
-                           int32_t *status, void *stream);
-int32_t sb_attn_decode_shared(const void *q, int64_t q_stride, const void *cache_k, const void *cache_v,
-                              const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk, int32_t dv,
-                              int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
-                              int32_t *status, void *stream);
+int32_t sb_attn_decode_fp8(const sb_attn_cached_args *args, void *stream);
+int32_t sb_attn_decode_shared(const sb_attn_cached_args *args, void *stream);
 
 /* Number of kernels the last sb_moe_layer_forward of this thread launched. */
 int32_t sb_last_launch_count(void);

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Dict, Tuple
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -21,7 +22,7 @@ SB_COPY_PEER_TO_DEVICE = 1
 SB_COPY_DEVICE_LOCAL = 2
 SB_TILE_M = 128
 
-i32, i64, vp, sz = C.c_int32, C.c_int64, C.c_void_p, C.c_size_t
+i32, vp, sz = C.c_int32, C.c_void_p, C.c_size_t
 
 
 class MoeLayer(C.Structure):
@@ -36,6 +37,14 @@ class MoeLayer(C.Structure):
         ("ws", vp), ("ws_bytes", sz),
     ]
 
+
+# The structs of the cache calls as packed bytes (native alignment), fields in the header's order:
+# sb_rope_append_args    11 pointers, 8 strides, T B n_q n_kv dk dv rope_dim s_max, theta, reserved
+# sb_cache_read_args     6 pointers, B n_kv dk dv s_max begin count shared_len
+# sb_attn_cached_args    9 pointers, q_stride, ws_bytes, B n_q n_kv dk dv s_max shared_len, scale
+ROPE_APPEND = struct.Struct("@11P8q8ifi")
+CACHE_READ = struct.Struct("@6P8i")
+ATTN_CACHED = struct.Struct("@9PqQ7if")
 
 # name -> (restype, argtypes); this table is also what the symbol-export test walks.
 # rows up to which `sb_moe_layer_forward` takes the weight-streaming path (SB_DECODE_MAX_TOKENS)
@@ -100,13 +109,12 @@ SIGNATURES: Dict[str, Tuple[object, list]] = {
                                  vp]),
     "sb_attn_decode_workspace_bytes": (sz, [i32, i32, i32, i32]),
     "sb_attn_decode": (i32, [vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, C.c_float, i32, vp, sz, vp, vp]),
-    "sb_rope_append_fp8": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, i32,
-                                 C.POINTER(i64), vp, vp, vp, vp, vp, vp]),
-    "sb_cache_read_fp8": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
+    "sb_cache_struct_bytes": (sz, [i32]),
+    "sb_rope_append_fp8": (i32, [C.c_char_p, vp]),
+    "sb_cache_read_fp8": (i32, [C.c_char_p, vp]),
     "sb_attn_cached_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
-    "sb_attn_decode_fp8": (i32, [vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, sz, vp, vp,
-                                 vp]),
-    "sb_attn_decode_shared": (i32, [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, sz, vp, vp, vp]),
+    "sb_attn_decode_fp8": (i32, [C.c_char_p, vp]),
+    "sb_attn_decode_shared": (i32, [C.c_char_p, vp]),
     "sb_moe_layer_struct_bytes": (sz, []),
     "sb_moe_layer_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
     "sb_moe_layer_forward": (i32, [C.POINTER(MoeLayer), vp, vp]),
@@ -129,6 +137,8 @@ def _load() -> C.CDLL:
 lib = _load()
 if lib.sb_moe_layer_struct_bytes() != C.sizeof(MoeLayer):
     raise ImportError("sparse_b200: struct sb_moe_layer of the library and its ctypes mirror differ")
+if [lib.sb_cache_struct_bytes(i) for i in range(3)] != [s.size for s in (ROPE_APPEND, CACHE_READ, ATTN_CACHED)]:
+    raise ImportError("sparse_b200: the cache calls' structs of the library and their packed forms differ")
 
 
 def apply_tuning_from_env(var: str = "SPARSE_B200_TUNING") -> None:

@@ -749,9 +749,13 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
 }
 
 template <bool FP8>
-int32_t attend(const char *name, const void *q, int64_t q_stride, Cache cache, const int32_t *seq_lens, int B, int n_q,
-               int n_kv, int dk, int dv, int s_max, int shared_len, float scale, void *ws, size_t ws_bytes, void *out,
-               int32_t *status, void *stream) {
+int32_t attend(const char *name, const sb_attn_cached_args *args, void *stream) {
+  if (!args) return fail(SB_E_INVALID_ARG, "%s: null pointer", name);
+  const sb_attn_cached_args &a = *args;
+  const int B = a.B, n_q = a.n_q, n_kv = a.n_kv, dk = a.dk, dv = a.dv, s_max = a.s_max, shared_len = a.shared_len;
+  const float scale = a.scale;
+  int64_t q_stride = a.q_stride;
+  const Cache cache = {a.k, a.v, static_cast<const uint8_t *>(a.scale_k), static_cast<const uint8_t *>(a.scale_v)};
   // (the line's tiles are counted in 32 bits)
   if (B < 0 || n_q < 1 || n_kv < 1 || n_kv > 65535 || n_q % n_kv != 0 || s_max < 1 || shared_len < 0 || shared_len > s_max ||
       (int64_t)B * n_q > (1 << 22) || (int64_t)B * n_q * (s_max / kLeastTile + 2) > (1ll << 30))
@@ -762,21 +766,21 @@ int32_t attend(const char *name, const void *q, int64_t q_stride, Cache cache, c
   if (!((dk == 128 && dv == 128) || (dk == 192 && dv == 128) || (dk == 64 && dv == 64)))
     return fail(SB_E_UNSUPPORTED, "%s: head dims (%d,%d) not built (128/128, 192/128, 64/64)", name, dk, dv);
   if (B == 0) return SB_OK;
-  if (!q || !cache.k || !cache.v || (FP8 && (!cache.ks || !cache.vs)) || !seq_lens || !ws || !out)
+  if (!a.q || !cache.k || !cache.v || (FP8 && (!cache.ks || !cache.vs)) || !a.seq_lens || !a.ws || !a.out)
     return fail(SB_E_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(cache.k, 16) || !aligned(cache.v, 16) || !aligned(ws, 16) || !aligned(out, 4))
+  if (!aligned(cache.k, 16) || !aligned(cache.v, 16) || !aligned(a.ws, 16) || !aligned(a.out, 4))
     return fail(SB_E_INVALID_ARG, "%s: cache and workspace must be 16-byte aligned, out 4-byte", name);
-  if (ws_bytes < sb_attn_cached_workspace_bytes(B, n_q, n_kv, dk, dv, s_max, shared_len))
+  if (a.ws_bytes < sb_attn_cached_workspace_bytes(B, n_q, n_kv, dk, dv, s_max, shared_len))
     return fail(SB_E_WORKSPACE, "%s: workspace too small", name);
   Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, q_stride, scale * 1.4426950408889634f};
   plan(s, dk);
-  const __nv_bfloat16 *qq = static_cast<const __nv_bfloat16 *>(q);
-  float *part = static_cast<float *>(ws);
-  __nv_bfloat16 *oo = static_cast<__nv_bfloat16 *>(out);
+  const __nv_bfloat16 *qq = static_cast<const __nv_bfloat16 *>(a.q);
+  float *part = static_cast<float *>(a.ws);
+  __nv_bfloat16 *oo = static_cast<__nv_bfloat16 *>(a.out);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dk == 128 ? launch<128, 128, FP8>(qq, cache, seq_lens, s, part, oo, status, st)
-         : dk == 192 ? launch<192, 128, FP8>(qq, cache, seq_lens, s, part, oo, status, st)
-                     : launch<64, 64, FP8>(qq, cache, seq_lens, s, part, oo, status, st);
+  return dk == 128 ? launch<128, 128, FP8>(qq, cache, a.seq_lens, s, part, oo, a.status, st)
+         : dk == 192 ? launch<192, 128, FP8>(qq, cache, a.seq_lens, s, part, oo, a.status, st)
+                     : launch<64, 64, FP8>(qq, cache, a.seq_lens, s, part, oo, a.status, st);
 }
 
 }  // namespace
@@ -795,21 +799,12 @@ size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int3
   return (size_t)(slot_rows(s) + pre_slot_rows(s)) * (dv + 1) * sizeof(float);
 }
 
-int32_t sb_attn_decode_shared(const void *q, int64_t q_stride, const void *cache_k, const void *cache_v,
-                              const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk, int32_t dv,
-                              int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
-                              int32_t *status, void *stream) {
-  return attend<false>("sb_attn_decode_shared", q, q_stride, Cache{cache_k, cache_v, nullptr, nullptr}, seq_lens, B, n_q,
-                       n_kv, dk, dv, s_max, shared_len, scale, ws, ws_bytes, out, status, stream);
+int32_t sb_attn_decode_shared(const sb_attn_cached_args *args, void *stream) {
+  return attend<false>("sb_attn_decode_shared", args, stream);
 }
 
-int32_t sb_attn_decode_fp8(const void *q, int64_t q_stride, const void *codes_k, const void *scale_k, const void *codes_v,
-                           const void *scale_v, const int32_t *seq_lens, int32_t B, int32_t n_q, int32_t n_kv, int32_t dk,
-                           int32_t dv, int32_t s_max, int32_t shared_len, float scale, void *ws, size_t ws_bytes, void *out,
-                           int32_t *status, void *stream) {
-  return attend<true>("sb_attn_decode_fp8", q, q_stride,
-                      Cache{codes_k, codes_v, static_cast<const uint8_t *>(scale_k), static_cast<const uint8_t *>(scale_v)},
-                      seq_lens, B, n_q, n_kv, dk, dv, s_max, shared_len, scale, ws, ws_bytes, out, status, stream);
+int32_t sb_attn_decode_fp8(const sb_attn_cached_args *args, void *stream) {
+  return attend<true>("sb_attn_decode_fp8", args, stream);
 }
 
 }  // extern "C"

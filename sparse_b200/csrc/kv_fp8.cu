@@ -257,27 +257,27 @@ using namespace sb;
 
 extern "C" {
 
-int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest, const void *v,
-                           const int32_t *seq_of_token, const int32_t *pos_of_token, int32_t T, int32_t B, int32_t n_q,
-                           int32_t n_kv, int32_t dk, int32_t dv, int32_t rope_dim, float theta, int32_t s_max,
-                           const int64_t *strides, void *q_out, void *codes_k, void *scale_k, void *codes_v,
-                           void *scale_v, void *stream) {
+int32_t sb_rope_append_fp8(const sb_rope_append_args *args, void *stream) {
+  if (!args) return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: null pointer");
+  const sb_rope_append_args &a = *args;
+  const int T = a.T, B = a.B, n_q = a.n_q, n_kv = a.n_kv, dk = a.dk, dv = a.dv, rope_dim = a.rope_dim, s_max = a.s_max;
+  const float theta = a.theta;
   if (T < 0 || B < 1 || n_q < 1 || n_kv < 1 || n_q > 65536 || n_kv > 65536 || s_max < 1 || !head_ok(dk) || !head_ok(dv) ||
       rope_dim < 0 || rope_dim > dk || rope_dim % 16 != 0 || !(theta > 0.f) || !isfinite(theta))
     return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: bad shape (T=%d B=%d heads %d/%d widths %d/%d rope %d s_max=%d)", T,
                 B, n_q, n_kv, dk, dv, rope_dim, s_max);
   if (T == 0) return SB_OK;
-  if (!q || (rope_dim > 0 && !k_rot) || (rope_dim < dk && !k_rest) || !v || !seq_of_token || !pos_of_token || !strides ||
-      !q_out || !codes_k || !scale_k || !codes_v || !scale_v)
+  if (!a.q || (rope_dim > 0 && !a.k_rot) || (rope_dim < dk && !a.k_rest) || !a.v || !a.seq_of_token || !a.pos_of_token ||
+      !a.q_out || !a.codes_k || !a.scale_k || !a.codes_v || !a.scale_v)
     return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: null pointer");
-  if (!aligned(q_out, 16) || !aligned(codes_k, 16) || !aligned(codes_v, 16))
+  if (!aligned(a.q_out, 16) || !aligned(a.codes_k, 16) || !aligned(a.codes_v, 16))
     return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: q_out and the codes must be 16-byte aligned");
-  const void *base[4] = {q, k_rot, k_rest, v};
+  const void *base[4] = {a.q, a.k_rot, a.k_rest, a.v};
   RowSource src[4];
   bool vec = true;
   for (int i = 0; i < 4; ++i) {
-    src[i] = RowSource{static_cast<const __nv_bfloat16 *>(base[i]), strides[2 * i], strides[2 * i + 1]};
-    vec = vec && aligned(base[i], 16) && strides[2 * i] % 8 == 0 && strides[2 * i + 1] % 8 == 0;
+    src[i] = RowSource{static_cast<const __nv_bfloat16 *>(base[i]), a.stride[2 * i], a.stride[2 * i + 1]};
+    vec = vec && aligned(base[i], 16) && a.stride[2 * i] % 8 == 0 && a.stride[2 * i + 1] % 8 == 0;
   }
   const RopeFreq &freq = rope_freq(theta, rope_dim);
   const int widest = dk > dv ? dk : dv;
@@ -290,21 +290,22 @@ int32_t sb_rope_append_fp8(const void *q, const void *k_rot, const void *k_rest,
   const dim3 grid(T, wanted < room ? wanted : room);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto launch = lanes == 4 ? launch_append<4> : lanes == 8 ? launch_append<8> : launch_append<16>;
-  return launch(vec, grid, st, src[0], src[1], src[2], src[3], q_out, seq_of_token, pos_of_token, B, n_q, n_kv, dk, dv,
-                rope_dim, s_max, codes_k, scale_k, codes_v, scale_v, freq);
+  return launch(vec, grid, st, src[0], src[1], src[2], src[3], a.q_out, a.seq_of_token, a.pos_of_token, B, n_q, n_kv, dk, dv,
+                rope_dim, s_max, a.codes_k, a.scale_k, a.codes_v, a.scale_v, freq);
 }
 
-int32_t sb_cache_read_fp8(const void *codes_k, const void *scale_k, const void *codes_v, const void *scale_v, int32_t B,
-                          int32_t n_kv, int32_t dk, int32_t dv, int32_t s_max, int32_t begin, int32_t count,
-                          int32_t shared_len, void *out_k, void *out_v, void *stream) {
+int32_t sb_cache_read_fp8(const sb_cache_read_args *args, void *stream) {
+  if (!args) return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: null pointer");
+  const sb_cache_read_args &a = *args;
+  const int B = a.B, n_kv = a.n_kv, dk = a.dk, dv = a.dv, s_max = a.s_max, begin = a.begin, count = a.count, shared_len = a.shared_len;
   if (B < 0 || B > 65535 || n_kv < 1 || n_kv > 65535 || !head_ok(dk) || !head_ok(dv) || s_max < 1 || begin < 0 ||
       count < 0 || count > s_max - begin || shared_len < 0 || shared_len > s_max)
     return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: bad shape (B=%d n_kv=%d widths %d/%d positions %d+%d of %d, shared %d)",
                 B, n_kv, dk, dv, begin, count, s_max, shared_len);
   if (B == 0 || count == 0) return SB_OK;
-  if (!codes_k || !scale_k || !codes_v || !scale_v || !out_k || !out_v)
+  if (!a.codes_k || !a.scale_k || !a.codes_v || !a.scale_v || !a.out_k || !a.out_v)
     return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: null pointer");
-  if (!aligned(codes_k, 16) || !aligned(codes_v, 16) || !aligned(out_k, 16) || !aligned(out_v, 16))
+  if (!aligned(a.codes_k, 16) || !aligned(a.codes_v, 16) || !aligned(a.out_k, 16) || !aligned(a.out_v, 16))
     return fail(SB_E_INVALID_ARG, "sb_cache_read_fp8: codes and outputs must be 16-byte aligned");
   const int step = kReadThreads / ((dk + dv) >> 3) * kReadAhead;
   const int wanted = (count + step - 1) / step;
@@ -313,12 +314,16 @@ int32_t sb_cache_read_fp8(const void *codes_k, const void *scale_k, const void *
   const long long room = (32ll * sms + heads - 1) / heads;
   const dim3 grid((unsigned)(wanted < room ? wanted : room), n_kv, B);
   SB_CUDA_CHECK(launch_pdl(cache_read_fp8_kernel, grid, dim3(kReadThreads), 0, static_cast<cudaStream_t>(stream),
-                           static_cast<const uint8_t *>(codes_k), static_cast<const uint8_t *>(scale_k),
-                           static_cast<const uint8_t *>(codes_v), static_cast<const uint8_t *>(scale_v), n_kv, dk, dv,
-                           s_max, begin, count, shared_len, static_cast<__nv_bfloat16 *>(out_k),
-                           static_cast<__nv_bfloat16 *>(out_v)));
+                           static_cast<const uint8_t *>(a.codes_k), static_cast<const uint8_t *>(a.scale_k),
+                           static_cast<const uint8_t *>(a.codes_v), static_cast<const uint8_t *>(a.scale_v), n_kv, dk, dv,
+                           s_max, begin, count, shared_len, static_cast<__nv_bfloat16 *>(a.out_k),
+                           static_cast<__nv_bfloat16 *>(a.out_v)));
   SB_LAUNCH_CHECK();
   return SB_OK;
+}
+
+size_t sb_cache_struct_bytes(int32_t which) {
+  return which == 0 ? sizeof(sb_rope_append_args) : which == 1 ? sizeof(sb_cache_read_args) : which == 2 ? sizeof(sb_attn_cached_args) : 0;
 }
 
 }  // extern "C"

@@ -6,7 +6,6 @@ of the tensors' device and never synchronise.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 from typing import Optional, Tuple
 
@@ -204,16 +203,13 @@ def combine(rows_out: torch.Tensor, slot_of_item: torch.Tensor, idx: torch.Tenso
 # The calls of a decode step, of which a layer makes several and whose kernels take a few
 # microseconds: checks without tensor temporaries, the stream's handle without a Stream object, a
 # device guard only where another device is current.
-_Strides = ctypes.c_int64 * 8
-
-
-def _call(fn, what: str, device: int, *args) -> None:
-    """fn(*args, stream) with `device` current, its current stream; raises on a status."""
+def _call(fn, what: str, device: int, args: bytes) -> None:
+    """fn(args, stream) with `device` current, its current stream; raises on a status."""
     if torch._C._cuda_getDevice() == device:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        status = fn(args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+            status = fn(args, torch._C._cuda_getCurrentRawStream(device))
     if status != 0:
         check(status, what)
 
@@ -257,7 +253,7 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
     ptrs, strides = [], []
     for view, heads, width in ((q, n_q, dk), (k_rot, n_kv, rope), (k_rest, n_kv, dk - rope), (v, n_kv, dv)):
         if view is None:
-            ptrs.append(None)
+            ptrs.append(0)
             strides += (0, 0)
             continue
         shape = view.shape
@@ -272,10 +268,10 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
         strides += (token, head if shape[1] > 1 else 0)
     seq = _index(seq_of_token, t, device, "rope_append_quantized: seq_of_token")
     pos = _index(pos_of_token, t, device, "rope_append_quantized: pos_of_token")
-    out = q.new_empty((t, n_q, dk))
-    _call(lib.sb_rope_append_fp8, "sb_rope_append_fp8", device, *ptrs, seq, pos, t, b, n_q, n_kv, dk, dv, rope, theta, s_max,
-          _Strides(*strides), out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
-          cache.v_scale.data_ptr())
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _call(lib.sb_rope_append_fp8, "sb_rope_append_fp8", device, _lib.ROPE_APPEND.pack(
+        *ptrs, seq, pos, out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
+        cache.v_scale.data_ptr(), *strides, t, b, n_q, n_kv, dk, dv, rope, s_max, theta, 0))
     return out
 
 
@@ -291,8 +287,9 @@ def cache_read(cache: QuantizedCache, begin: int, count: int, shared_len: int = 
             begin, begin + count, shared_len, s_max))
     k = cache.k.new_empty((b, n_kv, count, dk), dtype=torch.bfloat16)
     v = cache.k.new_empty((b, n_kv, count, dv), dtype=torch.bfloat16)
-    _call(lib.sb_cache_read_fp8, "sb_cache_read_fp8", device, cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
-          cache.v_scale.data_ptr(), b, n_kv, dk, dv, s_max, begin, count, shared_len, k.data_ptr(), v.data_ptr())
+    _call(lib.sb_cache_read_fp8, "sb_cache_read_fp8", device, _lib.CACHE_READ.pack(
+        cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), k.data_ptr(),
+        v.data_ptr(), b, n_kv, dk, dv, s_max, begin, count, shared_len))
     return k, v
 
 
@@ -314,12 +311,12 @@ def _decode_attention(name: str, call, q: torch.Tensor, cache_ptrs, seq_lens: to
     if status is not None and (status.dtype != torch.int32 or status.get_device() != device or status.numel() < 1):
         raise RuntimeError("%s: status must be int32 on the cache's device" % name)
     lens = _index(seq_lens, b, device, name)
-    out = q.new_empty((b, n_q, dv))
+    out = torch.empty_like(q) if dv == dk and q.is_contiguous() else q.new_empty((b, n_q, dv))
     ws_bytes = _attn_workspace(b, n_q, n_kv, dk, dv, s_max, shared_len) or 16
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
-    _call(call, name, device, q.data_ptr(), seq_stride if b > 1 else 0, *cache_ptrs, lens, b, n_q, n_kv, dk, dv, s_max,
-          shared_len, dk ** -0.5 if scale is None else scale, ws.data_ptr(), ws_bytes, out.data_ptr(),
-          None if status is None else status.data_ptr())
+    _call(call, name, device, _lib.ATTN_CACHED.pack(
+        q.data_ptr(), *cache_ptrs, lens, ws.data_ptr(), out.data_ptr(), 0 if status is None else status.data_ptr(),
+        seq_stride if b > 1 else 0, ws_bytes, b, n_q, n_kv, dk, dv, s_max, shared_len, dk ** -0.5 if scale is None else scale))
     return out
 
 
@@ -350,7 +347,7 @@ def attn_decode_shared(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Te
     if cache_k.dtype != torch.bfloat16 or cache_v.dtype != torch.bfloat16 or cache_v.get_device() != device:
         raise RuntimeError("attn_decode_shared needs bf16 caches on one device")
     b, s_max, n_kv, dk = cache_k.shape
-    return _decode_attention("attn_decode_shared", lib.sb_attn_decode_shared, q, (_ptr(cache_k), _ptr(cache_v)), seq_lens, b,
+    return _decode_attention("attn_decode_shared", lib.sb_attn_decode_shared, q, (_ptr(cache_k), 0, _ptr(cache_v), 0), seq_lens, b,
                              n_kv, dk, cache_v.shape[3], s_max, shared_len, scale, status, device)
 
 
