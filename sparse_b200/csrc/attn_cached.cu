@@ -648,8 +648,8 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
     const int r = b * s.group + hg, rt = r / s.pre_tile_rows;
     from[0] = pre_part;
     from_lse[0] = pre_lse;
-    step[0] = prefix_rows(s);
-    first_row[0] = ((size_t)hk * prefix_row_tiles(s) + rt) * s.pre_splits * step[0] + r - rt * s.pre_tile_rows;
+    step[0] = s.pre_rows;
+    first_row[0] = ((size_t)hk * s.pre_tiles + rt) * s.pre_splits * step[0] + r - rt * s.pre_tile_rows;
     n[0] = s.pre_splits;
   } else if (pre_line > 0 && prefix) {
     const int r = b * s.group + hg, rt = r / s.rows, tiles = pre_tiles<FP8>(s), seg = hk * s.pre_row_tiles + rt;
@@ -712,7 +712,7 @@ constexpr int kMaxRows = 16;
 void plan(Shape &s, int dk) {
   const int64_t pre_rows = s.shared_len > 0 ? (int64_t)s.B * s.group : 0;
   s.pre_splits = 0;
-  s.pre_tile_rows = 1;
+  s.pre_tile_rows = s.pre_tiles = s.pre_rows = 0;
   if (pre_rows > kMaxRows) plan_prefix(s, dk);
   s.rows = s.group > kMaxRows ? kMaxRows : s.group;
   if (pre_rows > s.rows && s.pre_splits == 0) s.rows = (int)pre_rows;
@@ -722,7 +722,7 @@ void plan(Shape &s, int dk) {
 // Partial results: of the streamed line, then of the shared positions' tiles; outputs first,
 // then logarithms.
 int64_t slot_rows(const Shape &s) { return (kMaxCtas + (int64_t)s.n_kv * (s.pre_row_tiles + (int64_t)s.B * s.row_tiles)) * s.rows; }
-int64_t pre_slot_rows(const Shape &s) { return s.pre_splits > 0 ? prefix_slots(s) * prefix_rows(s) : 0; }
+int64_t pre_slot_rows(const Shape &s) { return s.pre_splits > 0 ? prefix_slots(s) * s.pre_rows : 0; }
 
 template <int DK, int DV, bool FP8>
 int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_lens, const Shape &s, float *part,
@@ -772,7 +772,7 @@ int32_t attend(const char *name, const sb_attn_cached_args *args, void *stream) 
     return fail(SB_E_INVALID_ARG, "%s: cache and workspace must be 16-byte aligned, out 4-byte", name);
   if (a.ws_bytes < sb_attn_cached_workspace_bytes(B, n_q, n_kv, dk, dv, s_max, shared_len))
     return fail(SB_E_WORKSPACE, "%s: workspace too small", name);
-  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, q_stride, scale * 1.4426950408889634f};
+  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, 0, 0, q_stride, scale * 1.4426950408889634f};
   plan(s, dk);
   const __nv_bfloat16 *qq = static_cast<const __nv_bfloat16 *>(a.q);
   float *part = static_cast<float *>(a.ws);
@@ -794,7 +794,7 @@ size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int3
                                       int32_t shared_len) {
   if (B < 0 || dk < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || dv < 1 || s_max < 1 || shared_len < 0 || (int64_t)B * n_q > (1 << 22))
     return 0;
-  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, 0, 0.f};
+  Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, 0, 0, 0, 0.f};
   plan(s, dk);
   return (size_t)(slot_rows(s) + pre_slot_rows(s)) * (dv + 1) * sizeof(float);
 }

@@ -15,7 +15,8 @@ struct Shape {
   int s_max, shared_len;
   int rows;                           // query rows of a segment of the streamed line (at most 16)
   int row_tiles, pre_row_tiles;       // its segments per key head: of a sequence, and of the shared positions
-  int pre_splits, pre_tile_rows;      // pre_splits > 0: the shared positions go through attn_prefix_kernel, cut in so many
+  int pre_splits;                     // > 0: the shared positions go through attn_prefix_kernel, cut in so many
+  int pre_tile_rows, pre_tiles, pre_rows;    // its rows per tile, row tiles of a key head, rows of a partial result
   int64_t q_stride;
   float scale_log2;                   // scale * log2(e), >= 0
 };
@@ -23,14 +24,10 @@ struct Shape {
 // attn_prefix_kernel takes the rows of a key head, numbered sequence by sequence (row = b * group
 // + h), in tiles of 128, or of two times 128.
 constexpr int kPrefixRows = 128;
-__host__ __device__ inline int prefix_row_tiles(const Shape &s) {
-  return (int)(((int64_t)s.B * s.group + s.pre_tile_rows - 1) / s.pre_tile_rows);
-}
-// Partial results of that kernel: one per CTA, of `prefix_rows` rows.
-__host__ __device__ inline int prefix_rows(const Shape &s) { return min(s.B * s.group, s.pre_tile_rows); }
-inline int64_t prefix_slots(const Shape &s) { return (int64_t)s.n_kv * prefix_row_tiles(s) * s.pre_splits; }
+// Partial results of that kernel: one per CTA, of `pre_rows` rows.
+inline int64_t prefix_slots(const Shape &s) { return (int64_t)s.n_kv * s.pre_tiles * s.pre_splits; }
 
-// Sets pre_tile_rows and pre_splits of a call whose shared positions go through attn_prefix_kernel.
+// Sets the pre_* fields of a call whose shared positions go through attn_prefix_kernel.
 void plan_prefix(Shape &s, int dk);
 
 // softmax(q k) v of every row of the batch over the shared positions, as partial results:

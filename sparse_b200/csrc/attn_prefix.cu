@@ -215,7 +215,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int hk = blockIdx.z, rt = blockIdx.y;
   const int all_tiles = (s.shared_len + kKeys - 1) / kKeys;
-  const int tile0 = (int)((int64_t)blockIdx.x * all_tiles / gridDim.x), tile1 = (int)((int64_t)(blockIdx.x + 1) * all_tiles / gridDim.x);
+  const int least = all_tiles / (int)gridDim.x, longer = all_tiles - least * (int)gridDim.x;      // (the first runs are one tile longer)
+  const int tile0 = (int)blockIdx.x * least + min((int)blockIdx.x, longer), tile1 = tile0 + least + ((int)blockIdx.x < longer ? 1 : 0);
   const int n = tile1 - tile0;                          // tiles of this run, at least one
   const int blocks = TWO ? 2 * n : n;                   // of each group
   const int rows = min(kRows, s.B * s.group - rt * kRows);
@@ -437,7 +438,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
     groups_sync();
     if (ok) {
-      const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * prefix_rows(s);
+      const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * s.pre_rows;
       const int r0 = TWO ? w * kPrefixRows : 0, here = min(kPrefixRows, rows - r0), threads = TWO ? 128 : 256;
 #pragma unroll 4
       for (int i = threadIdx.x - kSoftmaxWarp * 32 - r0; i < here * (DV / 4); i += threads) {
@@ -556,7 +557,7 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float
     SB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem));
     opted_in.fetch_or(bit, std::memory_order_relaxed);
   }
-  const dim3 grid(s.pre_splits, prefix_row_tiles(s), s.n_kv);
+  const dim3 grid(s.pre_splits, s.pre_tiles, s.n_kv);
   SB_CUDA_CHECK(launch_pdl(kern, grid, dim3(L::kThreads), L::kSmem, stream, tm_k, tm_v, q, cache, s, part, lse, status));
   SB_LAUNCH_CHECK();
   return SB_OK;
@@ -565,8 +566,11 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const Shape &s, float
 }  // namespace
 
 void plan_prefix(Shape &s, int dk) {
-  s.pre_tile_rows = (int64_t)s.B * s.group > kPrefixRows && dk <= 128 ? 2 * kPrefixRows : kPrefixRows;
-  const int64_t tiles = (s.shared_len + kKeys - 1) / kKeys, heads = (int64_t)s.n_kv * prefix_row_tiles(s);
+  const int rows = s.B * s.group;                       // (at most 2^22)
+  s.pre_tile_rows = rows > kPrefixRows && dk <= 128 ? 2 * kPrefixRows : kPrefixRows;
+  s.pre_tiles = (rows + s.pre_tile_rows - 1) / s.pre_tile_rows;
+  s.pre_rows = rows < s.pre_tile_rows ? rows : s.pre_tile_rows;
+  const int64_t tiles = (s.shared_len + kKeys - 1) / kKeys, heads = (int64_t)s.n_kv * s.pre_tiles;
   const int64_t fit = 148 / heads;
   s.pre_splits = (int)(fit < 1 ? 1 : fit < tiles ? fit : tiles);
 }
