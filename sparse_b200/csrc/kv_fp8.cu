@@ -75,25 +75,32 @@ __device__ __forceinline__ uint2 codes8(float (&x)[8], uint32_t byte, float inv)
   return make_uint2(e4m3x4(x[0], x[1], x[2], x[3]), e4m3x4(x[4], x[5], x[6], x[7]));
 }
 
-// Codes and scale byte of the row that L lanes hold; `scale` null: no row.
+// max(a, |b|), NaN where one is
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+
+// Codes and scale byte of the row that L lanes hold (`mask`: those lanes), `in`: the lane has values of it.
 template <int L>
-__device__ __forceinline__ void store_codes(float (&x)[8], float (&y)[8], RowPlace at, bool in, int lane, uint8_t *codes,
-                                            uint8_t *scale) {
-  uint32_t top = 0;
+__device__ __forceinline__ void store_codes(float (&x)[8], float (&y)[8], RowPlace at, bool in, int lane, uint32_t mask,
+                                            uint8_t *codes, uint8_t *scale) {
+  float top = 0.f;
+  if (in) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    top = max(top, max(__float_as_uint(x[i]) & 0x7fffffffu, __float_as_uint(y[i]) & 0x7fffffffu));
+    for (int i = 0; i < 8; ++i) top = max_abs(max_abs(top, x[i]), y[i]);
+  }
 #pragma unroll
-  for (int off = L / 2; off >= 1; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-  const uint32_t byte = e8m0_of_amax(top);
+  for (int off = L / 2; off >= 1; off >>= 1) top = max_abs(top, __shfl_xor_sync(mask, top, off));
+  if (!in) return;
+  const uint32_t byte = e8m0_of_amax(__float_as_uint(top) & 0x7fffffffu);
   const float inv = e8m0_inverse(byte);
   uint2 c0 = codes8(x, byte, inv), c1 = codes8(y, byte, inv);
   if (byte == kScaleNan) c0 = c1 = make_uint2(0, 0);
-  if (scale != nullptr && in) {
-    *reinterpret_cast<uint2 *>(codes + at.e0) = c0;
-    *reinterpret_cast<uint2 *>(codes + at.e1) = c1;
-    if (lane == 0) *scale = (uint8_t)byte;
-  }
+  *reinterpret_cast<uint2 *>(codes + at.e0) = c0;
+  *reinterpret_cast<uint2 *>(codes + at.e1) = c1;
+  if (lane == 0) *scale = (uint8_t)byte;
 }
 
 __device__ __forceinline__ void store_bf16(__nv_bfloat16 *p, const float (&x)[8]) {
@@ -129,43 +136,43 @@ rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource
   const bool cached = pos >= 0 && pos < s_max && seq >= 0 && seq < B;
   const int rows = n_q + (cached ? 2 * n_kv : 0);
   const int lane = threadIdx.x % L;
+  const uint32_t mask = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
   const RowPlace key_at = row_place(lane, half), value_at = row_place(lane, 0);
   const bool in_key = lane * 16 < dk, in_value = lane * 16 < dv;
+  const size_t row0 = (size_t)(cached ? seq : 0) * n_kv * s_max + (cached ? pos : 0);      // of head 0 in the cache
   constexpr int kRows = kAppendThreads / L;              // rows of a CTA in one turn
-  // (all lanes of a warp take the same turns: the scale's reduction shuffles across a row)
-  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
-    const int r = r0 + threadIdx.x / L;
-    float x[8], y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
-    uint8_t *codes = nullptr, *scale = nullptr;
-    const bool value = r >= n_q + n_kv;
-    if (r < n_q + n_kv) {
+  float x[8], y[8];
+  for (int r = blockIdx.y * kRows + threadIdx.x / L; r < rows; r += gridDim.y * kRows) {
+    if (r < n_q) {
+      if (!in_key) continue;
+      const __nv_bfloat16 *src = q.at(t, r);
+      load8<VEC>(src + key_at.e0, x);
+      load8<VEC>(src + key_at.e1, y);
+      if (key_at.turned) turn(x, y, table, pairs, lane);
+      __nv_bfloat16 *dst = q_out + ((size_t)t * n_q + r) * dk;
+      store_bf16(dst + key_at.e0, x);
+      store_bf16(dst + key_at.e1, y);
+    } else if (r < n_q + n_kv) {
+      const int h = r - n_q;
+      const size_t row = row0 + (size_t)h * s_max;
       if (in_key) {
-        const bool query = r < n_q;
         // (an unrotated vector of a key stands in k_rest, rope elements further on than there)
-        const __nv_bfloat16 *src = query ? q.at(t, r) : key_at.turned ? k_rot.at(t, r - n_q) : k_rest.at(t, r - n_q) - rope;
+        const __nv_bfloat16 *src = key_at.turned ? k_rot.at(t, h) : k_rest.at(t, h) - rope;
         load8<VEC>(src + key_at.e0, x);
         load8<VEC>(src + key_at.e1, y);
         if (key_at.turned) turn(x, y, table, pairs, lane);
-        if (query) {
-          __nv_bfloat16 *dst = q_out + ((size_t)t * n_q + r) * dk;
-          store_bf16(dst + key_at.e0, x);
-          store_bf16(dst + key_at.e1, y);
-        }
       }
-    } else if (r < rows && in_value) {
-      const __nv_bfloat16 *src = v.at(t, r - n_q - n_kv);
-      load8<VEC>(src + value_at.e0, x);
-      load8<VEC>(src + value_at.e1, y);
+      store_codes<L>(x, y, key_at, in_key, lane, mask, codes_k + row * dk, scale_k + row);
+    } else {
+      const int h = r - n_q - n_kv;
+      const size_t row = row0 + (size_t)h * s_max;
+      if (in_value) {
+        const __nv_bfloat16 *src = v.at(t, h);
+        load8<VEC>(src + value_at.e0, x);
+        load8<VEC>(src + value_at.e1, y);
+      }
+      store_codes<L>(x, y, value_at, in_value, lane, mask, codes_v + row * dv, scale_v + row);
     }
-    if (r0 + kRows <= n_q) continue;                     // (queries only; the same for the whole CTA)
-    if (r >= n_q && r < rows) {
-      const size_t row = ((size_t)seq * n_kv + (value ? r - n_q - n_kv : r - n_q)) * s_max + pos;
-      codes = value ? codes_v + row * dv : codes_k + row * dk;
-      scale = value ? scale_v + row : scale_k + row;
-    }
-    store_codes<L>(x, y, value ? value_at : key_at, value ? in_value : in_key, lane, codes, scale);
   }
 }
 
@@ -201,17 +208,18 @@ cache_read_fp8_kernel(const uint8_t *__restrict__ codes_k, const uint8_t *__rest
   const bool key = lane < (dk >> 3);
   const int d = key ? dk : dv, e = (key ? lane : lane - (dk >> 3)) * 8;
   const uint8_t *codes = key ? codes_k : codes_v, *scales = key ? scale_k : scale_v;
+  // rows of this head in sequence 0's cache and in the sequence's own, from position `begin` on
+  const size_t row_shared = (size_t)h * s_max + begin, row_own = row_shared + (size_t)b * n_kv * s_max;
+  const int shared = shared_len - begin;
   __nv_bfloat16 *dst = (key ? out_k : out_v) + ((size_t)b * n_kv + h) * count * d + e;
   for (int i0 = blockIdx.x * step * kReadAhead + first; i0 < count; i0 += gridDim.x * step * kReadAhead) {
     uint2 c[kReadAhead];
     uint32_t byte[kReadAhead];
 #pragma unroll
     for (int a = 0; a < kReadAhead; ++a) {
-      const int i = i0 + a * step, pos = begin + i;
-      c[a] = make_uint2(0, 0);
-      byte[a] = 0;
+      const int i = i0 + a * step;
       if (i < count) {
-        const size_t row = ((size_t)(pos < shared_len ? 0 : b) * n_kv + h) * s_max + pos;
+        const size_t row = (i < shared ? row_shared : row_own) + i;
         c[a] = __ldg(reinterpret_cast<const uint2 *>(codes + row * d + e));
         byte[a] = __ldg(scales + row);
       }
@@ -219,13 +227,13 @@ cache_read_fp8_kernel(const uint8_t *__restrict__ codes_k, const uint8_t *__rest
 #pragma unroll
     for (int a = 0; a < kReadAhead; ++a) {
       const int i = i0 + a * step;
+      if (i >= count) break;
       const float scale = e8m0_value(byte[a]);
       const float2 v0 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].x)), v1 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].x >> 16));
       const float2 v2 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].y)), v3 = f16x2_to_float2(e4m3x2_to_f16x2(c[a].y >> 16));
-      if (i < count)
-        __stcs(reinterpret_cast<uint4 *>(dst + (size_t)i * d),
-            make_uint4(pack_bf16x2(v0.x * scale, v0.y * scale), pack_bf16x2(v1.x * scale, v1.y * scale),
-                       pack_bf16x2(v2.x * scale, v2.y * scale), pack_bf16x2(v3.x * scale, v3.y * scale)));
+      __stcs(reinterpret_cast<uint4 *>(dst + (size_t)i * d),
+             make_uint4(pack_bf16x2(v0.x * scale, v0.y * scale), pack_bf16x2(v1.x * scale, v1.y * scale),
+                        pack_bf16x2(v2.x * scale, v2.y * scale), pack_bf16x2(v3.x * scale, v3.y * scale)));
     }
   }
 }
