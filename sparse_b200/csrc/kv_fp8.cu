@@ -31,16 +31,16 @@ struct RowSource {
 };
 
 template <bool VEC>
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8]) {
-  if constexpr (VEC) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16 *p) {
+  if constexpr (VEC) return __ldg(reinterpret_cast<const uint4 *>(p));
+  const unsigned short *e = reinterpret_cast<const unsigned short *>(p);
+  return make_uint4(e[0] | ((uint32_t)e[1] << 16), e[2] | ((uint32_t)e[3] << 16), e[4] | ((uint32_t)e[5] << 16),
+                    e[6] | ((uint32_t)e[7] << 16));
+}
+__device__ __forceinline__ void unpack8(const uint4 &v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = bf16_lo(w[i]); x[2 * i + 1] = bf16_hi(w[i]); }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __bfloat162float(p[i]);
-  }
+  for (int i = 0; i < 4; ++i) { x[2 * i] = bf16_lo(w[i]); x[2 * i + 1] = bf16_hi(w[i]); }
 }
 
 // A row is held by L lanes, two vectors of eight values each: a lane of the rotated part has
@@ -122,57 +122,62 @@ rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource
   pdl_launch_dependents();
   pdl_wait();
   const int t = blockIdx.x;
-  const int pos = pos_of_token[t], seq = seq_of_token[t];
   const int half = rope >> 1, pairs = half >> 3;
+  const int lane = threadIdx.x % L;
+  const RowPlace key_at = row_place(lane, half), value_at = row_place(lane, 0);
+  const bool in_key = lane * 16 < dk, in_value = lane * 16 < dv;
+  constexpr int kRows = kAppendThreads / L;              // rows of a CTA in one turn
+  // a lane's two vectors of row r: queries, then keys, then values
+  const auto fetch = [&](int r, uint4 &a, uint4 &b) {
+    const bool value = r >= n_q + n_kv;
+    if (r >= n_q + 2 * n_kv || !(value ? in_value : in_key)) return;
+    // (an unrotated vector of a key stands in k_rest, rope elements further on than there)
+    const __nv_bfloat16 *src = r < n_q ? q.at(t, r) : value ? v.at(t, r - n_q - n_kv)
+                               : key_at.turned ? k_rot.at(t, r - n_q) : k_rest.at(t, r - n_q) - rope;
+    a = load8<VEC>(src + (value ? value_at.e0 : key_at.e0));
+    b = load8<VEC>(src + (value ? value_at.e1 : key_at.e1));
+  };
+  // the first turn's rows are on their way while the position is read and its angles are worked out,
+  // a later turn's during the one before it
+  int r = blockIdx.y * kRows + threadIdx.x / L;
+  uint4 a = make_uint4(0, 0, 0, 0), b = a;
+  fetch(r, a, b);
+  const int pos = pos_of_token[t], seq = seq_of_token[t];
   if (threadIdx.x < half) {
     const float p = (float)pos, hi = freq.turns[threadIdx.x].x, lo = freq.turns[threadIdx.x].y;
-    const float a = p * hi;
-    const float turn = (a - rintf(a)) + (fmaf(p, hi, -a) + p * lo);
+    const float f = p * hi;
+    const float turns = (f - rintf(f)) + (fmaf(p, hi, -f) + p * lo);
     float sn, cs;
-    sincospif(2.f * turn, &sn, &cs);
+    sincospif(2.f * turns, &sn, &cs);
     table[(threadIdx.x & 7) * pairs + (threadIdx.x >> 3)] = make_float2(cs, sn);
   }
   __syncthreads();
   const bool cached = pos >= 0 && pos < s_max && seq >= 0 && seq < B;
   const int rows = n_q + (cached ? 2 * n_kv : 0);
-  const int lane = threadIdx.x % L;
-  const uint32_t mask = (L == 32 ? 0xffffffffu : (1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
-  const RowPlace key_at = row_place(lane, half), value_at = row_place(lane, 0);
-  const bool in_key = lane * 16 < dk, in_value = lane * 16 < dv;
+  const uint32_t mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
   const size_t row0 = (size_t)(cached ? seq : 0) * n_kv * s_max + (cached ? pos : 0);      // of head 0 in the cache
-  constexpr int kRows = kAppendThreads / L;              // rows of a CTA in one turn
-  float x[8], y[8];
-  for (int r = blockIdx.y * kRows + threadIdx.x / L; r < rows; r += gridDim.y * kRows) {
+  while (r < rows) {
+    const int next = r + gridDim.y * kRows;
+    float x[8], y[8];
+    unpack8(a, x);
+    unpack8(b, y);
+    fetch(next, a, b);
     if (r < n_q) {
-      if (!in_key) continue;
-      const __nv_bfloat16 *src = q.at(t, r);
-      load8<VEC>(src + key_at.e0, x);
-      load8<VEC>(src + key_at.e1, y);
-      if (key_at.turned) turn(x, y, table, pairs, lane);
-      __nv_bfloat16 *dst = q_out + ((size_t)t * n_q + r) * dk;
-      store_bf16(dst + key_at.e0, x);
-      store_bf16(dst + key_at.e1, y);
-    } else if (r < n_q + n_kv) {
-      const int h = r - n_q;
-      const size_t row = row0 + (size_t)h * s_max;
       if (in_key) {
-        // (an unrotated vector of a key stands in k_rest, rope elements further on than there)
-        const __nv_bfloat16 *src = key_at.turned ? k_rot.at(t, h) : k_rest.at(t, h) - rope;
-        load8<VEC>(src + key_at.e0, x);
-        load8<VEC>(src + key_at.e1, y);
         if (key_at.turned) turn(x, y, table, pairs, lane);
+        __nv_bfloat16 *dst = q_out + ((size_t)t * n_q + r) * dk;
+        store_bf16(dst + key_at.e0, x);
+        store_bf16(dst + key_at.e1, y);
       }
+    } else if (r < n_q + n_kv) {
+      const size_t row = row0 + (size_t)(r - n_q) * s_max;
+      if (in_key && key_at.turned) turn(x, y, table, pairs, lane);
       store_codes<L>(x, y, key_at, in_key, lane, mask, codes_k + row * dk, scale_k + row);
     } else {
-      const int h = r - n_q - n_kv;
-      const size_t row = row0 + (size_t)h * s_max;
-      if (in_value) {
-        const __nv_bfloat16 *src = v.at(t, h);
-        load8<VEC>(src + value_at.e0, x);
-        load8<VEC>(src + value_at.e1, y);
-      }
+      const size_t row = row0 + (size_t)(r - n_q - n_kv) * s_max;
       store_codes<L>(x, y, value_at, in_value, lane, mask, codes_v + row * dv, scale_v + row);
     }
+    r = next;
   }
 }
 
