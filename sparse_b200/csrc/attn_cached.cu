@@ -434,7 +434,7 @@ struct Cursor {
 template <int DK, int DV, bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 && DK <= 128 ? 3 : 2)
 attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32_t *__restrict__ seq_lens, Shape s,
-                   float *__restrict__ part, float *__restrict__ part_lse) {
+                   float *__restrict__ part, float *__restrict__ part_lse, int2 *__restrict__ pieces) {
   using St = Stream<DK, DV, FP8, NT>;
   constexpr int kStep = 16 * St::U;
   static_assert(4 * kStep == kTile<FP8>, "four warps cover a tile");
@@ -526,6 +526,9 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
     // one piece: tiles of one segment
     const Cursor<FP8> now = at;
     const int piece_end = min(last, t + now.tiles - now.tile);
+    // the segment's slots follow one another: its first one, and how many, for attn_join_kernel
+    if (now.tile == 0 && threadIdx.x == 0)
+      pieces[now.segment(s)] = make_int2(blockIdx.x + now.segment(s), runs.cta_of(t + now.tiles - 1) - (int)blockIdx.x + 1);
     st.fetch(s_q[buffer], rows_of(now), g, c);
     buffer ^= 1;
     st.begin(s.scale_log2, c);
@@ -602,62 +605,55 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
   }
 }
 
-// One CTA per (sequence, query head): its pieces of the shared positions and of its own, weighted
-// by their sums of exponentials.  A lane of each warp looks after one piece's weight; then the
-// four warps sum a quarter of the pieces each, a lane its columns, with loads that do not wait
-// for one another.
-constexpr int kJoinWarps = 4;
+// One CTA per (sequence, key head, up to eight of its rows): each row's pieces of the shared
+// positions and of its own, weighted by their sums of exponentials.  A warp takes a row, or, where
+// there are fewer rows than four, a share of a row's pieces: a lane looks after one piece's
+// weight and then after its columns of all pieces, whose loads do not wait for one another.
+constexpr int kJoinRows = 8;
 template <int DV, bool FP8>
-__global__ void __launch_bounds__(kJoinWarps * 32)
-attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, const float *__restrict__ part,
-                 const float *__restrict__ part_lse, const float *__restrict__ pre_part, const float *__restrict__ pre_lse,
-                 __nv_bfloat16 *__restrict__ out) {
+__global__ void __launch_bounds__(kJoinRows * 32)
+attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, const int2 *__restrict__ pieces,
+                 const float *__restrict__ part, const float *__restrict__ part_lse, const float *__restrict__ pre_part,
+                 const float *__restrict__ pre_lse, __nv_bfloat16 *__restrict__ out) {
   constexpr int kCols = DV / 32;
-  __shared__ __align__(8) float s_acc[kJoinWarps][DV];
+  __shared__ __align__(8) float s_acc[kJoinRows][DV];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x;
-  const int b = row / s.n_q, h = row - b * s.n_q, hk = h / s.group, hg = h - hk * s.group;
-  int before = 0, all = 0;
-  for (int i = lane; i < s.B; i += 32) {
-    const int n = own_tiles<FP8>(s, seq_len(s, seq_lens, i));
-    all += n;
-    if (i < b) before += n;
-  }
-  before = warp_sum_int(before);
-  all = warp_sum_int(all);
-  const int own_heads = s.n_kv * s.row_tiles, pre_line = s.n_kv * s.pre_row_tiles * pre_tiles<FP8>(s);
-  const int total = pre_line + own_heads * all;
-  const Runs runs{total / n_ctas, total % n_ctas};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = min(s.group, kJoinRows), groups = (s.group + rows - 1) / rows;
+  const int share = rows < 3 ? 4 / rows : 1;             // warps of a row
+  const int head = blockIdx.x / groups, b = head / s.n_kv, hk = head - b * s.n_kv;
+  const int hg = (blockIdx.x - head * groups) * rows + warp / share, mine_of = warp % share;
+  const bool row_ok = warp / share < rows && hg < s.group;
   const int len = seq_len(s, seq_lens, b);
-  const bool prefix = s.shared_len > 0 && len >= s.shared_len;
   float top = -INFINITY, sum = 0.f, acc[kCols];
 #pragma unroll
   for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
-  // Where the row's pieces are: of the shared positions, then (a segment's slots follow one
-  // another: CTA + segment) of its own.
+  // where the row's pieces are: of the shared positions, then of its own
   const float *from[2] = {part, part}, *from_lse[2] = {part_lse, part_lse};
   size_t first_row[2] = {0, 0}, step[2] = {(size_t)s.rows, (size_t)s.rows};
   int n[2] = {0, 0};
-  const auto line = [&](int x, int first, int tiles, int segment, int r) {
-    const int cta = runs.cta_of(first);
-    first_row[x] = ((size_t)cta + segment) * s.rows + r;
-    n[x] = runs.cta_of(first + tiles - 1) - cta + 1;
-  };
-  if (s.pre_splits > 0 && prefix) {
-    const int r = b * s.group + hg, rt = r / s.pre_tile_rows;
-    from[0] = pre_part;
-    from_lse[0] = pre_lse;
-    step[0] = s.pre_rows;
-    first_row[0] = ((size_t)hk * s.pre_tiles + rt) * s.pre_splits * step[0] + r - rt * s.pre_tile_rows;
-    n[0] = s.pre_splits;
-  } else if (pre_line > 0 && prefix) {
-    const int r = b * s.group + hg, rt = r / s.rows, tiles = pre_tiles<FP8>(s), seg = hk * s.pre_row_tiles + rt;
-    line(0, seg * tiles, tiles, seg, r - rt * s.rows);
-  }
-  if (const int tiles = own_tiles<FP8>(s, len); tiles > 0) {
-    const int rt = hg / s.rows, w = hk * s.row_tiles + rt;
-    line(1, pre_line + own_heads * before + w * tiles, tiles, s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + w, hg - rt * s.rows);
+  if (row_ok) {
+    const int r = b * s.group + hg, rt = hg / s.rows;
+    if (s.shared_len > 0 && len >= s.shared_len) {
+      if (s.pre_splits > 0) {
+        const int tile = r / s.pre_tile_rows;
+        from[0] = pre_part;
+        from_lse[0] = pre_lse;
+        step[0] = s.pre_rows;
+        first_row[0] = ((size_t)hk * s.pre_tiles + tile) * s.pre_splits * step[0] + r - tile * s.pre_tile_rows;
+        n[0] = s.pre_splits;
+      } else {                                           // (all rows of a key head in one segment)
+        const int2 at = __ldg(pieces + hk);
+        first_row[0] = (size_t)at.x * s.rows + r;
+        n[0] = at.y;
+      }
+    }
+    if (own_tiles<FP8>(s, len) > 0) {
+      const int2 at = __ldg(pieces + s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + hk * s.row_tiles + rt);
+      first_row[1] = (size_t)at.x * s.rows + hg - rt * s.rows;
+      n[1] = at.y;
+    }
   }
   for (int i0 = 0; i0 < n[0] + n[1]; i0 += 32) {
     const int here = min(32, n[0] + n[1] - i0), mine = i0 + lane, x = mine < n[0] ? 0 : 1;
@@ -676,7 +672,7 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
 #pragma unroll
     for (int e = 0; e < kCols; ++e) acc[e] *= f;
 #pragma unroll 8
-    for (int i = warp; i < here; i += kJoinWarps) {
+    for (int i = mine_of; i < here; i += share) {
       const float wi = __shfl_sync(0xffffffffu, w, i);
       const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), i)) + lane * kCols;
       if constexpr (kCols == 4) {
@@ -689,20 +685,21 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, int n_ctas, cons
     }
     top = most;
   }
+  if (share > 1) {
 #pragma unroll
-  for (int e = 0; e < kCols; ++e) s_acc[warp][lane * kCols + e] = acc[e];
-  __syncthreads();
-  if (threadIdx.x < DV / 2) {
-    float2 o = make_float2(0.f, 0.f);
+    for (int e = 0; e < kCols; ++e) s_acc[warp][lane * kCols + e] = acc[e];
+    __syncthreads();
+    if (mine_of != 0) return;
+    for (int y = 1; y < share; ++y)
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float2 x = *reinterpret_cast<const float2 *>(&s_acc[w][2 * threadIdx.x]);
-      o.x += x.x; o.y += x.y;
-    }
-    // no piece, or only such without weight: zeros
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint32_t *>(out + (size_t)row * DV + 2 * threadIdx.x) = sum == 0.f ? 0u : pack_bf16x2(o.x * f, o.y * f);
+      for (int e = 0; e < kCols; ++e) acc[e] += s_acc[warp + y][lane * kCols + e];
   }
+  if (!row_ok) return;
+  // no piece, or only such without weight: zeros
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  uint32_t *dst = reinterpret_cast<uint32_t *>(out + ((size_t)b * s.n_q + hk * s.group + hg) * DV + lane * kCols);
+#pragma unroll
+  for (int e = 0; e < kCols; e += 2) dst[e / 2] = sum == 0.f ? 0u : pack_bf16x2(acc[e] * f, acc[e + 1] * f);
 }
 
 constexpr int kMaxRows = 16;
@@ -719,15 +716,17 @@ void plan(Shape &s, int dk) {
   s.row_tiles = (s.group + s.rows - 1) / s.rows;
   s.pre_row_tiles = pre_rows > 0 && s.pre_splits == 0 ? 1 : 0;
 }
-// Partial results: of the streamed line, then of the shared positions' tiles; outputs first,
-// then logarithms.
-int64_t slot_rows(const Shape &s) { return (kMaxCtas + (int64_t)s.n_kv * (s.pre_row_tiles + (int64_t)s.B * s.row_tiles)) * s.rows; }
+// Workspace: partial results of the streamed line and of the shared positions' tiles, then their
+// logarithms, then the place of each segment's pieces.
+int64_t segments(const Shape &s) { return (int64_t)s.n_kv * (s.pre_row_tiles + (int64_t)s.B * s.row_tiles); }
+int64_t slot_rows(const Shape &s) { return (kMaxCtas + segments(s)) * s.rows; }
 int64_t pre_slot_rows(const Shape &s) { return s.pre_splits > 0 ? prefix_slots(s) * s.pre_rows : 0; }
 
 template <int DK, int DV, bool FP8>
 int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_lens, const Shape &s, float *part,
                __nv_bfloat16 *out, int32_t *status, cudaStream_t st) {
   float *pre_part = part + slot_rows(s) * DV, *lse = pre_part + pre_slot_rows(s) * DV, *pre_lse = lse + slot_rows(s);
+  int2 *pieces = reinterpret_cast<int2 *>((reinterpret_cast<uintptr_t>(pre_lse + pre_slot_rows(s)) + 7) & ~(uintptr_t)7);
   if (s.pre_splits > 0) {
     const int32_t rc = launch_attn_prefix(FP8, DK, DV, q, cache, s, pre_part, pre_lse, status, st);
     if (rc != SB_OK) return rc;
@@ -739,11 +738,13 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
   const int per_sm = s.rows <= 8 && DK <= 128 ? 3 : 2, most = per_sm * sms < kMaxCtas ? per_sm * sms : kMaxCtas;
   const int ctas = tiles < most ? (int)tiles : most;
   auto kern = s.rows <= 8 ? attn_stream_kernel<DK, DV, FP8, 1> : attn_stream_kernel<DK, DV, FP8, 2>;
-  SB_CUDA_CHECK(launch_pdl(kern, dim3(ctas), dim3(kThreads), 0, st, q, cache, seq_lens, s, part, lse));
+  SB_CUDA_CHECK(launch_pdl(kern, dim3(ctas), dim3(kThreads), 0, st, q, cache, seq_lens, s, part, lse, pieces));
   SB_LAUNCH_CHECK();
-  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3(s.B * s.n_q), dim3(kJoinWarps * 32), 0, st, seq_lens, s, ctas,
-                           static_cast<const float *>(part), static_cast<const float *>(lse),
-                           static_cast<const float *>(pre_part), static_cast<const float *>(pre_lse), out));
+  const int rows = s.group < kJoinRows ? s.group : kJoinRows, warps = rows < 4 ? 4 : rows;
+  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3(s.B * s.n_kv * ((s.group + rows - 1) / rows)), dim3(warps * 32), 0, st,
+                           seq_lens, s, static_cast<const int2 *>(pieces), static_cast<const float *>(part),
+                           static_cast<const float *>(lse), static_cast<const float *>(pre_part),
+                           static_cast<const float *>(pre_lse), out));
   SB_LAUNCH_CHECK();
   return SB_OK;
 }
@@ -796,7 +797,7 @@ size_t sb_attn_cached_workspace_bytes(int32_t B, int32_t n_q, int32_t n_kv, int3
     return 0;
   Shape s = {B, n_q, n_kv, n_q / n_kv, s_max, shared_len, 0, 0, 0, 0, 0, 0, 0, 0, 0.f};
   plan(s, dk);
-  return (size_t)(slot_rows(s) + pre_slot_rows(s)) * (dv + 1) * sizeof(float);
+  return (size_t)(slot_rows(s) + pre_slot_rows(s)) * (dv + 1) * sizeof(float) + (size_t)(segments(s) + 1) * sizeof(int2);
 }
 
 int32_t sb_attn_decode_shared(const sb_attn_cached_args *args, void *stream) {
