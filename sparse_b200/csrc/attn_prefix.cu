@@ -136,29 +136,22 @@ __device__ __forceinline__ void convert16(const uint4 &c, float scale, uint4 &lo
 
 constexpr float kNone = -3.0e38f;                // the maximum of no score, or of scores of -inf alone
 
-// 32 scores of a row from position x of its block on; in the last blocks (TAIL) those behind the last
-// shared position are -inf.
-template <bool TAIL>
-__device__ __forceinline__ void row_scores(uint32_t st_at, int x, int keys, uint32_t (&r)[32]) {
-  tc_ld32(st_at + x, r);
-  tc_wait_ld();
-  if constexpr (TAIL) {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) r[e] = x + e < keys ? r[e] : 0xff800000u;
-  }
-}
-
-// The largest score of a row, kNone at least.
+// The largest score of a row, kNone at least.  In the last blocks (TAIL) only the first `keys`
+// positions count.
 template <bool TAIL>
 __device__ __forceinline__ float row_top(uint32_t st_at, int keys) {
   float top[4] = {kNone, kNone, kNone, kNone};
 #pragma unroll
   for (int x = 0; x < kBlock; x += 32) {
     uint32_t r[32];
-    row_scores<TAIL>(st_at, x, keys, r);
+    tc_ld32(st_at + x, r);
+    tc_wait_ld();
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      top[e & 3] = fmaxf(top[e & 3], fmaxf(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])));
+    for (int e = 0; e < 16; ++e) {
+      const float a = TAIL && x + 2 * e >= keys ? kNone : __uint_as_float(r[2 * e]);
+      const float b = TAIL && x + 2 * e + 1 >= keys ? kNone : __uint_as_float(r[2 * e + 1]);
+      top[e & 3] = fmaxf(top[e & 3], fmaxf(a, b));
+    }
   }
   return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
@@ -171,11 +164,16 @@ __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float sc
 #pragma unroll
   for (int x = 0; x < kBlock; x += 32) {
     uint32_t r[32], p[16];
-    row_scores<TAIL>(st_at, x, keys, r);
+    tc_ld32(st_at + x, r);
+    tc_wait_ld();
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float a = exp2_approx(fmaf(__uint_as_float(r[2 * e]), scale_log2, -m));
-      const float b = exp2_approx(fmaf(__uint_as_float(r[2 * e + 1]), scale_log2, -m));
+      float a = exp2_approx(fmaf(__uint_as_float(r[2 * e]), scale_log2, -m));
+      float b = exp2_approx(fmaf(__uint_as_float(r[2 * e + 1]), scale_log2, -m));
+      if constexpr (TAIL) {
+        a = x + 2 * e < keys ? a : 0.f;
+        b = x + 2 * e + 1 < keys ? b : 0.f;
+      }
       sum[e & 3] += a + b;
       p[e] = pack_bf16x2(a, b);
     }

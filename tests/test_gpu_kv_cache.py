@@ -530,3 +530,14 @@ def test_calls_back_to_back_end_in_time_with_the_same_bits(kind, b, n_q, n_kv, d
     for _ in range(300):
         wrong += (call() != want).sum()
     assert int(status) == 0 and int(wrong) == 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("b,n_kv,shared", [(3, 2, 0), (3, 2, 77), (200, 8, 77)])
+def test_a_scale_of_zero_weighs_all_positions_alike(kind, b, n_kv, shared):
+    s_max = 140
+    q, k, v = _rand(b, 2 * n_kv, 64, seed=1), _rand(b, n_kv, s_max, 64, seed=2), _rand(b, n_kv, s_max, 64, seed=3)
+    lens = [77 + i % 64 for i in range(b)]
+    got, kk, vv = _attend(kind, q, k, v, lens, shared, scale=0.0)
+    want, tol = _want(q, kk, vv, lens, shared, 0.0)
+    assert bool(((got.double() - want).abs() <= tol).all())
