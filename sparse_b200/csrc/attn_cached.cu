@@ -17,6 +17,8 @@
 // or reaches over several leaves a partial result for each, and attn_join_kernel joins those.
 #include <math.h>
 
+#include <type_traits>
+
 #include "attn_cached.cuh"
 
 namespace sb {
@@ -606,60 +608,61 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
 }
 
 // One CTA per (sequence, key head, up to eight of its rows): each row's pieces of the shared
-// positions and of its own, weighted by their sums of exponentials.  A warp takes a row, or, where
-// there are fewer rows than four, a share of a row's pieces: a lane looks after one piece's
-// weight and then after its columns of all pieces, whose loads do not wait for one another.
+// positions and of its own, weighted by their sums of exponentials.  SHARE warps take a row (four
+// where a key head has one row, two where it has two).  Bound by round trips to L2, so there are
+// two behind one another: the length and the place of the pieces, then their rows and, at the same
+// time, their logarithms (lane i looks after the weight of piece i of a round).
 constexpr int kJoinRows = 8;
-template <int DV, bool FP8>
+template <int DV, int SHARE>
 __global__ void __launch_bounds__(kJoinRows * 32)
 attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, const int2 *__restrict__ pieces,
                  const float *__restrict__ part, const float *__restrict__ part_lse, const float *__restrict__ pre_part,
                  const float *__restrict__ pre_lse, __nv_bfloat16 *__restrict__ out) {
-  constexpr int kCols = DV / 32;
-  __shared__ __align__(8) float s_acc[kJoinRows][DV];
+  constexpr int kCols = DV / 32, kAhead = SHARE == 1 ? 16 : 8, kRound = kAhead * SHARE;       // at most a warp's lanes
+  using Vec = typename std::conditional<kCols == 4, float4, float2>::type;
+  __shared__ __align__(16) float s_acc[kJoinRows][DV];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = min(s.group, kJoinRows), groups = (s.group + rows - 1) / rows;
-  const int share = rows < 3 ? 4 / rows : 1;             // warps of a row
   const int head = blockIdx.x / groups, b = head / s.n_kv, hk = head - b * s.n_kv;
-  const int hg = (blockIdx.x - head * groups) * rows + warp / share, mine_of = warp % share;
-  const bool row_ok = warp / share < rows && hg < s.group;
+  const int hg = (blockIdx.x - head * groups) * rows + warp / SHARE, mine_of = warp % SHARE;
+  const bool row_ok = warp / SHARE < rows && hg < s.group;
+  const int rt = min(hg, s.group - 1) / s.rows, r = b * s.group + hg;
   const int len = seq_len(s, seq_lens, b);
-  float top = -INFINITY, sum = 0.f, acc[kCols];
+  const int2 own_at = __ldg(pieces + s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + hk * s.row_tiles + rt);
+  const int2 pre_at = s.pre_row_tiles > 0 ? __ldg(pieces + hk) : make_int2(0, 0);
+  // pieces: of the shared positions, then of the sequence's own (whose place stands only where there are any)
+  const float *pre = part, *pre_l = part_lse;
+  size_t pre_first = (size_t)pre_at.x * s.rows + r, pre_step = s.rows;
+  int n_pre = pre_at.y;
+  if (s.pre_splits > 0) {
+    const int tile = r / s.pre_tile_rows;
+    pre = pre_part;
+    pre_l = pre_lse;
+    pre_step = s.pre_rows;
+    pre_first = ((size_t)hk * s.pre_tiles + tile) * s.pre_splits * pre_step + r - tile * s.pre_tile_rows;
+    n_pre = s.pre_splits;
+  }
+  if (s.shared_len == 0 || len < s.shared_len) n_pre = 0;
+  const size_t own_first = (size_t)own_at.x * s.rows + hg - rt * s.rows;
+  const int n = row_ok ? n_pre + (len > own_begin(s, len) ? own_at.y : 0) : 0;
+  const auto row_of = [&](int i) { return i < n_pre ? pre_first + i * pre_step : own_first + (size_t)(i - n_pre) * s.rows; };
+  float top = -INFINITY, sum = 0.f;
+  __align__(16) float acc[kCols];
 #pragma unroll
   for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
-  // where the row's pieces are: of the shared positions, then of its own
-  const float *from[2] = {part, part}, *from_lse[2] = {part_lse, part_lse};
-  size_t first_row[2] = {0, 0}, step[2] = {(size_t)s.rows, (size_t)s.rows};
-  int n[2] = {0, 0};
-  if (row_ok) {
-    const int r = b * s.group + hg, rt = hg / s.rows;
-    if (s.shared_len > 0 && len >= s.shared_len) {
-      if (s.pre_splits > 0) {
-        const int tile = r / s.pre_tile_rows;
-        from[0] = pre_part;
-        from_lse[0] = pre_lse;
-        step[0] = s.pre_rows;
-        first_row[0] = ((size_t)hk * s.pre_tiles + tile) * s.pre_splits * step[0] + r - tile * s.pre_tile_rows;
-        n[0] = s.pre_splits;
-      } else {                                           // (all rows of a key head in one segment)
-        const int2 at = __ldg(pieces + hk);
-        first_row[0] = (size_t)at.x * s.rows + r;
-        n[0] = at.y;
-      }
+  for (int i0 = 0; i0 < n; i0 += kRound) {
+    Vec v[kAhead];
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      const int i = i0 + y * SHARE + mine_of;
+      v[y] = Vec{};
+      if (i < n) v[y] = __ldg(reinterpret_cast<const Vec *>((i < n_pre ? pre : part) + row_of(i) * DV) + lane);
     }
-    if (own_tiles<FP8>(s, len) > 0) {
-      const int2 at = __ldg(pieces + s.n_kv * (s.pre_row_tiles + b * s.row_tiles) + hk * s.row_tiles + rt);
-      first_row[1] = (size_t)at.x * s.rows + hg - rt * s.rows;
-      n[1] = at.y;
-    }
-  }
-  for (int i0 = 0; i0 < n[0] + n[1]; i0 += 32) {
-    const int here = min(32, n[0] + n[1] - i0), mine = i0 + lane, x = mine < n[0] ? 0 : 1;
-    const size_t at = first_row[x] + (mine - (x ? n[0] : 0)) * step[x];
-    const float lse = lane < here ? from_lse[x][at] : -INFINITY;
-    const float *mine_at = from[x] + at * DV;
+    const int mine = i0 + lane;
+    const bool ok = lane < kRound && mine < n;
+    const float lse = ok ? __ldg((mine < n_pre ? pre_l : part_lse) + row_of(mine)) : -INFINITY;
     float most = lse;
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
@@ -671,26 +674,20 @@ attn_join_kernel(const int32_t *__restrict__ seq_lens, Shape s, const int2 *__re
     sum = sum * f + weights;
 #pragma unroll
     for (int e = 0; e < kCols; ++e) acc[e] *= f;
-#pragma unroll 8
-    for (int i = mine_of; i < here; i += share) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), i)) + lane * kCols;
-      if constexpr (kCols == 4) {
-        const float4 v = *reinterpret_cast<const float4 *>(src);
-        acc[0] += wi * v.x; acc[1] += wi * v.y; acc[2] += wi * v.z; acc[3] += wi * v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2 *>(src);
-        acc[0] += wi * v.x; acc[1] += wi * v.y;
-      }
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      const float wy = __shfl_sync(0xffffffffu, w, y * SHARE + mine_of);
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) acc[e] += wy * reinterpret_cast<const float *>(&v[y])[e];
     }
     top = most;
   }
-  if (share > 1) {
-#pragma unroll
-    for (int e = 0; e < kCols; ++e) s_acc[warp][lane * kCols + e] = acc[e];
+  if (SHARE > 1) {
+    *(reinterpret_cast<Vec *>(s_acc[warp]) + lane) = *reinterpret_cast<const Vec *>(acc);
     __syncthreads();
     if (mine_of != 0) return;
-    for (int y = 1; y < share; ++y)
+#pragma unroll
+    for (int y = 1; y < SHARE; ++y)
 #pragma unroll
       for (int e = 0; e < kCols; ++e) acc[e] += s_acc[warp + y][lane * kCols + e];
   }
@@ -741,7 +738,8 @@ int32_t launch(const __nv_bfloat16 *q, const Cache &cache, const int32_t *seq_le
   SB_CUDA_CHECK(launch_pdl(kern, dim3(ctas), dim3(kThreads), 0, st, q, cache, seq_lens, s, part, lse, pieces));
   SB_LAUNCH_CHECK();
   const int rows = s.group < kJoinRows ? s.group : kJoinRows, warps = rows < 4 ? 4 : rows;
-  SB_CUDA_CHECK(launch_pdl(attn_join_kernel<DV, FP8>, dim3(s.B * s.n_kv * ((s.group + rows - 1) / rows)), dim3(warps * 32), 0, st,
+  auto join = rows == 1 ? attn_join_kernel<DV, 4> : rows == 2 ? attn_join_kernel<DV, 2> : attn_join_kernel<DV, 1>;
+  SB_CUDA_CHECK(launch_pdl(join, dim3(s.B * s.n_kv * ((s.group + rows - 1) / rows)), dim3(warps * 32), 0, st,
                            seq_lens, s, static_cast<const int2 *>(pieces), static_cast<const float *>(part),
                            static_cast<const float *>(lse), static_cast<const float *>(pre_part),
                            static_cast<const float *>(pre_lse), out));
