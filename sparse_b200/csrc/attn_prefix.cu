@@ -120,18 +120,56 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
   return (uint32_t)(chunk >> 3) * kBox + (uint32_t)row * 128 + (uint32_t)(((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// sixteen codes (one 16-byte chunk) times a power of two -> two chunks of bf16, exact
-__device__ __forceinline__ void convert16(const uint4 &c, float scale, uint4 &lo, uint4 &hi) {
+// Codes -> bf16 operands, exact.  An e4m3 byte s eeee mmm put at bit 4 of a bf16 (s 0000eeee mmm0000) is
+// the code's value times 2^-120 (subnormal codes included: both types have the same step there), so
+// one packed multiplication by 2^(e + 120) makes two operands; powers above bf16's largest, 2^127,
+// in two steps.
+struct RowScale { uint32_t first, second; };           // bf16 pairs; second: 1 unless e > 7
+__device__ __forceinline__ RowScale row_scale(uint32_t byte) {
+  if (byte == kScaleNan) return RowScale{0x7fc07fc0u, 0x3f803f80u};
+  const uint32_t first = min(byte + 120u, 254u), second = 127u + (byte + 120u - first);
+  return RowScale{(first << 7) * 0x10001u, (second << 7) * 0x10001u};
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// sixteen codes (one 16-byte chunk) -> two chunks
+template <bool TWICE>
+__device__ __forceinline__ void convert16(const uint4 &c, RowScale scale, uint4 &lo, uint4 &hi) {
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
   uint32_t o[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 a = f16x2_to_float2(e4m3x2_to_f16x2(w[i])), b = f16x2_to_float2(e4m3x2_to_f16x2(w[i] >> 16));
-    o[2 * i] = pack_bf16x2(a.x * scale, a.y * scale);
-    o[2 * i + 1] = pack_bf16x2(b.x * scale, b.y * scale);
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t t = __byte_perm(w[i >> 1], 0, i & 1 ? 0x3424 : 0x1404);       // two codes, each in the high byte of a half
+    o[i] = mul_bf16x2(((t >> 4) & 0x07f007f0u) | (t & 0x80008000u), scale.first);
+    if (TWICE) o[i] = mul_bf16x2(o[i], scale.second);
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// two fp32 operations at once
+__device__ __forceinline__ unsigned long long pack_f32x2(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(unsigned long long v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma_f32x2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 constexpr float kNone = -3.0e38f;                // the maximum of no score, or of scores of -inf alone
@@ -160,7 +198,8 @@ __device__ __forceinline__ float row_top(uint32_t st_at, int keys) {
 // stored behind the scores it replaces); returns their sum.
 template <bool TAIL>
 __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float scale_log2, float m) {
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  unsigned long long sum[2] = {0ull, 0ull};
+  const unsigned long long scale2 = pack_f32x2(scale_log2, scale_log2), m2 = pack_f32x2(-m, -m);
 #pragma unroll
   for (int x = 0; x < kBlock; x += 32) {
     uint32_t r[32], p[16];
@@ -168,18 +207,19 @@ __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float sc
     tc_wait_ld();
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      float a = exp2_approx(fmaf(__uint_as_float(r[2 * e]), scale_log2, -m));
-      float b = exp2_approx(fmaf(__uint_as_float(r[2 * e + 1]), scale_log2, -m));
+      const float2 t = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), scale2, m2));
+      float a = exp2_approx(t.x), b = exp2_approx(t.y);
       if constexpr (TAIL) {
         a = x + 2 * e < keys ? a : 0.f;
         b = x + 2 * e + 1 < keys ? b : 0.f;
       }
-      sum[e & 3] += a + b;
+      sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(a, b));
       p[e] = pack_bf16x2(a, b);
     }
     tc_st16(st_at + x / 2, p);
   }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  const float2 s = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+  return s.x + s.y;
 }
 
 // Warps of a group that have one of its `rows` rows (one at least: a barrier counts them).  What
@@ -314,29 +354,26 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       tc_fence_after();
       return ok;
     };
-    const auto scores = [&](int j) {
+    // scores of block j of group w
+    const auto scores = [&](int j, int w) {
       const int i = tile_of(j), st = i % NS;
-      if ((!TWO || !(j & 1)) && !wait(k_full + 8 * st, (i / NS) & 1)) return false;
+      if (w == 0 && (!TWO || !(j & 1)) && !wait(k_full + 8 * st, (i / NS) & 1)) return false;
       if (leader) {
+        const uint64_t a = q_desc + (TWO ? w * (L::kQ >> 4) : 0), b = k_desc + (uint64_t)(st * (L::kK >> 4) + half_of(j, w) * half_rows);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint64_t a = q_desc + (TWO ? w * (L::kQ >> 4) : 0), b = k_desc + (uint64_t)(st * (L::kK >> 4) + half_of(j, w) * half_rows);
-#pragma unroll
-          for (int x = 0; x < DK / 16; ++x) {
-            const uint64_t off = (uint64_t)((x >> 2) * (kBox >> 4) + (x & 3) * 2);
-            tc_mma_ss(s_tmem + (2 * w + (j & 1)) * kBlock, a + off, b + off, id_s, x > 0);
-          }
-          tc_commit(s_full + 8 * (2 * w + (j & 1)));
+        for (int x = 0; x < DK / 16; ++x) {
+          const uint64_t off = (uint64_t)((x >> 2) * (kBox >> 4) + (x & 3) * 2);
+          tc_mma_ss(s_tmem + (2 * w + (j & 1)) * kBlock, a + off, b + off, id_s, x > 0);
         }
-        if (!TWO || (j & 1)) tc_commit(k_empty + 8 * st);
+        tc_commit(s_full + 8 * (2 * w + (j & 1)));
+        if (w == 1 && (!TWO || (j & 1))) tc_commit(k_empty + 8 * st);
       }
       __syncwarp();
       return true;
     };
-    bool ok = scores(0);
+    bool ok = true;
+    for (int j = 0; j < 2 && j < blocks; ++j) ok = ok && scores(j, 0) && scores(j, 1);
     for (int j = 0; ok && j < blocks; ++j) {
-      // (the scores of block j + 1 go where those of j - 1 were: their second product is issued)
-      if (j + 1 < blocks && !scores(j + 1)) break;
       const int i = tile_of(j), st = i % NS;
       if ((!TWO || !(j & 1)) && !wait(v_full + 8 * st, (i / NS) & 1)) break;
 #pragma unroll
@@ -351,6 +388,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           if (w == 1 && (!TWO || (j & 1))) tc_commit(v_empty + 8 * st);
         }
         __syncwarp();
+        // (block j + 2's scores go where this block's probabilities are: products run in the order of their issue)
+        if (ok && j + 2 < blocks) ok = scores(j + 2, w);
       }
     }
   } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
@@ -476,14 +515,16 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       if (!__all_sync(0xffffffffu, ok)) break;
       const unsigned char *src = aligned_base + (raw_smem - base) + st * (L::kRawK + L::kRawV) + (keys_side ? 0 : L::kRawK) + row * d;
       unsigned char *dst = aligned_base + (op_smem - base) + op * op_bytes;
-      const float scale = e8m0_value(byte);
+      const RowScale scale = in ? row_scale(byte) : RowScale{0u, 0u};
+      const bool twice = __any_sync(0xffffffffu, in && scale.second != 0x3f803f80u);
       const int op_row = (i & 1) * kBlock + row;
       int chunk = start;
 #pragma unroll 4
       for (int x = 0; x < chunks / 2; ++x) {
         uint4 c = make_uint4(0, 0, 0, 0), lo, hi;
         if (in) c = *reinterpret_cast<const uint4 *>(src + chunk * 16);       // (behind the end stands whatever was there before)
-        convert16(c, in ? scale : 0.f, lo, hi);
+        if (twice) convert16<true>(c, scale, lo, hi);
+        else convert16<false>(c, scale, lo, hi);
         *reinterpret_cast<uint4 *>(dst + swizzled(op_row, 2 * chunk)) = lo;
         *reinterpret_cast<uint4 *>(dst + swizzled(op_row, 2 * chunk + 1)) = hi;
         chunk = chunk + 2 >= chunks ? chunk + 2 - chunks : chunk + 2;

@@ -541,3 +541,23 @@ def test_a_scale_of_zero_weighs_all_positions_alike(kind, b, n_kv, shared):
     got, kk, vv = _attend(kind, q, k, v, lens, shared, scale=0.0)
     want, tol = _want(q, kk, vv, lens, shared, 0.0)
     assert bool(((got.double() - want).abs() <= tol).all())
+
+
+def test_shared_prefix_with_values_of_any_size():
+    """Quantised rows with powers of two from the smallest to the largest, through the tensor-core pass: the operand
+    that a code becomes is exact for every one of them."""
+    b, n, d, shared = 130, 16, 64, 256
+    q = torch.zeros(b, n, d, dtype=BF, device=DEV)
+    q[:, :, 0] = 1.0
+    k = torch.zeros(b, n, shared + 1, d, dtype=BF, device=DEV)
+    v = _rand(b, n, shared + 1, d, seed=4)
+    # every shared position is the one that counts for some query row: positions differ in their first 8 key bits
+    sizes = torch.linspace(-120, 100, shared, device=DEV).round()
+    v[0, :, :shared] = (v[0, :, :shared].double() * torch.exp2(sizes.double())[None, :, None]).to(BF)
+    for at in (0, 1, 17, 100, 130, 150, 180, 200, 240, 255):
+        k.zero_()
+        k[0, :, at, 0] = 300.0
+        got, _, vv = _attend("fp8", q, k, v, [shared + 1] * b, shared, scale=1.0)
+        want = vv[0, :, at].expand(b, -1, -1)
+        # the others weigh exp(-300): nothing, whatever their size
+        assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs()).all()), at
