@@ -109,8 +109,9 @@ __device__ __forceinline__ void store_bf16(__nv_bfloat16 *p, const float (&x)[8]
 }
 
 // grid = (tokens, shares of a token's rows).  A token's angles are worked out once per CTA:
-// turns = pos * frequency as a product of three floats without error in its fraction, so
-// positions far into a long context have the angle of the 64-bit formula to fp32's last bits.
+// turns = pos * frequency, both as sums of two floats, the large product without error in its
+// fraction, so positions far into a long context have the angle of the 64-bit formula to fp32's
+// last bits (to 2^-14 at the last positions that 32 bits have).
 template <int L, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads)
 rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource v, __nv_bfloat16 *__restrict__ q_out,
@@ -144,9 +145,11 @@ rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource
   fetch(r, a, b);
   const int pos = pos_of_token[t], seq = seq_of_token[t];
   if (threadIdx.x < half) {
-    const float p = (float)pos, hi = freq.turns[threadIdx.x].x, lo = freq.turns[threadIdx.x].y;
+    // (pos = p + what a float's 24 bits leave of it, none below 2^24)
+    const float p = __int2float_rz(pos), rest = (float)(pos - (int)p);
+    const float hi = freq.turns[threadIdx.x].x, lo = freq.turns[threadIdx.x].y;
     const float f = p * hi;
-    const float turns = (f - rintf(f)) + (fmaf(p, hi, -f) + p * lo);
+    const float turns = (f - rintf(f)) + (fmaf(p, hi, -f) + (p * lo + rest * hi));
     float sn, cs;
     sincospif(2.f * turns, &sn, &cs);
     table[(threadIdx.x & 7) * pairs + (threadIdx.x >> 3)] = make_float2(cs, sn);

@@ -170,6 +170,19 @@ def test_append_angles_of_far_positions(pos):
     assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 5 * 2.0 ** -21).all())
 
 
+@pytest.mark.parametrize("pos", [2 ** 24 + 1, 2 ** 29 + 12345677, 2 ** 31 - 1, -(2 ** 24) - 3])
+def test_append_angles_of_positions_that_fp32_does_not_have(pos):
+    """Four sums of turns of at most 2^6, half an ulp each, are 2^-17 turns: 2^-14 rad."""
+    q = _rand(1, 2, 128, seed=pos % 97)
+    cache = QuantizedCache.zeros(1, 1, 2, 128, 128, DEV)
+    p = torch.tensor([pos], dtype=torch.int32, device=DEV)
+    out = ops.rope_append_quantized(q, q, None, q, torch.zeros_like(p), p, cache, 1e6)
+    ang = pos * 1e6 ** (-torch.arange(64, device=DEV).double() / 64)
+    a, c = q[..., :64].double(), q[..., 64:].double()
+    want = torch.cat([a * ang.cos() - c * ang.sin(), c * ang.cos() + a * ang.sin()], -1)
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 5 * 2.0 ** -13).all())
+
+
 # -- read back -------------------------------------------------------------------------------
 @pytest.mark.parametrize("b,n,dk,dv,begin,count,shared", [
     (1, 1, 16, 16, 0, 1, 0), (3, 2, 64, 64, 3, 37, 11), (2, 16, 128, 128, 0, 40, 40), (2, 3, 192, 128, 39, 1, 40),
@@ -249,6 +262,21 @@ def test_attention(kind, n_q, n_kv, dk, dv, lens, shared, s_max):
     assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() - tol).max())
     # of the whole: the roundings are independent of one another, so well inside the bound of each
     assert float((got.double() - want).norm()) <= 2.0 ** -8 * max(float(want.norm()), 1e-30)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("n_q,n_kv,shared,step", [(4, 2, 0, 31), (4, 4, 60, 7), (320, 160, 60, 211)])
+def test_many_sequences_of_which_few_have_positions(kind, n_q, n_kv, shared, step):
+    """Empty sequences before, between and behind the others; more tiles of the shared positions than SMs."""
+    b, s_max, d = 1000 if n_kv < 100 else 300, 200, 64
+    lens = [0] * b
+    for i in range(step, b - 40, step):
+        lens[i] = 1 + (i * 37) % s_max
+    lens[0] = shared
+    q, k, v = _rand(b, n_q, d, seed=5), _rand(b, n_kv, s_max, d, seed=6), _rand(b, n_kv, s_max, d, seed=7)
+    got, kk, vv = _attend(kind, q, k, v, lens, shared)
+    want, tol = _want(q, kk, vv, lens, shared, d ** -0.5)
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() - tol).max())
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
