@@ -556,12 +556,6 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 
 // The shared rows of a bf16 cache as [shared_len][n_kv][d], boxes of 64 columns, one head, 128 positions.
 int32_t encode_rows(CUtensorMap *tm, const void *base, int d, int n_kv, int shared_len) {
-  // A map depends on these values only: the last ones of a thread are kept, as for the grouped GEMM.
-  struct Entry { const void *base; int d, n_kv, len; CUtensorMap map; };
-  static thread_local Entry kept[64];
-  static thread_local int used = 0, next = 0;
-  for (int i = 0; i < used; ++i)
-    if (kept[i].base == base && kept[i].d == d && kept[i].n_kv == n_kv && kept[i].len == shared_len) { *tm = kept[i].map; return SB_OK; }
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(SB_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)n_kv, (cuuint64_t)shared_len};
@@ -571,8 +565,6 @@ int32_t encode_rows(CUtensorMap *tm, const void *base, int d, int n_kv, int shar
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(SB_E_CUDA, "cuTensorMapEncodeTiled of the shared rows failed with CUresult %d", (int)r);
-  const int slot = used < 64 ? used++ : next++ % 64;
-  kept[slot] = Entry{base, d, n_kv, shared_len, *tm};
   return SB_OK;
 }
 
