@@ -635,8 +635,8 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  *                  (i, i + rope_dim/2), angle pos * theta^(-2i/rope_dim)), stores q to
  *                  q_out [T,n_q,dk] bf16 (q itself is not written) and quantises k and v
  *                  into row (seq_of_token[t], pos_of_token[t]).  Angles, products and the
- *                  scaled row are fp32, a value is rounded once; angles are those of the
- *                  64-bit formula within 2^-20, from position 2^24 on within 2^-14.  A key
+ *                  scaled row are fp32, a value is rounded once; cosines and sines are
+ *                  those of the 64-bit formula within 2^-23, from position 2^24 on 2^-14.  A key
  *                  head's first rope_dim elements come from k_rot and the others from k_rest
  *                  (NULL where there are none).  stride: elements between tokens and between
  *                  heads of each; a head stride of 0 shares one row between the heads.  A

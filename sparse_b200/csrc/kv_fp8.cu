@@ -82,6 +82,12 @@ __device__ __forceinline__ float max_abs(float a, float b) {
   return r;
 }
 
+// a + b as the rounded sum and what the rounding leaves
+__device__ __forceinline__ float2 two_sum(float a, float b) {
+  const float s = __fadd_rn(a, b), b_part = __fsub_rn(s, a);
+  return make_float2(s, __fadd_rn(__fsub_rn(a, __fsub_rn(s, b_part)), __fsub_rn(b, b_part)));
+}
+
 // Codes and scale byte of the row that L lanes hold (`mask`: those lanes), `in`: the lane has values of it.
 template <int L>
 __device__ __forceinline__ void store_codes(float (&x)[8], float (&y)[8], RowPlace at, bool in, int lane, uint32_t mask,
@@ -110,8 +116,10 @@ __device__ __forceinline__ void store_bf16(__nv_bfloat16 *p, const float (&x)[8]
 
 // grid = (tokens, shares of a token's rows).  A token's angles are worked out once per CTA:
 // turns = pos * frequency, both as sums of two floats, the large product without error in its
-// fraction, so positions far into a long context have the angle of the 64-bit formula to fp32's
-// last bits (to 2^-14 at the last positions that 32 bits have).
+// fraction and what a float leaves of the turns put behind the sine and cosine, so that these are
+// the 64-bit formula's to fp32's last bits, far into a long context too (to 2^-14 at the last
+// positions that 32 bits have): codes differ from the 64-bit rows' as often as those of rows turned
+// by correctly rounded cosines do (148 each of 132 million values, positions up to 30 thousand).
 template <int L, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads)
 rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource v, __nv_bfloat16 *__restrict__ q_out,
@@ -149,9 +157,14 @@ rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource
     const float p = __int2float_rz(pos), rest = (float)(pos - (int)p);
     const float hi = freq.turns[threadIdx.x].x, lo = freq.turns[threadIdx.x].y;
     const float f = p * hi;
-    const float turns = (f - rintf(f)) + (fmaf(p, hi, -f) + (p * lo + rest * hi));
+    const float2 whole = two_sum(f - rintf(f), fmaf(p, hi, -f));
+    const float2 turns = two_sum(whole.x, p * lo + rest * hi);
     float sn, cs;
-    sincospif(2.f * turns, &sn, &cs);
+    sincospif(2.f * turns.x, &sn, &cs);
+    const float tiny = 6.2831853f * (whole.y + turns.y);       // radians that a float of the turns leaves
+    const float sn0 = sn;
+    sn = fmaf(tiny, cs, sn);
+    cs = fmaf(-tiny, sn0, cs);
     table[(threadIdx.x & 7) * pairs + (threadIdx.x >> 3)] = make_float2(cs, sn);
   }
   __syncthreads();
