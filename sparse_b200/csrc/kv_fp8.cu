@@ -17,6 +17,7 @@ namespace sb {
 namespace {
 
 constexpr int kAppendThreads = 128;
+constexpr int kAppendCtas = 10;                  // an SM holds at once, 48 registers a thread
 constexpr int kMaxHead = 256;                    // angles are kept for one CTA's threads
 constexpr int kMaxHalf = kMaxHead / 2;
 
@@ -121,7 +122,7 @@ __device__ __forceinline__ void store_bf16(__nv_bfloat16 *p, const float (&x)[8]
 // positions that 32 bits have): codes differ from the 64-bit rows' as often as those of rows turned
 // by correctly rounded cosines do (148 each of 132 million values, positions up to 30 thousand).
 template <int L, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads)
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas)
 rope_append_fp8_kernel(RowSource q, RowSource k_rot, RowSource k_rest, RowSource v, __nv_bfloat16 *__restrict__ q_out,
                        const int32_t *__restrict__ seq_of_token, const int32_t *__restrict__ pos_of_token, int B,
                        int n_q, int n_kv, int dk, int dv, int rope, int s_max, uint8_t *__restrict__ codes_k,
@@ -311,11 +312,13 @@ int32_t sb_rope_append_fp8(const sb_rope_append_args *args, void *stream) {
   const RopeFreq &freq = rope_freq(theta, rope_dim);
   const int widest = dk > dv ? dk : dv;
   const int lanes = widest <= 64 ? 4 : widest <= 128 ? 8 : 16;
-  // as many CTAs as the SMs hold at once (16 each), so that a CTA has one or two turns: a turn is a
-  // load round trip (1003 tokens of 16 heads of 192/128 with six turns a CTA: 10.9 us)
+  // As many CTAs as the SMs hold at once, so that a CTA has few turns: a turn is a load round trip.
+  // 1003 tokens of 16 heads of 192/128: one CTA a token (six turns) 10.9 us, two 8.2 us; 8 x 512 tokens
+  // of 16 heads of 128, one CTA a token in either case, 16.3 us.  At 61 registers, eight CTAs an SM:
+  // 8.8 and 17.3 us; at 40, twelve: 8.7 and 16.1 us.
   const int sms = sb_device_sm_count() > 0 ? sb_device_sm_count() : 148;
   const int wanted = ((n_q + 2 * n_kv) * lanes + kAppendThreads - 1) / kAppendThreads;
-  const int room = (int)((16ll * sms + T - 1) / T);
+  const int room = (int)(((int64_t)kAppendCtas * sms + T - 1) / T);
   const dim3 grid(T, wanted < room ? wanted : room);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto launch = lanes == 4 ? launch_append<4> : lanes == 8 ? launch_append<8> : launch_append<16>;
