@@ -9,12 +9,24 @@
 // that the keys fill the 16-row side of the warp-level MMA and up to eight query rows its
 // 8-column side.  Keys and values then go from global memory straight into the fragments of
 // the instruction (which positions of a row a lane holds is free, as long as both operands
-// agree), without shared memory: what counts is bytes in flight, and each warp has the 16
-// keys and 16 values of its next step on the way while it works on the present ones.
+// agree), without shared memory: what counts is bytes in flight, and each warp has the keys
+// and values of its next step (16 positions of bf16, 32 quantised: 8 KB) on the way while it
+// works on the present ones.  The tensor core's own rate is no concern here (13 % busy), which
+// is why the warp-level instruction does: an accumulator in tensor memory would need the keys
+// in shared memory first.
 //
-// The work, all 64-position tiles of all sequences and heads in one line, is cut into
-// equal runs, one per CTA, whatever the lengths are; a head that ends in the middle of a run
-// or reaches over several leaves a partial result for each, and attn_join_kernel joins those.
+// The work, all tiles (64 positions of bf16, 128 quantised) of all sequences and heads in one
+// line, is cut into equal runs, one per CTA, whatever the lengths are; a head that ends in the
+// middle of a run or reaches over several leaves a partial result for each, and
+// attn_join_kernel joins those.
+//
+// Measured (repeated in a graph, inputs larger than L2 in turn): 64 sequences of 0 to 16384
+// quantised positions, 32 query and 8 key heads of 128: 171 us, 6.3 TB/s; 8 x 2048, 16 heads: 20 us
+// for 68 MB, of which 2 to 4 us pass before the first keys are there (the lengths come first), CTAs end
+// between 9 and 15 us, and the second kernel takes 3.5 us; one sequence of
+// 1000: 7.2 us, all of it round trips.  A join inside this kernel (marks in memory, the last CTA
+// joins) has one launch less but five round trips to L2 behind one another instead of three:
+// 9.6 us for the sequence of 1000, 23.7 us for 8 x 2048.
 #include <math.h>
 
 #include <type_traits>
@@ -90,8 +102,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 // registers [nt][r] of lanes with lane % 4 == c), U * 16 positions a step.
 //
 // Quantised: the keys' codes become fp16 (exact) and so do the queries, each row scaled by a
-// power of two to a largest value in [1, 2) (bf16's eight bits fit; what falls below 2^-24 of the
-// row's largest is below the rounding of the fp32 sum).  The row's and the key's powers of two
+// power of two to a largest value in [1, 2) (bf16's eight bits fit; a value below 2^-14 of the
+// row's largest is rounded to 2^-25 of that).  The row's and the key's powers of two
 // multiply the fp32 score.  The weight of a value is its probability times the value's power of
 // two, rounded to fp16 (2^-11) relative to a maximum of its own: powers of two that differ by
 // more than fp16's range do not push a small value with all the probability out of it.

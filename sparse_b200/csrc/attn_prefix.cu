@@ -5,8 +5,14 @@
 //
 // Bound by the bytes of the prefix while the rows fit one tile (bf16, heads of 128: 64 KB
 // per 128 positions are 2.8 K clocks of an SM's share of HBM, the two products 1 K, the
-// exponentials 1 K), by the exponentials and the conversion of codes beyond.  One CTA per
-// SM; the positions are cut into as many runs as fill the machine.
+// exponentials 1 K).  Beyond, with codes, by the chain from a block's scores to its product: of
+// the 6.2 K clocks that 128 positions of 256 rows take, the tensor core is busy for 31 % (an M of 128
+// rows takes as long for 64 columns as for 128), the exponentials' unit for 32 %, and an instruction
+// is issued in 47 %.  One CTA per SM; the positions are cut into as many runs as fill the machine.
+//
+// Measured (alone, ncu): 8192 positions of a bf16 cache of 16 heads for 32 sequences 19 us
+// (67 MB, 3.5 TB/s); 16384 quantised positions of 4 heads for 512 rows each 32 us (17 GFLOP, 0.54
+// PF/s; 34 M exponentials).
 //
 // Roles: warp 0 loads tiles of 128 keys and values (TMA: bf16 boxes into the swizzled operand
 // layout; codes as one run of bytes each), warp 1 issues the products, two groups of four
@@ -18,7 +24,7 @@
 // the block before it.  Probabilities go back into TMEM (bf16, over their scores), where the
 // second product takes its left operand from.  Quantised: four warps turn the keys' codes into
 // bf16 operands and four the values', a row per thread, scale applied (exact), so the products
-// are the bf16 ones.
+// are the bf16 ones.  (The fp8 products would round the queries and probabilities to codes.)
 //
 // Probabilities are rounded to bf16 (2^-8), the type of the values that they are multiplied
 // with; scores, their sums and the accumulators are fp32.
