@@ -231,6 +231,21 @@ def _cache_device(cache: QuantizedCache) -> int:
     return device
 
 
+def _head_rows(view: Optional[torch.Tensor], t: int, heads: int, width: int, device: int) -> Tuple[int, int, int]:
+    """Address, token stride and head stride (0: one head for all) of bf16 rows [t, heads or 1, width]."""
+    if view is None:
+        return 0, 0, 0
+    shape = view.shape
+    if len(shape) != 3 or shape[0] != t or shape[1] != heads and shape[1] != 1 or shape[2] != width or (
+            view.dtype is not torch.bfloat16) or view.get_device() != device:
+        raise RuntimeError("rope_append_quantized: needs bf16 [%d, %d or 1, %d] on the cache's device, got %s %s" % (
+            t, heads, width, view.dtype, tuple(shape)))
+    token, head, element = view.stride()
+    if element != 1 and t > 0:
+        raise RuntimeError("rope_append_quantized: the elements of a head must lie side by side")
+    return view.data_ptr(), token, head if shape[1] > 1 else 0
+
+
 def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest: Optional[torch.Tensor],
                           v: torch.Tensor, seq_of_token: torch.Tensor, pos_of_token: torch.Tensor,
                           cache: QuantizedCache, theta: float) -> torch.Tensor:
@@ -250,28 +265,17 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
         raise RuntimeError("rope_append_quantized: q %s and a key of %d rotated and %s other elements for a cache of heads of %d"
                            % (tuple(q.shape), rope, None if k_rest is None else k_rest.shape[-1], dk))
     t, n_q, _ = q.shape
-    ptrs, strides = [], []
-    for view, heads, width in ((q, n_q, dk), (k_rot, n_kv, rope), (k_rest, n_kv, dk - rope), (v, n_kv, dv)):
-        if view is None:
-            ptrs.append(0)
-            strides += (0, 0)
-            continue
-        shape = view.shape
-        if (shape != (t, heads, width) and (shape != (t, 1, width) or view is q)) or view.dtype != torch.bfloat16 or (
-                view.get_device() != device):
-            raise RuntimeError("rope_append_quantized: needs bf16 [%d, %d or 1, %d] on the cache's device, got %s %s" % (
-                t, heads, width, view.dtype, tuple(shape)))
-        token, head, element = view.stride()
-        if element != 1 and t > 0:
-            raise RuntimeError("rope_append_quantized: the elements of a head must lie side by side")
-        ptrs.append(view.data_ptr())
-        strides += (token, head if shape[1] > 1 else 0)
+    q_ptr, q_token, q_head = _head_rows(q, t, n_q, dk, device)
+    rot_ptr, rot_token, rot_head = _head_rows(k_rot, t, n_kv, rope, device)
+    rest_ptr, rest_token, rest_head = _head_rows(k_rest, t, n_kv, dk - rope, device)
+    v_ptr, v_token, v_head = _head_rows(v, t, n_kv, dv, device)
     seq = _index(seq_of_token, t, device, "rope_append_quantized: seq_of_token")
     pos = _index(pos_of_token, t, device, "rope_append_quantized: pos_of_token")
     out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     _call(lib.sb_rope_append_fp8, "sb_rope_append_fp8", device, _lib.ROPE_APPEND.pack(
-        *ptrs, seq, pos, out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
-        cache.v_scale.data_ptr(), *strides, t, b, n_q, n_kv, dk, dv, rope, s_max, theta, 0))
+        q_ptr, rot_ptr, rest_ptr, v_ptr, seq, pos, out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),
+        cache.v.data_ptr(), cache.v_scale.data_ptr(), q_token, q_head, rot_token, rot_head, rest_token, rest_head, v_token,
+        v_head, t, b, n_q, n_kv, dk, dv, rope, s_max, theta, 0))
     return out
 
 
