@@ -23,13 +23,12 @@ class QuantizedCache:
     __slots__ = ("k", "k_scale", "v", "v_scale")
 
     def __init__(self, k: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor, v_scale: torch.Tensor):
-        shape = k.shape
-        rows = shape[:3]
-        if len(shape) != 4 or v.dim() != 4 or v.shape[:3] != rows or k_scale.shape != rows or v_scale.shape != rows:
+        rows, device = k_scale.shape, k.get_device()
+        if len(rows) != 3 or k.shape[:-1] != rows or v.shape[:-1] != rows or v_scale.shape != rows:
             raise RuntimeError("QuantizedCache: codes [B, n_kv, S, d] and scales [B, n_kv, S] do not fit: %s" % (
                 [tuple(t.shape) for t in (k, k_scale, v, v_scale)],))
-        if k.dtype != CODES or v.dtype != CODES or k_scale.dtype != SCALES or v_scale.dtype != SCALES or not (
-                k.get_device() == v.get_device() == k_scale.get_device() == v_scale.get_device()) or not (
+        if k.dtype is not CODES or v.dtype is not CODES or k_scale.dtype is not SCALES or v_scale.dtype is not SCALES or (
+                v.get_device() != device) or k_scale.get_device() != device or v_scale.get_device() != device or not (
                 k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise RuntimeError("QuantizedCache needs contiguous %s codes and %s scales on one device" % (CODES, SCALES))
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale

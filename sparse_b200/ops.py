@@ -219,7 +219,7 @@ _attn_workspace = functools.lru_cache(maxsize=1024)(lib.sb_attn_cached_workspace
 
 
 def _index(t: torch.Tensor, n: int, device: int, what: str) -> int:
-    if t.dtype != torch.int32 or t.get_device() != device or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != device or t.shape != (n,) or not t.is_contiguous():
         raise RuntimeError("%s must be a contiguous int32 tensor of %d elements on CUDA device %d" % (what, n, device))
     return t.data_ptr()
 
@@ -261,17 +261,18 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
     b, n_kv, s_max, dk = cache.k.shape
     dv = cache.v.shape[3]
     rope = 0 if k_rot is None else k_rot.shape[-1]
-    if q.dim() != 3 or q.shape[1] < 1 or q.shape[2] != dk or rope > dk or (k_rest is None) != (rope == dk):
+    shape = q.shape
+    if len(shape) != 3 or shape[1] < 1 or shape[2] != dk or rope > dk or (k_rest is None) != (rope == dk):
         raise RuntimeError("rope_append_quantized: q %s and a key of %d rotated and %s other elements for a cache of heads of %d"
-                           % (tuple(q.shape), rope, None if k_rest is None else k_rest.shape[-1], dk))
-    t, n_q, _ = q.shape
+                           % (tuple(shape), rope, None if k_rest is None else k_rest.shape[-1], dk))
+    t, n_q, _ = shape
     q_ptr, q_token, q_head = _head_rows(q, t, n_q, dk, device)
     rot_ptr, rot_token, rot_head = _head_rows(k_rot, t, n_kv, rope, device)
     rest_ptr, rest_token, rest_head = _head_rows(k_rest, t, n_kv, dk - rope, device)
     v_ptr, v_token, v_head = _head_rows(v, t, n_kv, dv, device)
     seq = _index(seq_of_token, t, device, "rope_append_quantized: seq_of_token")
     pos = _index(pos_of_token, t, device, "rope_append_quantized: pos_of_token")
-    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     _call(lib.sb_rope_append_fp8, "sb_rope_append_fp8", device, _lib.ROPE_APPEND.pack(
         q_ptr, rot_ptr, rest_ptr, v_ptr, seq, pos, out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),
         cache.v.data_ptr(), cache.v_scale.data_ptr(), q_token, q_head, rot_token, rot_head, rest_token, rest_head, v_token,
@@ -302,20 +303,21 @@ def _decode_attention(name: str, call, q: torch.Tensor, cache_ptrs, seq_lens: to
                       device: int) -> torch.Tensor:
     """Checks of the operands that both kinds of cache share, output and workspace, the call."""
     shape = q.shape
-    if len(shape) != 3 or q.dtype != torch.bfloat16 or q.get_device() != device or shape[0] != b or shape[2] != dk or (
+    if len(shape) != 3 or q.dtype is not torch.bfloat16 or q.get_device() != device or shape[0] != b or shape[2] != dk or (
             shape[1] < 1):
         raise RuntimeError("%s: q must be bf16 [%d, n_q, %d] on the cache's device, got %s %s on %s" % (
             name, b, dk, q.dtype, tuple(shape), q.device))
-    n_q = shape[1]
-    seq_stride, head_stride, element = q.stride()
-    if b > 0 and (element != 1 or (n_q > 1 and head_stride != dk) or (b > 1 and seq_stride < n_q * dk)):
-        raise RuntimeError("%s: the heads of a sequence's query must lie side by side, sequences apart" % name)
+    n_q, seq_stride, packed = shape[1], 0, q.is_contiguous()
+    if not packed:
+        seq_stride, head_stride, element = q.stride()
+        if element != 1 or (n_q > 1 and head_stride != dk) or (b > 1 and seq_stride < n_q * dk):
+            raise RuntimeError("%s: the heads of a sequence's query must lie side by side, sequences apart" % name)
     if not 0 <= shared_len <= s_max:
         raise RuntimeError("%s: %d shared positions of a cache of %d" % (name, shared_len, s_max))
     if status is not None and (status.dtype != torch.int32 or status.get_device() != device or status.numel() < 1):
         raise RuntimeError("%s: status must be int32 on the cache's device" % name)
     lens = _index(seq_lens, b, device, name)
-    out = torch.empty_like(q) if dv == dk and q.is_contiguous() else q.new_empty((b, n_q, dv))
+    out = torch.empty_like(q) if dv == dk and packed else q.new_empty((b, n_q, dv))
     ws_bytes = _attn_workspace(b, n_q, n_kv, dk, dv, s_max, shared_len) or 16
     ws = seq_lens.new_empty((ws_bytes + 3) // 4)          # (without a dtype of its own: half a microsecond less)
     _call(call, name, device, _lib.ATTN_CACHED.pack(
