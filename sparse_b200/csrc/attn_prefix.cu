@@ -5,10 +5,11 @@
 //
 // Bound by the bytes of the prefix while the rows fit one tile (bf16, heads of 128: 64 KB
 // per 128 positions are 2.8 K clocks of an SM's share of HBM, the two products 1 K, the
-// exponentials 1 K).  Beyond, with codes, by the chain from a block's scores to its product: of
-// the 6.2 K clocks that 128 positions of 256 rows take, the tensor core is busy for 31 % (an M of 128
-// rows takes as long for 64 columns as for 128), the exponentials' unit for 32 %, and an instruction
-// is issued in 47 %.  One CTA per SM; the positions are cut into as many runs as fill the machine.
+// exponentials 1 K).  For 256 rows by the products: 128 positions take 3.6 K clocks, of which the 48
+// products issued for them take 3.1 K (one of 64 score columns takes as long as one of 128, but
+// leaves room in TMEM for a second score buffer, without which the products wait for the
+// exponentials: 52 instead of 50 us).  With codes and few rows by the conversion, 2.7 K clocks.  One CTA
+// per SM; the positions are cut into as many runs as fill the machine.
 //
 // Measured (alone, ncu): 8192 positions of a bf16 cache of 16 heads for 32 sequences 19 us
 // (67 MB, 3.5 TB/s); 16384 quantised positions of 4 heads for 512 rows each 32 us (17 GFLOP, 0.54
