@@ -24,7 +24,7 @@
 // groups exchange nothing until the end, and a block's products run under the exponentials of
 // the block before it.  Probabilities go back into TMEM (bf16, over their scores), where the
 // second product takes its left operand from.  Quantised: four warps turn the keys' codes into
-// bf16 operands and four the values', a row per thread, scale applied (exact), so the products
+// bf16 operands and four the values', scale applied (exact), so the products
 // are the bf16 ones.  (The fp8 products would round the queries and probabilities to codes.)
 //
 // Probabilities are rounded to bf16 (2^-8), the type of the values that they are multiplied
