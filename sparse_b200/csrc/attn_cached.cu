@@ -125,7 +125,7 @@ struct Stream {
   uint32_t q[NT][DK / 16][2];
   float q_factor[NT][2];
   float m[NT][2], l[NT][2];                            // running maximum (log2 units) and sum
-  float mv[NT][2], r_v[NT][2];                         // quantised: maximum of the weights, 2^(m - mv)
+  float mv[NT][2], r_v[NT][2];                         // quantised: maximum of the weights, 2^(m - mv): up to 2^127, for byte 0
   float acc[MT][NT][4];
 
   // the value columns of a lane: column(e), e < CPL
@@ -357,7 +357,7 @@ struct Stream {
             topv = fmaxf(topv, mv[nt][r]);
             f = exp2_approx(mv[nt][r] - topv);
             mv[nt][r] = topv;
-            r_v[nt][r] = exp2_approx(fminf(top - topv, 126.f));
+            r_v[nt][r] = exp2_approx(fminf(top - topv, 127.f));
           }
 #pragma unroll
           for (int t = 0; t < MT; ++t) { acc[t][nt][r] *= f; acc[t][nt][2 + r] *= f; }
@@ -577,17 +577,18 @@ attn_stream_kernel(const __nv_bfloat16 *__restrict__ q, Cache cache, const int32
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
         const int row = nt * 8 + 2 * c + r;
-        float f = 1.f / l;
-        if constexpr (FP8) f *= exp2f(st.mv[nt][r] - st.m[nt][r]);
-        if (l == 0.f) f = 0.f;
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        // back from weights against mv: the inverse of r_v, which may be 2^-127, as a factor of its own
+        // (with 1 / l in one number it would have few bits left, or none)
+        const float back = FP8 ? exp2f(fmaxf(st.mv[nt][r] - st.m[nt][r], -127.f)) : 1.f;
         if (g == 0) s_lse[warp][row] = l == 0.f ? -INFINITY : st.m[nt][r] + log2f(l);
         // (four columns at a time; the four rows that a warp writes together go to different banks)
         float4 *dst = reinterpret_cast<float4 *>(s_out[warp][row]);
 #pragma unroll
         for (int e = 0; e < DV / 8; e += 4)
           dst[(st.column(g, e) >> 2) ^ ((row >> 1) & 3)] =
-              make_float4(st.acc[e >> 1][nt][r] * f, st.acc[e >> 1][nt][2 + r] * f, st.acc[(e >> 1) + 1][nt][r] * f,
-                          st.acc[(e >> 1) + 1][nt][2 + r] * f);
+              make_float4(st.acc[e >> 1][nt][r] * f * back, st.acc[e >> 1][nt][2 + r] * f * back,
+                          st.acc[(e >> 1) + 1][nt][r] * f * back, st.acc[(e >> 1) + 1][nt][2 + r] * f * back);
       }
     asm volatile("cp.async.wait_all;" ::: "memory");     // the next piece's queries
     __syncthreads();

@@ -1,0 +1,89 @@
+"""GPU: the quantised cache and the attention over it at the ends of what their formats hold, against
+64-bit restatements.  Tolerances as in the tests of the ordinary range: with A = sum_j p_j |v_j| an
+attention output is off by 2^-8 of itself and (2^-7 + 2^-10) A at most."""
+import math
+
+import pytest
+import torch
+
+from sparse_b200 import ops
+from sparse_b200.kv_cache import CODES, SCALES, QuantizedCache
+from test_gpu_kv_cache import BF, DEV, _attend, _bytes, _quantized, _rand, _want
+
+pytestmark = pytest.mark.gpu
+
+# (sequences, query heads, key heads): streamed alone or with the shared positions as rows of the same pass, one row
+# tile of the tensor-core pass, two
+ROWS = [(2, 4, 2), (40, 4, 2), (90, 4, 2)]
+
+
+def _cache(k_codes, k_scales, v_codes, v_scales):
+    return QuantizedCache(k_codes.view(CODES), k_scales.view(SCALES), v_codes.view(CODES), v_scales.view(SCALES))
+
+
+# -- values of the smallest power of two -----------------------------------------------------------
+@pytest.mark.parametrize("b,n_q,n_kv", ROWS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("shared", [0, 70, 150])
+def test_values_of_the_smallest_power_of_two(b, n_q, n_kv, d, shared):
+    """Every row's scale byte is 0.  A code under 2^-6 stands for less than bf16's smallest step and an output may
+    be less than its smallest normal: half a step of 2^-133 for each of the two roundings."""
+    s_max = 170
+    q, k = _rand(b, n_q, d, seed=1), _rand(b, n_kv, s_max, d, seed=2)
+    v = (_rand(b, n_kv, s_max, d, seed=3).float() * 2.0 ** -121).to(BF)
+    assert int(_bytes(_quantized(v)[1]).max()) == 0
+    lens = [s_max - i % 17 for i in range(b)]
+    got, kk, vv = _attend("fp8", q, k, v, lens, shared)
+    want, tol = _want(q, kk, vv, lens, shared, d ** -0.5)
+    assert bool(((got.double() - want).abs() <= tol + 2.0 ** -133).all())
+
+
+def test_a_large_sum_of_weights_over_values_of_the_smallest_power_of_two():
+    """Scores that lag behind the largest ones leave weights of up to e^5.5 in the sum of one pass of a CTA, some
+    2^20: its inverse times 2^-127 is not a number that fp32 has many bits of.  All values are 2^-119, so is the output:
+    2^-11 for a weight in 16 bits, 2^-10 for sums of ten thousand terms in 32, 2^-8 for the output."""
+    d, s = 64, 2 ** 24
+    k = torch.zeros(1, 1, s, d, dtype=torch.uint8, device=DEV)
+    k.view(-1, 2, 128, d)[:, 1, :, 0] = int(torch.tensor(5.5).to(CODES).view(torch.uint8))      # every second tile
+    v = torch.full((1, 1, s, d), int(torch.tensor(256.0).to(CODES).view(torch.uint8)), dtype=torch.uint8, device=DEV)
+    one, least = (torch.full((1, 1, s), e, dtype=torch.uint8, device=DEV) for e in (127, 0))
+    q = torch.zeros(1, 1, d, dtype=BF, device=DEV)
+    q[..., 0] = 1.0
+    got = ops.attn_decode_quantized(q, _cache(k, one, v, least), torch.tensor([s], dtype=torch.int32, device=DEV), scale=1.0)
+    assert float((got.double() * 2.0 ** 119 - 1.0).abs().max()) <= 2.0 ** -8 + 2.0 ** -10 + 2.0 ** -11
+
+
+@pytest.mark.parametrize("b,n_q,n_kv", ROWS)
+@pytest.mark.parametrize("where", ["keys", "values"])
+def test_rows_of_every_power_of_two_below_the_largest(b, n_q, n_kv, where):
+    """One position counts at a time; its key, or its value, has one of the sizes 2^-126 .. 2^99 (bytes 0 to 218), on
+    both sides of the border between shared and own positions."""
+    d, shared, s_max = 64, 226, 300
+    sizes = torch.exp2(torch.arange(-126, 100, device=DEV).double())
+    k = torch.zeros(b, n_kv, s_max, d, dtype=BF, device=DEV)
+    v = _rand(b, n_kv, s_max, d, seed=4)
+    if where == "values":
+        v[:, :, :226] = (v[:, :, :226].double() * sizes[None, None, :, None]).to(BF)
+    q = torch.zeros(b, n_q, d, dtype=BF, device=DEV)
+    lens = [s_max - i % 3 for i in range(b)]
+    for at in (0, 1, 2, 60, 63, 64, 119, 126, 127, 128, 180, 190, 224, 225):
+        k.zero_()
+        size = float(sizes[at])
+        for split in (shared, 0):
+            src = torch.zeros(b, dtype=torch.long, device=DEV) if split else torch.arange(b, device=DEV)
+            if where == "keys":
+                # the query's largest value is 2^6 over the key's size, as far as bf16 goes: a score of 2^6
+                k[src, :, at, 5] = size
+                q[..., 5] = min(64.0 / size, 2.0 ** 127)
+                score = float(q[0, 0, 5]) * size
+            else:
+                k[src, :, at, 5], q[..., 5], score = 300.0, 1.0, 300.0
+            got, _, vv = _attend("fp8", q, k, v, lens, split, scale=1.0)
+            if score < 64.0:
+                # (sizes under 2^-121: the query cannot make up for them)
+                mean, tol = _want(q, k.double(), vv, lens, split, 1.0)
+                assert bool(((got.double() - mean).abs() <= tol).all()), (at, split)
+                continue
+            want = vv[src, :, at].repeat_interleave(n_q // n_kv, dim=1)
+            # the others weigh exp(-64) each and are at most 2^102 times as large where values differ, exp(-300) then
+            assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -133 if where == "values" else 1e-20)).all()), (at, split)
