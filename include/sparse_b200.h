@@ -632,8 +632,8 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  * binding fills one block of bytes faster than it converts twenty arguments.
  *
  * sb_rope_append_fp8  rotates the first rope_dim elements of every q and k head (pairs
- *                  (i, i + rope_dim/2), angle pos * theta^(-2i/rope_dim)), stores q to
- *                  q_out [T,n_q,dk] bf16 (q itself is not written) and quantises k and v
+ *                  (i, i + rope_dim/2), angle pos * base^(-2i/rope_dim), base = theta +
+ *                  theta_rest), stores q to q_out [T,n_q,dk] bf16 (q itself is not written) and quantises k and v
  *                  into row (seq_of_token[t], pos_of_token[t]).  Angles, products and the
  *                  scaled row are fp32, a value is rounded once; cosines and sines are
  *                  those of the 64-bit formula within 2^-23, from position 2^24 on 2^-14.  A key
@@ -667,8 +667,7 @@ typedef struct sb_rope_append {
   void *q_out, *codes_k, *scale_k, *codes_v, *scale_v;
   int64_t stride[8];                  /* between tokens and between heads of q, k_rot, k_rest, v */
   int32_t T, B, n_q, n_kv, dk, dv, rope_dim, s_max;
-  float theta;
-  int32_t reserved_;
+  float theta, theta_rest;            /* the base is their sum: its fp32 rounding and what that leaves (or 0) */
 } sb_rope_append_args;
 
 typedef struct sb_cache_read {

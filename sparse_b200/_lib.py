@@ -39,10 +39,10 @@ class MoeLayer(C.Structure):
 
 
 # The structs of the cache calls as packed bytes (native alignment), fields in the header's order:
-# sb_rope_append_args    11 pointers, 8 strides, T B n_q n_kv dk dv rope_dim s_max, theta, reserved
+# sb_rope_append_args    11 pointers, 8 strides, T B n_q n_kv dk dv rope_dim s_max, theta, theta_rest
 # sb_cache_read_args     6 pointers, B n_kv dk dv s_max begin count shared_len
 # sb_attn_cached_args    9 pointers, q_stride, ws_bytes, B n_q n_kv dk dv s_max shared_len, scale
-ROPE_APPEND = struct.Struct("@11P8q8ifi")
+ROPE_APPEND = struct.Struct("@11P8q8i2f")
 CACHE_READ = struct.Struct("@6P8i")
 ATTN_CACHED = struct.Struct("@9PqQ7if")
 

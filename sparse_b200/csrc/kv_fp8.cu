@@ -263,12 +263,12 @@ cache_read_fp8_kernel(const uint8_t *__restrict__ codes_k, const uint8_t *__rest
 }
 
 // The frequencies of a model are the same in every call: a thread keeps the last table.
-const RopeFreq &rope_freq(float theta, int rope_dim) {
+const RopeFreq &rope_freq(double theta, int rope_dim) {
   static thread_local RopeFreq kept;
-  static thread_local float kept_theta = 0.f;
+  static thread_local double kept_theta = 0.0;
   static thread_local int kept_dim = -1;
   if (kept_theta != theta || kept_dim != rope_dim) {
-    const double log_theta = log((double)theta);
+    const double log_theta = log(theta);
     for (int j = 0; j < rope_dim / 2; ++j) {
       const double turns = exp(-2.0 * j / rope_dim * log_theta) / (2.0 * M_PI);
       kept.turns[j].x = (float)turns;
@@ -293,9 +293,9 @@ int32_t sb_rope_append_fp8(const sb_rope_append_args *args, void *stream) {
   if (!args) return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: null pointer");
   const sb_rope_append_args &a = *args;
   const int T = a.T, B = a.B, n_q = a.n_q, n_kv = a.n_kv, dk = a.dk, dv = a.dv, rope_dim = a.rope_dim, s_max = a.s_max;
-  const float theta = a.theta;
+  const double theta = (double)a.theta + (double)a.theta_rest;
   if (T < 0 || B < 1 || n_q < 1 || n_kv < 1 || n_q > 65536 || n_kv > 65536 || s_max < 1 || !head_ok(dk) || !head_ok(dv) ||
-      rope_dim < 0 || rope_dim > dk || rope_dim % 16 != 0 || !(theta > 0.f) || !isfinite(theta))
+      rope_dim < 0 || rope_dim > dk || rope_dim % 16 != 0 || !(theta > 0.0) || !isfinite(theta))
     return fail(SB_E_INVALID_ARG, "sb_rope_append_fp8: bad shape (T=%d B=%d heads %d/%d widths %d/%d rope %d s_max=%d)", T,
                 B, n_q, n_kv, dk, dv, rope_dim, s_max);
   if (T == 0) return SB_OK;

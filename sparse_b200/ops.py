@@ -6,6 +6,7 @@ of the tensors' device and never synchronise.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 from typing import Optional, Tuple
 
@@ -218,6 +219,13 @@ def _call(fn, what: str, device: int, args: bytes) -> None:
 _attn_workspace = functools.lru_cache(maxsize=1024)(lib.sb_attn_cached_workspace_bytes)
 
 
+@functools.lru_cache(maxsize=64)
+def _two_floats(x: float) -> Tuple[float, float]:
+    """x as its fp32 rounding and what that leaves."""
+    hi = ctypes.c_float(x).value
+    return hi, x - hi
+
+
 def _index(t: torch.Tensor, n: int, device: int, what: str) -> int:
     if t.dtype is not torch.int32 or t.get_device() != device or t.shape != (n,) or not t.is_contiguous():
         raise RuntimeError("%s must be a contiguous int32 tensor of %d elements on CUDA device %d" % (what, n, device))
@@ -256,7 +264,8 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
     (one head: shared by all), the rest k_rest [T, n_kv or 1, dk - r] (None where nothing is
     left, as k_rot where nothing is rotated); v [T, n_kv or 1, dv].  All are bf16 views with any
     token and head strides.  Token t goes to row (seq_of_token[t], pos_of_token[t]), int32; one
-    outside the cache is not stored.  Two tokens of a call must not name the same row."""
+    outside the cache is not stored.  Two tokens of a call must not name the same row.  `theta`,
+    the base of the angles, is taken in 64 bits (to 48 of its bits)."""
     device = _cache_device(cache)
     b, n_kv, s_max, dk = cache.k.shape
     dv = cache.v.shape[3]
@@ -276,7 +285,7 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
     _call(lib.sb_rope_append_fp8, "sb_rope_append_fp8", device, _lib.ROPE_APPEND.pack(
         q_ptr, rot_ptr, rest_ptr, v_ptr, seq, pos, out.data_ptr(), cache.k.data_ptr(), cache.k_scale.data_ptr(),
         cache.v.data_ptr(), cache.v_scale.data_ptr(), q_token, q_head, rot_token, rot_head, rest_token, rest_head, v_token,
-        v_head, t, b, n_q, n_kv, dk, dv, rope, s_max, theta, 0))
+        v_head, t, b, n_q, n_kv, dk, dv, rope, s_max, *_two_floats(float(theta))))
     return out
 
 

@@ -87,3 +87,32 @@ def test_rows_of_every_power_of_two_below_the_largest(b, n_q, n_kv, where):
             want = vv[src, :, at].repeat_interleave(n_q // n_kv, dim=1)
             # the others weigh exp(-64) each and are at most 2^102 times as large where values differ, exp(-300) then
             assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -133 if where == "values" else 1e-20)).all()), (at, split)
+
+
+# -- bases that fp32 does not have -----------------------------------------------------------------
+@pytest.mark.parametrize("theta", [1e4 * 8 ** (128 / 126), 1e4 / 3, 12345.678, 1e6 * 4 ** (64 / 62), 1e4])
+@pytest.mark.parametrize("first", [0, 131072 - 2000, 2 ** 24 - 2001])
+def test_append_angles_of_a_base_that_fp32_does_not_have(theta, first):
+    """Pairs (1, 0): the outputs are the cosines and sines themselves, 2^-21 off at most, then rounded to bf16."""
+    t, d = 2000, 128
+    q = torch.zeros(t, 1, d, dtype=BF, device=DEV)
+    q[..., :d // 2] = 1.0
+    cache = QuantizedCache.zeros(1, 1, 1, d, d, DEV)
+    pos = torch.arange(first, first + t, dtype=torch.int32, device=DEV)
+    out = ops.rope_append_quantized(q, q, None, q, torch.full_like(pos, -1), pos, cache, theta)
+    ang = pos.double()[:, None] * theta ** (-torch.arange(d // 2, device=DEV).double() / (d // 2))
+    want = torch.cat([ang.cos(), ang.sin()], -1)
+    assert bool(((out[:, 0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -21).all())
+
+
+def test_bases_in_turn():
+    """Each call has the angles of its own base, whichever was there before it."""
+    q, c = _rand(3, 2, 64, seed=1), QuantizedCache.zeros(1, 1, 2, 64, 64, DEV)
+    pos = torch.tensor([5, 1000, 99999], dtype=torch.int32, device=DEV)
+    bases = [1e4, 1e4 * (1 + 2.0 ** -30), 5e5]
+    outs = [ops.rope_append_quantized(q, q, None, q, pos * 0 - 1, pos, c, t) for t in bases]
+    for t, want in list(zip(bases, outs))[::-1]:
+        assert torch.equal(ops.rope_append_quantized(q, q, None, q, pos * 0 - 1, pos, c, t), want)
+    for t in (0.0, -1.0, math.nan, math.inf, 1e39):
+        with pytest.raises(RuntimeError):
+            ops.rope_append_quantized(q, q, None, q, pos * 0 - 1, pos, c, t)
