@@ -390,11 +390,14 @@ class ShapedMoeModel:
         return self.cur_ids
 
     def check_status(self) -> None:
+        attn = int(self.attn_status.item())
+        if attn != 0:
+            self.attn_status.zero_()                     # (a later request's steps say for themselves)
         for ly in self.layers:
             if ly.block is not None:
                 ly.block.check_status()
-        if int(self.attn_status.item()) != 0:
-            raise RuntimeError("decode attention: a bounded wait gave up (status %d)" % int(self.attn_status.item()))
+        if attn != 0:
+            raise RuntimeError("decode attention: a bounded wait gave up (status %d)" % attn)
 
 
 class RunningStats:
