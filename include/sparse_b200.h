@@ -657,8 +657,8 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  *                  the division by the weights' sum: values beyond 2^100 may overflow.  ws:
  *                  sb_attn_cached_workspace_bytes(), 16-byte aligned, not shared by calls
  *                  that may overlap on the GPU.  status: device int32 (may be NULL), set
- *                  non-zero if a bounded wait gave up.  (dk,dv) = (128,128), (192,128),
- *                  (64,64).
+ *                  non-zero if a bounded wait gave up; the outputs that depend on what was waited
+ *                  for are then NaN.  (dk,dv) = (128,128), (192,128), (64,64).
  * sb_attn_decode_shared  the same over a bf16 cache, k [B,s_max,n_kv,dk] and v [B,s_max,n_kv,dv].
  */
 typedef struct sb_rope_append {

@@ -31,7 +31,7 @@
 // with; scores, their sums and the accumulators are fp32.
 //
 // All mbarrier waits are bounded; when one runs out the CTA raises its abort flag, reports
-// through `status`, waits for its copies and frees its TMEM.
+// through `status`, makes its partial result NaN, waits for its copies and frees its TMEM.
 #include <math.h>
 
 #include <atomic>
@@ -591,6 +591,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   __syncthreads();
   if (*abort_flag) {
     if (threadIdx.x == 0 && status) atomicExch(status, 1);
+    // what this CTA should have found is not known: NaN, for every output that is joined from it
+    const size_t slot_row = (((size_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * s.pre_rows;
+    for (int i = threadIdx.x; i < rows; i += L::kThreads) part_lse[slot_row + i] = __uint_as_float(0x7fc00000u);
     const unsigned long long t0 = gtime_ns();
     while (gtime_ns() - t0 < 2000000ull) __nanosleep(1000);       // copies in flight
     __syncthreads();

@@ -342,7 +342,8 @@ def attn_decode_quantized(q: torch.Tensor, cache: QuantizedCache, seq_lens: torc
 
     n_q is a multiple of the cache's heads.  `shared_len`: as many first positions are the
     same for the whole batch and stand in sequence 0's rows; they are read once.  `scale`
-    (at least 0) defaults to dk ** -0.5; `status` as in `grouped_swiglu`."""
+    (at least 0) defaults to dk ** -0.5; `status` (int32 on the device) becomes non-zero if a bounded
+    wait gave up, and the outputs that depend on it NaN."""
     b, n_kv, s_max, dk = cache.k.shape
     ptrs = (cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr())
     return _decode_attention("attn_decode_quantized", lib.sb_attn_decode_fp8, q, ptrs, seq_lens, b, n_kv, dk, cache.v.shape[3],
