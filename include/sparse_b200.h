@@ -626,15 +626,16 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  * for code * 2^(scale - 127), scale byte 255 for NaN throughout; the writer takes the least
  * power of two, 2^-127 or more, by which the row's largest magnitude is at most 448 (codes
  * then stop at 240 where 256 would stand for 2^128), and byte 255 with zero codes for a row that
- * holds an infinity or a NaN.  The codes 0x7f and 0xff, e4m3's own NaN, have no place in this
- * format (the scale byte says it for the row): the writer makes none, and what attention makes of
- * them is not defined.  All codes and bf16 caches must be 16-byte aligned.  A call's operands come as a struct (host memory, not kept); these calls are a decode step's, and a
+ * holds an infinity or a NaN.  The writer makes no codes 0x7f and 0xff, e4m3's own NaN (the scale byte
+ * says it for the row); in a cache that was filled in some other way they are NaN to every call that
+ * reads them.  All codes and bf16 caches must be 16-byte aligned.  A call's operands come as a struct (host memory, not kept); these calls are a decode step's, and a
  * binding fills one block of bytes faster than it converts twenty arguments.
  *
  * sb_rope_append_fp8  rotates the first rope_dim elements of every q and k head (pairs
- *                  (i, i + rope_dim/2), angle pos * base^(-2i/rope_dim), base = theta +
- *                  theta_rest), stores q to q_out [T,n_q,dk] bf16 (q itself is not written) and quantises k and v
- *                  into row (seq_of_token[t], pos_of_token[t]).  Angles, products and the
+ *                  (i, i + rope_dim/2), angle pos * base^(-2i/rope_dim),
+ *                  base = theta + theta_rest), stores q to q_out [T,n_q,dk] bf16 (q itself is not
+ *                  written) and quantises k and v into row (seq_of_token[t], pos_of_token[t]).
+ *                  Angles, products and the
  *                  scaled row are fp32, a value is rounded once; cosines and sines are
  *                  those of the 64-bit formula within 2^-23, from position 2^24 on 2^-14.  A key
  *                  head's first rope_dim elements come from k_rot and the others from k_rest

@@ -142,14 +142,18 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// sixteen codes (one 16-byte chunk) -> two chunks
-__device__ __forceinline__ void convert16(const uint4 &c, RowScale scale, bool twice, uint4 &lo, uint4 &hi) {
+// sixteen codes (one 16-byte chunk) -> two chunks; `top`: the largest magnitudes so far, of both halves of a pair
+constexpr uint32_t kNanSize = 0x07f0u;                 // e4m3's own NaN, 0x7f or 0xff: it becomes 480 here
+__device__ __forceinline__ void convert16(const uint4 &c, RowScale scale, bool twice, uint4 &lo, uint4 &hi, uint32_t &top) {
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
   uint32_t o[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t t = __byte_perm(w[i >> 1], 0, i & 1 ? 0x3424 : 0x1404);       // two codes, each in the high byte of a half
-    o[i] = mul_bf16x2(((t >> 4) & 0x07f007f0u) | (t & 0x80008000u), scale.first);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t0 = __byte_perm(w[i], 0, 0x1404), t1 = __byte_perm(w[i], 0, 0x3424);     // two codes, each in the high byte of a half
+    const uint32_t size0 = (t0 >> 4) & 0x07f007f0u, size1 = (t1 >> 4) & 0x07f007f0u;
+    top = __vimax3_u16x2(top, size0, size1);
+    o[2 * i] = mul_bf16x2(size0 | (t0 & 0x80008000u), scale.first);
+    o[2 * i + 1] = mul_bf16x2(size1 | (t1 & 0x80008000u), scale.first);
   }
   if (twice) {
 #pragma unroll
@@ -167,8 +171,9 @@ __device__ __forceinline__ void convert16(const uint4 &c, RowScale scale, bool t
 // back right behind the loads, it was refilled under them).  The loop is short on purpose: one code for
 // both sides and all scales takes 0.93 of the time of one for each (16384 positions, 24 rows a head:
 // 44.6 and 48.0 us), unrolled over both halves with the next one's codes fetched ahead 62 us.
+// Returns whether one of the thread's codes is e4m3's own NaN.
 template <int D, int NS, int RAW>
-__device__ __forceinline__ void convert_tiles(const unsigned char *raw, uint32_t raw_stage, unsigned char *op, uint32_t raw_full,
+__device__ __forceinline__ bool convert_tiles(const unsigned char *raw, uint32_t raw_stage, unsigned char *op, uint32_t raw_full,
                                               uint32_t raw_empty, uint32_t full, uint32_t empty, const uint8_t *scales, int first,
                                               int end, int n, volatile int *abort_flag) {
   constexpr int kChunks = D / 16, kMine = kChunks / 2;
@@ -191,14 +196,16 @@ __device__ __forceinline__ void convert_tiles(const unsigned char *raw, uint32_t
   const auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
   uint4 c[kMine];
   uint32_t byte = scale_at(0);
-  if (!wait(raw_full, 0)) return;
+  uint32_t top = 0;
+  const auto nan_seen = [&] { return (top & 0xffffu) == kNanSize || (top >> 16) == kNanSize; };
+  if (!wait(raw_full, 0)) return false;
   fetch(0, c);
 #pragma unroll 1
   for (int i = 0; i < 2 * n; ++i) {
     const int st = (i >> 1) % NS;
     const bool more = i + 1 < 2 * n;
     const uint32_t next_byte = scale_at(i + 1);
-    if (!(i & 1) && !wait(empty + 8 * st, (((i >> 1) / NS) & 1) ^ 1u)) return;
+    if (!(i & 1) && !wait(empty + 8 * st, (((i >> 1) / NS) & 1) ^ 1u)) return nan_seen();
     const bool in = key_of(i) < end;
     const RowScale scale = in ? row_scale(byte) : RowScale{0u, 0u};
     const bool twice = __any_sync(0xffffffffu, in && scale.second != 0x3f803f80u);
@@ -206,7 +213,7 @@ __device__ __forceinline__ void convert_tiles(const unsigned char *raw, uint32_t
 #pragma unroll
     for (int x = 0; x < kMine; ++x) {
       uint4 lo, hi;
-      convert16(c[x], scale, twice, lo, hi);
+      convert16(c[x], scale, twice, lo, hi, top);
       *reinterpret_cast<uint4 *>(dst + to[x]) = lo;
       *reinterpret_cast<uint4 *>(dst + (to[x] ^ 16u)) = hi;
     }
@@ -217,11 +224,33 @@ __device__ __forceinline__ void convert_tiles(const unsigned char *raw, uint32_t
       if (i & 1) mbar_arrive(full + 8 * st);
     }
     if (more) {
-      if (!wait(raw_full + 8 * ((i + 1) % RAW), ((i + 1) / RAW) & 1)) return;
+      if (!wait(raw_full + 8 * ((i + 1) % RAW), ((i + 1) / RAW) & 1)) return nan_seen();
       fetch(i + 1, c);
     }
     byte = next_byte;
   }
+  return nan_seen();
+}
+
+// A cache that somebody filled by a cast of their own may hold e4m3's NaN, and the conversion makes 480
+// of it.  What such a code does is the same for every query row: with one in a key all scores are NaN, with one
+// in a value its column.  So the conversion only notes that there was one, and at the end all threads of the CTA
+// look through its run of codes once more and put NaN where it belongs in the partial result: cold, out of
+// line.  (16384 positions, 24 and 512 rows a head: without the note 43.8 and 48.1 us, with it 44.8 and 48.6, with
+// NaN put into the operands as they are made 45.5 and 48.6, with the note made by the two warps without a
+// role 44.5 and 49.1.)
+__device__ __noinline__ void mark_nan_codes(const uint8_t *k, int64_t k_bytes, const uint8_t *v, int64_t v_bytes, int dv, int rows,
+                                            float *part, float *lse, uint32_t *found) {
+  const float nan = __uint_as_float(0x7fc00000u);
+  for (int64_t i = threadIdx.x; i < k_bytes; i += blockDim.x)
+    if ((k[i] & 0x7f) == 0x7f) atomicOr(found, 1u);
+  for (int64_t i = threadIdx.x; i < v_bytes; i += blockDim.x)
+    if ((v[i] & 0x7f) == 0x7f) atomicOr(found + 1 + i % dv / 32, 1u << (i % 32));
+  __syncthreads();
+  if (found[0] != 0)
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) lse[i] = nan;
+  for (int i = threadIdx.x; i < rows * dv; i += blockDim.x)
+    if ((found[1 + i % dv / 32] >> (i % 32)) & 1) part[i] = nan;
 }
 
 // two fp32 operations at once
@@ -321,6 +350,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const uint32_t rk_full = pv_done + 8 * 4, rv_full = rk_full + 8 * 4, r_empty = rv_full + 8 * 4;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(aligned_base + L::kBytes + 8 * (10 * 4));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  uint32_t *nan_found = tmem_slot + 2;                  // a NaN among the codes: at all; among the keys', in a column (four words)
 
   // (the warp's number and the TMEM address as values that are the same for the whole warp: the
   // instructions that issue products and copies take uniform registers)
@@ -343,6 +373,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       mbar_init(rk_full + 8 * i, 1); mbar_init(rv_full + 8 * i, 1); mbar_init(r_empty + 8 * i, 8);
     }
     *abort_flag = 0;
+    for (int i = 0; i < 6; ++i) nan_found[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -580,10 +611,12 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     unsigned char *op = aligned_base + ((keys_side ? k_smem : v_smem) - base);
     const uint8_t *scales = (keys_side ? cache.ks : cache.vs) + row0;
     const uint32_t raw_full = keys_side ? rk_full : rv_full, full = keys_side ? k_full : v_full, empty = keys_side ? k_empty : v_empty;
+    bool nan;
     if (DK == DV || keys_side)
-      convert_tiles<DK, NS, L::kRaw>(raw, L::kRawK + L::kRawV, op, raw_full, r_empty, full, empty, scales, first, end, n, abort_flag);
+      nan = convert_tiles<DK, NS, L::kRaw>(raw, L::kRawK + L::kRawV, op, raw_full, r_empty, full, empty, scales, first, end, n, abort_flag);
     else
-      convert_tiles<DV, NS, L::kRaw>(raw, L::kRawK + L::kRawV, op, raw_full, r_empty, full, empty, scales, first, end, n, abort_flag);
+      nan = convert_tiles<DV, NS, L::kRaw>(raw, L::kRawK + L::kRawV, op, raw_full, r_empty, full, empty, scales, first, end, n, abort_flag);
+    if (nan) atomicOr(nan_found, 1u);
   }
 
   __syncwarp();
@@ -597,6 +630,12 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const unsigned long long t0 = gtime_ns();
     while (gtime_ns() - t0 < 2000000ull) __nanosleep(1000);       // copies in flight
     __syncthreads();
+  }
+  if (FP8 && nan_found[0] != 0) {
+    const int64_t slot_row = (((int64_t)hk * gridDim.y + rt) * gridDim.x + blockIdx.x) * s.pre_rows;
+    const int64_t row0 = (int64_t)hk * s.s_max + (int64_t)tile0 * kKeys, keys = min((int64_t)n * kKeys, s.shared_len - (int64_t)tile0 * kKeys);
+    mark_nan_codes(static_cast<const uint8_t *>(cache.k) + row0 * DK, keys * DK, static_cast<const uint8_t *>(cache.v) + row0 * DV,
+                   keys * DV, DV, rows, part + slot_row * DV, part_lse + slot_row, nan_found + 1);
   }
   if (warp == 1) {
     tc_fence_after();

@@ -6,10 +6,10 @@ context of a given length takes of HBM.  Written by `ops.rope_append_quantized`,
 
 The row of a (sequence, head, position) is e4m3 codes and one power of two, the least
 one (2^-127 or more) by which the row's largest magnitude is at most 448.  A row with an
-infinity or a NaN has scale byte 255; e4m3's NaN codes 0x7f and 0xff do not occur (who fills a
-cache by a cast of their own has to see to that).  Heads come
-before positions, unlike in the bf16 cache: a head's codes are then one run of bytes, and
-so are its scales, of which a position has only one byte per head.
+infinity or a NaN has scale byte 255 and no e4m3 NaN among its codes; in a cache that somebody
+filled by a cast of their own the codes 0x7f and 0xff read as NaN.  Heads come before positions,
+unlike in the bf16 cache: a head's codes are then one run of bytes, and so are its scales, of which
+a position has only one byte per head.
 """
 from __future__ import annotations
 

@@ -116,3 +116,38 @@ def test_bases_in_turn():
     for t in (0.0, -1.0, math.nan, math.inf, 1e39):
         with pytest.raises(RuntimeError):
             ops.rope_append_quantized(q, q, None, q, pos * 0 - 1, pos, c, t)
+
+
+# -- e4m3's own NaN ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("b,n_q,n_kv", ROWS)
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (192, 128)])
+@pytest.mark.parametrize("code", [0x7f, 0xff])
+def test_a_code_that_is_nan_reads_as_nan_everywhere(b, n_q, n_kv, dk, dv, code):
+    """A cache that somebody filled by a cast of their own: read back, streamed and on the tensor cores the code is
+    NaN, in its column where a value holds it, in the whole row where a key does."""
+    s_max, shared = 200, 140
+    k, v = _rand(b, n_kv, s_max, dk, seed=1), _rand(b, n_kv, s_max, dv, seed=2)
+    q = _rand(b, n_q, dk, seed=3)
+    lens = torch.full((b,), s_max - 1, dtype=torch.int32, device=DEV)
+    lens[-1] = shared - 3                                  # ends before the later ones
+    clean = ops.attn_decode_quantized(q, QuantizedCache(*_quantized(k), *_quantized(v)), lens, shared)
+    group = n_q // n_kv
+    for row, at, width in ((0, 0, dv), (0, 63, dv), (0, 64, dv), (0, 127, dv), (0, shared - 1, dv), (0, 7, dk), (0, shared - 2, dk),
+                           (0, s_max - 1, dv), (1, 5, dv), (1, 150, dv), (1, 160, dk), (1, 6, dk)):
+        for col in (0, 15, 16, width - 1):
+            c = QuantizedCache(*_quantized(k), *_quantized(v))
+            key = width == dk and at in (7, shared - 2, 160, 6)
+            _bytes(c.k if key else c.v)[row, 1, at, col] = code
+            want = clean.double().clone()
+            # a shared position is sequence 0's and every sequence's that reaches it, another one its own's
+            hit = (lens > at) & (torch.arange(b, device=DEV) == row if at >= shared else torch.tensor(row == 0, device=DEV))
+            rows = hit.nonzero()[:, 0][:, None], torch.arange(group, 2 * group, device=DEV)[None]
+            if key:
+                want[rows] = math.nan
+            else:
+                want[..., col][rows] = math.nan
+            got = ops.attn_decode_quantized(q, c, lens, shared)
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), (row, at, col, key)
+            assert torch.equal(got[~torch.isnan(got)], clean[~torch.isnan(got)]), (row, at, col, key)
+    read, _ = ops.cache_read(c, 6, 1)
+    assert bool(torch.isnan(read[1, 1, 0, col])) and int(torch.isnan(read).sum()) == 1
