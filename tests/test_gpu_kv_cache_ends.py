@@ -151,3 +151,27 @@ def test_a_code_that_is_nan_reads_as_nan_everywhere(b, n_q, n_kv, dk, dv, code):
             assert torch.equal(got[~torch.isnan(got)], clean[~torch.isnan(got)]), (row, at, col, key)
     read, _ = ops.cache_read(c, 6, 1)
     assert bool(torch.isnan(read[1, 1, 0, col])) and int(torch.isnan(read).sum()) == 1
+
+
+# -- scores of -inf, sizes up to the largest -----------------------------------------------------------
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("b,n_q,n_kv", ROWS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("shared", [1, 130, 200])
+@pytest.mark.parametrize("own", ["-inf", "zero", "none"])
+def test_shared_scores_of_minus_infinity_weigh_nothing(kind, b, n_q, n_kv, d, shared, own):
+    """Shared positions whose every score is -inf: the own positions alone count; where there are none, or theirs are
+    -inf too, zeros."""
+    s_max = shared + 9
+    q = torch.full((b, n_q, d), -3.0e38, dtype=BF, device=DEV)
+    k, v = torch.full((b, n_kv, s_max, d), 3.0e38, dtype=BF, device=DEV), _rand(b, n_kv, s_max, d)
+    if own == "zero":
+        k[:, :, shared:] = 0.0
+    lens = [shared if own == "none" else s_max - i % 9 for i in range(b)]
+    got, _, vv = _attend(kind, q, k, v, lens, shared)
+    if own != "zero":
+        assert float(got.float().abs().max()) == 0.0
+        return
+    # scores of zero: the mean of the own positions
+    want, tol = _want(torch.zeros_like(q), torch.zeros_like(vv[:, :, shared:]), vv[:, :, shared:], [n - shared for n in lens], 0, 1.0)
+    assert bool(((got.double() - want).abs() <= tol).all())
