@@ -106,7 +106,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 // row's largest is rounded to 2^-25 of that).  The row's and the key's powers of two
 // multiply the fp32 score.  The weight of a value is its probability times the value's power of
 // two, rounded to fp16 (2^-11) relative to a maximum of its own: powers of two that differ by
-// more than fp16's range do not push a small value with all the probability out of it.
+// more than fp16's range do not push a small value with all the probability out of it.  The sum is
+// of the unrounded probabilities: 2^-11 is a quarter of what the output's own rounding may leave.
 // bf16: probabilities are rounded to bf16 (2^-8, the type of the values they are multiplied
 // with), and their sum is taken over the rounded ones.
 template <int DK, int DV, bool FP8, int NT>

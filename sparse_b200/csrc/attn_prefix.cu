@@ -28,7 +28,9 @@
 // are the bf16 ones.  (The fp8 products would round the queries and probabilities to codes.)
 //
 // Probabilities are rounded to bf16 (2^-8), the type of the values that they are multiplied
-// with; scores, their sums and the accumulators are fp32.
+// with, and their sum is taken over the rounded ones; scores, sums and accumulators are fp32.  Against
+// probabilities in fp32 (attn_decode_kernel) that shows where values average out: 8192 positions of
+// independent values 2.3e-3 from 64 bits in norm, of which the rounding of the output makes 1.65e-3.
 //
 // All mbarrier waits are bounded; when one runs out the CTA raises its abort flag, reports
 // through `status`, makes its partial result NaN, waits for its copies and frees its TMEM.
@@ -298,7 +300,9 @@ __device__ __forceinline__ float row_top(uint32_t st_at, int keys) {
 }
 
 // A row's exponentials against the maximum `m` into TMEM, bf16 pairs over the scores (a pair is
-// stored behind the scores it replaces); returns their sum.
+// stored behind the scores it replaces); returns the sum of the pairs as stored, so that the weights
+// of a row add up to one (0 to 0.9 % of a call's time; summed before they are rounded, equal values of 1
+// came out as 0.996 where most probabilities round the same way).
 template <bool TAIL>
 __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float scale_log2, float m) {
   unsigned long long sum[2] = {0ull, 0ull};
@@ -316,8 +320,8 @@ __device__ __forceinline__ float exponentials(uint32_t st_at, int keys, float sc
         a = x + 2 * e < keys ? a : 0.f;
         b = x + 2 * e + 1 < keys ? b : 0.f;
       }
-      sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(a, b));
       p[e] = pack_bf16x2(a, b);
+      sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(bf16_lo(p[e]), bf16_hi(p[e])));
     }
     tc_st16(st_at + x / 2, p);
   }

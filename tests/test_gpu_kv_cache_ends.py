@@ -175,3 +175,23 @@ def test_shared_scores_of_minus_infinity_weigh_nothing(kind, b, n_q, n_kv, d, sh
     # scores of zero: the mean of the own positions
     want, tol = _want(torch.zeros_like(q), torch.zeros_like(vv[:, :, shared:]), vv[:, :, shared:], [n - shared for n in lens], 0, 1.0)
     assert bool(((got.double() - want).abs() <= tol).all())
+
+
+# -- weights sum to one -------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("b,n_q,n_kv", ROWS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_mean_of_equal_values_is_their_value(kind, b, n_q, n_kv, d):
+    """All values 1: so is the output, whatever the probabilities are rounded to, as long as the sum that they are
+    divided by is that of the rounded ones (half a step of bf16 below 1 is 2^-9).  The probabilities are 1 and, 63 times as
+    often, 0.5 + 0.98 * 2^-9, which bf16 rounds to 0.5."""
+    shared, s_max = 1280, 1290
+    k = torch.zeros(b, n_kv, s_max, d, dtype=BF, device=DEV)
+    k[..., 0], k[..., 1] = -0.6875, -0.46875               # exact in e4m3 too
+    k[:, :, ::64] = 0.0
+    v = torch.ones(b, n_kv, s_max, d, dtype=BF, device=DEV)
+    q = torch.zeros(b, n_q, d, dtype=BF, device=DEV)
+    q[..., 0], q[..., 1] = 1.0, 2.0 ** -8
+    assert abs(math.exp(-0.6875 - 0.46875 / 256) - (0.5 + 0.98 * 2.0 ** -9)) < 2.0 ** -14
+    got, _, _ = _attend(kind, q, k, v, [s_max - i % 3 for i in range(b)], shared, scale=1.0)
+    assert bool((got == 1.0).all())
