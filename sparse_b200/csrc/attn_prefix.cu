@@ -60,7 +60,12 @@ struct Layout {
   static constexpr int kRaw = FP8 ? (TWO && DK > 64 ? 2 : 4) : 0;
   static constexpr uint32_t kRawK = kBlock * DK, kRawV = kBlock * DV;
   static constexpr uint32_t kBytes = kAllQ + kStages * (kK + kV) + kRaw * (kRawK + kRawV);
-  static constexpr uint32_t kSmem = kBytes + 1024 + 384;
+  // One CTA per SM, whatever its registers are: a CTA takes all of the tensor memory, ahead of its wait for the
+  // launches before it.  With room for two, one that started early could hold what one of an earlier launch,
+  // which it waits for, still has to get.
+  static constexpr uint32_t kAlone = 117 * 1024;
+  static constexpr uint32_t kSmem = kBytes + 1024 + 384 > kAlone ? kBytes + 1024 + 384 : kAlone;
+  static_assert(2 * (kSmem + 1024) > 228 * 1024, "room for one CTA only");
   static constexpr int kThreads = FP8 ? 640 : 384;
   static_assert(kSmem <= 232448, "shared memory of a CTA");
   static_assert(!TWO || DK <= 128, "two row tiles of wider heads leave no room for the keys");
