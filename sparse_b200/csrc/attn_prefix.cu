@@ -60,9 +60,8 @@ struct Layout {
   static constexpr int kRaw = FP8 ? (TWO && DK > 64 ? 2 : 4) : 0;
   static constexpr uint32_t kRawK = kBlock * DK, kRawV = kBlock * DV;
   static constexpr uint32_t kBytes = kAllQ + kStages * (kK + kV) + kRaw * (kRawK + kRawV);
-  // One CTA per SM, whatever its registers are: a CTA takes all of the tensor memory, ahead of its wait for the
-  // launches before it.  With room for two, one that started early could hold what one of an earlier launch,
-  // which it waits for, still has to get.
+  // One CTA per SM, whatever its registers are: a CTA takes all of the tensor memory, and a second one on the SM
+  // would stand there until the first is through.
   static constexpr uint32_t kAlone = 117 * 1024;
   static constexpr uint32_t kSmem = kBytes + 1024 + 384 > kAlone ? kBytes + 1024 + 384 : kAlone;
   static_assert(2 * (kSmem + 1024) > 228 * 1024, "room for one CTA only");
@@ -386,12 +385,14 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  pdl_launch_dependents();
+  pdl_wait();
+  // (behind the wait: a CTA that started early would hold the tensor memory that one of a launch before this
+  // one, a library's too, may still have to get; 0.1 us of the calls that are measured)
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_launch_dependents();
-  pdl_wait();
   // Loads of a tile of bf16 keys or values; positions behind the last shared one lie outside the
   // tensor map: zeros.
   const auto load_keys = [&](int i) {

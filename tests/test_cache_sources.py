@@ -28,3 +28,10 @@ def test_a_wait_that_gives_up_leaves_no_result_as_it_was():
     # (no condition of its own in front of it but the status word's, which ends with its statement)
     before = _block(kernel, at)[:marks.start()]
     assert before.count("if (") == 1 and before.count("{") == 0
+
+
+def test_tensor_memory_is_taken_behind_the_wait_for_the_launches_before():
+    """A CTA that started early and holds tensor memory could keep it from one that it waits for."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, "attn_prefix.cu")).read())
+    kernel = _block(text, text.index("attn_prefix_kernel(const __grid_constant__"))
+    assert kernel.count("tcgen05.alloc") == 1 and kernel.index("pdl_wait();") < kernel.index("tcgen05.alloc")
