@@ -621,45 +621,49 @@ int32_t sb_attn_decode(const void *q, int32_t q_stride, const void *cache_k, con
  * prefix that the whole batch shares.  (No counterpart in the reference: its cache is
  * the Transformers one, in the model dtype, one copy of every position per sequence.)
  *
- * Quantised cache: codes_k [B,n_kv,s_max,dk] and codes_v [B,n_kv,s_max,dv] e4m3 bytes,
- * scale_k / scale_v [B,n_kv,s_max] bytes.  A row (one sequence, head and position) stands
- * for code * 2^(scale - 127), scale byte 255 for NaN throughout; the writer takes the least
- * power of two, 2^-127 or more, by which the row's largest magnitude is at most 448 (codes
- * then stop at 240 where 256 would stand for 2^128), and byte 255 with zero codes for a row that
- * holds an infinity or a NaN.  The writer makes no codes 0x7f and 0xff, e4m3's own NaN (the scale byte
- * says it for the row); in a cache that was filled in some other way they are NaN to every call that
- * reads them.  All codes and bf16 caches must be 16-byte aligned.  A call's operands come as a struct (host memory, not kept); these calls are a decode step's, and a
- * binding fills one block of bytes faster than it converts twenty arguments.
+ * Quantised cache: codes_k [B,n_kv,s_max,dk] and codes_v [B,n_kv,s_max,dv] e4m3 bytes, scale_k
+ * / scale_v [B,n_kv,s_max] bytes.  A row (one sequence, head and position) stands for code *
+ * 2^(scale - 127), scale byte 255 for NaN throughout; the writer takes the least power of two,
+ * 2^-127 or more, by which the row's largest magnitude is at most 448 (codes then stop at 240
+ * where 256 would stand for 2^128), and byte 255 with zero codes for a row that holds an
+ * infinity or a NaN. The writer makes no codes 0x7f and 0xff, e4m3's own NaN (the scale byte
+ * says it for the row); in a cache that was filled in some other way they are NaN to every call
+ * that reads them.  All codes and bf16 caches must be 16-byte aligned.  A call's operands come as
+ * a struct (host memory, not kept); these calls are a decode step's, and a binding fills one
+ * block of bytes faster than it converts twenty arguments.
  *
- * sb_rope_append_fp8  rotates the first rope_dim elements of every q and k head (pairs
- *                  (i, i + rope_dim/2), angle pos * base^(-2i/rope_dim),
- *                  base = theta + theta_rest), stores q to q_out [T,n_q,dk] bf16 (q itself is not
- *                  written) and quantises k and v into row (seq_of_token[t], pos_of_token[t]).
- *                  Angles, products and the
- *                  scaled row are fp32, a value is rounded once; cosines and sines are
- *                  those of the 64-bit formula within 2^-23, from position 2^24 on 2^-14.  A key
- *                  head's first rope_dim elements come from k_rot and the others from k_rest
- *                  (NULL where there are none).  stride: elements between tokens and between
- *                  heads of each; a head stride of 0 shares one row between the heads.  A
- *                  token whose sequence is outside [0,B) or whose position is outside
- *                  [0,s_max) stores nothing but its q; two tokens of one call must not name
- *                  the same row.  dk, dv: multiples of 16 up to 256, rope_dim a multiple of
- *                  16 up to dk.
+ * sb_rope_append_fp8  rotates the first rope_dim elements of every q and k head (pairs (i, i +
+ *                  rope_dim/2), angle pos * base^(-2i/rope_dim), base = theta + theta_rest),
+ *                  stores q to q_out [T,n_q,dk] bf16 (q itself is not written) and quantises k
+ *                  and v into row (seq_of_token[t], pos_of_token[t]).  Angles, products and the
+ *                  scaled row are fp32, a value is rounded once; cosines and sines are those of
+ *                  the 64-bit formula within 2^-23, from position 2^24 on 2^-14.  A key head's
+ *                  first rope_dim elements come from k_rot and the others from k_rest (NULL
+ *                  where there are none). stride: elements between tokens and between heads of
+ *                  each; a head stride of 0 shares one row between the heads.  A token whose
+ *                  sequence is outside [0,B) or whose position is outside [0,s_max) stores
+ *                  nothing but its q; two tokens of one call must not name the same row. dk,
+ *                  dv: multiples of 16 up to 256, rope_dim a multiple of 16 up to dk.
  * sb_cache_read_fp8   positions begin .. begin+count-1 of every sequence as bf16, out_k
  *                  [B,n_kv,count,dk], out_v [B,n_kv,count,dv]; exact (a code has four
- *                  significant bits).  Positions below shared_len come from sequence 0.
+ *                  significant bits) but for what lies under bf16's smallest step, 2^-133.
+ *                  Positions below shared_len come from sequence 0.
  * sb_attn_decode_fp8  one query per sequence, q [B,n_q,dk] bf16 (q_stride elements between
  *                  sequences, 0 = packed), against the first seq_lens[b] (device int32)
  *                  positions of its quantised cache; softmax in fp32; out [B,n_q,dv] bf16,
- *                  zeros for a sequence without positions.  Query head h reads key head
- *                  h / (n_q / n_kv).  With shared_len > 0 positions below it are read from
- *                  sequence 0's rows, once for all sequences that reach over them.
- *                  scale >= 0.  Weights of up to 2^8 times values are summed in fp32 before
- *                  the division by the weights' sum: values beyond 2^100 may overflow.  ws:
- *                  sb_attn_cached_workspace_bytes(), 16-byte aligned, not shared by calls
- *                  that may overlap on the GPU.  status: device int32 (may be NULL), set
- *                  non-zero if a bounded wait gave up; the outputs that depend on what was waited
- *                  for are then NaN.  (dk,dv) = (128,128), (192,128), (64,64).
+ *                  zeros for a sequence without positions.  Query head h reads key head h / (n_q
+ *                  / n_kv).  With shared_len > 0 positions below it are read from sequence 0's
+ *                  rows, once for all sequences that reach over them. scale >= 0.  Weights of up
+ *                  to 2^8 times values are summed in fp32 before the division by the weights'
+ *                  sum, and scores before the query's power of two: values or keys beyond 2^100
+ *                  may overflow.  Probabilities are rounded before they meet the values, to bf16
+ *                  (2^-8; a shared prefix on the tensor cores, a bf16 cache) or with the
+ *                  value's power of two to fp16 (2^-11; quantised).  More than 16 query heads of
+ *                  a key head read its cache once per 16. ws: sb_attn_cached_workspace_bytes(),
+ *                  16-byte aligned, not shared by calls that may overlap on the GPU. status:
+ *                  device int32 (may be NULL), set non-zero if a bounded wait gave up; the
+ *                  outputs that depend on what was waited for are then NaN. (dk,dv) =
+ *                  (128,128), (192,128), (64,64).
  * sb_attn_decode_shared  the same over a bf16 cache, k [B,s_max,n_kv,dk] and v [B,s_max,n_kv,dv].
  */
 typedef struct sb_rope_append {

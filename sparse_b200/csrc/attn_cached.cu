@@ -3,17 +3,19 @@
 // rows only.  out[b, h] = sum_j p_j v_j,  p = softmax_j(scale * q[b, h] . k_j), over the
 // positions j < seq_lens[b]; a sequence without positions gives zeros.
 //
-// Bound by the bytes of the cache, each of which should be read once: the query heads that
-// share a key head (and, over the shared positions, the sequences) are rows of one small
-// matrix product.  attn_stream_kernel turns it round, S^T = K Q^T and O^T = V^T P^T, so
-// that the keys fill the 16-row side of the warp-level MMA and up to eight query rows its
-// 8-column side.  Keys and values then go from global memory straight into the fragments of
-// the instruction (which positions of a row a lane holds is free, as long as both operands
-// agree), without shared memory: what counts is bytes in flight, and each warp has the keys
-// and values of its next step (16 positions of bf16, 32 quantised: 8 KB) on the way while it
-// works on the present ones.  The tensor core's own rate is no concern here (13 % busy), which
-// is why the warp-level instruction does: an accumulator in tensor memory would need the keys
-// in shared memory first.
+// Bound by the bytes of the cache, each of which should be read once: up to sixteen query heads
+// that share a key head (and, over the shared positions, the sequences) are rows of one small
+// matrix product.  More query heads than that are row tiles of sixteen, and each asks for the keys
+// and values again (20 heads over one key head, 64 sequences of up to 16384 positions: 67 us for a
+// cache of 136 MB, of which DRAM gives 179 MB and L2 the rest of twice 136). attn_stream_kernel
+// turns it round, S^T = K Q^T and O^T = V^T P^T, so that the keys fill the 16-row side of the
+// warp-level MMA and up to eight query rows its 8-column side.  Keys and values then go from global
+// memory straight into the fragments of the instruction (which positions of a row a lane holds is
+// free, as long as both operands agree), without shared memory: what counts is bytes in flight, and
+// each warp has the keys and values of its next step (16 positions of bf16, 32 quantised: 8 KB) on
+// the way while it works on the present ones.  The tensor core's own rate is no concern here (13 %
+// busy), which is why the warp-level instruction does: an accumulator in tensor memory would need
+// the keys in shared memory first.
 //
 // The work, all tiles (64 positions of bf16, 128 quantised) of all sequences and heads in one
 // line, is cut into equal runs, one per CTA, whatever the lengths are; a head that ends in the
@@ -21,12 +23,14 @@
 // attn_join_kernel joins those.
 //
 // Measured (repeated in a graph, inputs larger than L2 in turn): 64 sequences of 0 to 16384
-// quantised positions, 32 query and 8 key heads of 128: 171 us, 6.3 TB/s; 8 x 2048, 16 heads: 20 us
-// for 68 MB, of which 2 to 4 us pass before the first keys are there (the lengths come first), CTAs end
-// between 9 and 15 us, and the second kernel takes 3.5 us; one sequence of
-// 1000: 7.2 us, all of it round trips.  A join inside this kernel (marks in memory, the last CTA
-// joins) has one launch less but five round trips to L2 behind one another instead of three:
-// 9.6 us for the sequence of 1000, 23.7 us for 8 x 2048.
+// quantised positions, 32 query and 8 key heads of 128: 171 us, 6.3 TB/s, in the first ten
+// milliseconds of a loop and 189 us, 5.7 TB/s, when it goes on; 8 x 2048, 16 heads: 20 us for 68
+// MB, of which 3 to 4.5 us pass before the first scores (1 us to read the lengths and find the run,
+// a load from DRAM), a tile takes 1.3 us, the end of a piece 1.2 us, so that CTAs of four tiles are
+// through at 10.5 to 13 us, those of five at 12.5 to 14.5, those of five in two pieces at 14 to 16,
+// and the second kernel is at 19; one sequence of 1000: 7.2 us, all of it round trips.  A join
+// inside this kernel (marks in memory, the last CTA joins) has one launch less but five round trips
+// to L2 behind one another instead of three: 9.6 us for the sequence of 1000, 23.7 us for 8 x 2048.
 #include <math.h>
 
 #include <type_traits>
@@ -734,7 +738,7 @@ int64_t slot_rows(const Shape &s) { return (kMaxCtas + segments(s)) * s.rows; }
 int64_t pre_slot_rows(const Shape &s) { return s.pre_splits > 0 ? prefix_slots(s) * s.pre_rows : 0; }
 
 // A dependent launch of the stream kernel that asks for 100 of the SM's 228 KB as shared memory, which
-// two or three of its CTAs take (85 KB at most).  Its loads in flight live in what is left as L1:
+// two or three of its CTAs take (two of 44.25 KB and 1 KB for the system each at most).  Its loads in flight live in what is left as L1:
 // behind a kernel that used all of the shared memory the SM would stay as it is otherwise, and 64
 // sequences of up to 16384 positions take 249 us with all of it against 171 with 66 to 148 KB.
 template <typename... KArgs, typename... Args>

@@ -8,11 +8,12 @@
 // exponentials 1 K).  For 256 rows by the products: 128 positions take 3.6 K clocks, of which the 48
 // products issued for them take 3.1 K (one of 64 score columns takes as long as one of 128, but
 // leaves room in TMEM for a second score buffer, without which the products wait for the
-// exponentials: 52 instead of 50 us).  With codes and few rows by the conversion, 2.7 K clocks.  One CTA
-// per SM; the positions are cut into as many runs as fill the machine.
+// exponentials: 52 instead of 50 us).  With codes and few rows by the conversion, some 2.9 K clocks.  One CTA
+// per SM.  The positions are cut into 148 / (key heads x row tiles) runs, rounded down, at least one:
+// between 75 and 147 such pairs the other SMs have nothing to do.
 //
-// Measured (alone, ncu): 8192 positions of a bf16 cache of 16 heads for 32 sequences 19 us
-// (67 MB, 3.5 TB/s); 16384 quantised positions of 4 heads for 512 rows each 32 us (17 GFLOP, 0.54
+// Measured (alone, cold, ncu): 8192 positions of a bf16 cache of 16 heads for 32 sequences 20.4 us
+// (67 MB, 3.3 TB/s); 16384 quantised positions of 4 heads for 512 rows each 33.6 us (17 GFLOP, 0.51
 // PF/s; 34 M exponentials).
 //
 // Roles: warp 0 loads tiles of 128 keys and values (TMA: bf16 boxes into the swizzled operand
@@ -24,8 +25,9 @@
 // groups exchange nothing until the end, and a block's products run under the exponentials of
 // the block before it.  Probabilities go back into TMEM (bf16, over their scores), where the
 // second product takes its left operand from.  Quantised: four warps turn the keys' codes into
-// bf16 operands and four the values', scale applied (exact), so the products
-// are the bf16 ones.  (The fp8 products would round the queries and probabilities to codes.)
+// bf16 operands and four the values', scale applied (as exact as reading the row back
+// is, kv_fp8.cuh), so the products are the bf16 ones.  (The fp8 products would round the queries and
+// probabilities to codes.)
 //
 // Probabilities are rounded to bf16 (2^-8), the type of the values that they are multiplied
 // with, and their sum is taken over the rounded ones; scores, sums and accumulators are fp32.  Against
@@ -133,7 +135,7 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
   return (uint32_t)(chunk >> 3) * kBox + (uint32_t)row * 128 + (uint32_t)(((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// Codes -> bf16 operands, exact.  An e4m3 byte s eeee mmm put at bit 4 of a bf16 (s 0000eeee mmm0000) is
+// Codes -> bf16 operands.  An e4m3 byte s eeee mmm put at bit 4 of a bf16 (s 0000eeee mmm0000) is
 // the code's value times 2^-120 (subnormal codes included: both types have the same step there), so
 // one packed multiplication by 2^(e + 120) makes two operands; powers above bf16's largest, 2^127,
 // in two steps.

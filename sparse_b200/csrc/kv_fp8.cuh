@@ -5,7 +5,9 @@
 // max|row| <= 448 * 2^e (448 = largest e4m3 value), kept as one byte e + 127 (E8M0).
 // A power of two because scaling by it is exact: a value is rounded once, when its
 // code is made, and code * 2^e has at most four significant bits, so reading the row
-// back as bf16 rounds nothing and every reader sees the same numbers.  A free fp32
+// back as bf16 rounds nothing and every reader sees the same numbers.  (Where bf16 has them: with e
+// of -125 to -127 the smallest codes stand for less than its smallest step, 2^-133, and are rounded to it, and
+// a code of 256 or more under 2^120, which the writer does not make, is infinite.)  A free fp32
 // scale would use the last half binade below 448 too, but e4m3 is a floating type:
 // its relative step is the same there, only values 2^-15 below the largest gain.
 // (A row with values above 1.9375 * 2^127 stops at code 240: 256 would stand for 2^128.)

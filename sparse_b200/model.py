@@ -306,7 +306,9 @@ class ShapedMoeModel:
 
         shared_len < S: as many first ids are the same in every row.  They are computed for
         sequence 0 and stored in its rows of the cache only; until the next `prefill` the decode
-        steps read them there, once for the whole batch."""
+        steps read them there, once for the whole batch.  (The room for them in the other sequences' rows
+        stays empty.  Over a bf16 cache the steps' attention is then the one that rounds probabilities to bf16,
+        `ops.attn_decode_shared`.)"""
         b, s = input_ids.shape
         if b != self.batch or s >= self.max_seq:
             raise RuntimeError("model was built for batch %d and fewer than %d positions" % (self.batch, self.max_seq))

@@ -291,8 +291,8 @@ def rope_append_quantized(q: torch.Tensor, k_rot: Optional[torch.Tensor], k_rest
 
 def cache_read(cache: QuantizedCache, begin: int, count: int, shared_len: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
     """Positions begin .. begin+count-1 of every sequence as bf16: (k [B, n_kv, count, dk],
-    v [B, n_kv, count, dv]), exactly the values the codes stand for.  Positions below
-    `shared_len` are sequence 0's."""
+    v [B, n_kv, count, dv]), exactly the values the codes stand for (but for those under bf16's
+    smallest step, 2^-133).  Positions below `shared_len` are sequence 0's."""
     device = _cache_device(cache)
     b, n_kv, s_max, dk = cache.k.shape
     dv = cache.v.shape[3]
@@ -355,7 +355,8 @@ def attn_decode_shared(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Te
                        status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`attn_decode_quantized` over a bf16 cache, cache_k [B, S, n_kv, dk] and cache_v
     [B, S, n_kv, dv]: the first `shared_len` positions of the batch stand in sequence 0's
-    rows and are read once for all sequences."""
+    rows and are read once for all sequences.  Probabilities are rounded to bf16 before they are multiplied
+    with values (`sb_attn_decode`, which the model uses where nothing is shared, keeps them in fp32)."""
     if cache_k.dim() != 4 or cache_v.dim() != 4 or cache_k.shape[:3] != cache_v.shape[:3]:
         raise RuntimeError("attn_decode_shared: caches [B, S, n_kv, d] do not fit: %s and %s" % (
             tuple(cache_k.shape), tuple(cache_v.shape)))
