@@ -195,3 +195,33 @@ def test_the_mean_of_equal_values_is_their_value(kind, b, n_q, n_kv, d):
     assert abs(math.exp(-0.6875 - 0.46875 / 256) - (0.5 + 0.98 * 2.0 ** -9)) < 2.0 ** -14
     got, _, _ = _attend(kind, q, k, v, [s_max - i % 3 for i in range(b)], shared, scale=1.0)
     assert bool((got == 1.0).all())
+
+
+# -- several at once -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,b,n_q,n_kv,d,shared", [("fp8", 60, 8, 2, 64, 2000), ("bf16", 90, 4, 2, 64, 2000), ("fp8", 80, 16, 8, 128, 1500),
+                                                      ("bf16", 40, 16, 16, 128, 1500)])
+def test_calls_with_a_shared_prefix_on_their_own_streams(kind, b, n_q, n_kv, d, shared):
+    """Launches of four streams run beside one another, those of a stream as close behind one another as they may: each
+    CTA of the tensor-core pass finds its tensor memory, and every call gives the bits of a call alone."""
+    s_max = shared + 40
+    k, v = _rand(b, n_kv, s_max, d, seed=2), _rand(b, n_kv, s_max, d, seed=3)
+    lens = torch.tensor([shared + i % 41 for i in range(b)], dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cache = QuantizedCache(*_quantized(k), *_quantized(v))
+    ck, cv = k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
+
+    def call(q):
+        if kind == "fp8":
+            return ops.attn_decode_quantized(q, cache, lens, shared, status=status)
+        return ops.attn_decode_shared(q, ck, cv, lens, shared, status=status)
+
+    qs = [_rand(b, n_q, d, seed=i) for i in range(4)]
+    want = [call(q) for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in qs], []
+    for _ in range(25):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append((i, call(qs[i])))
+    torch.cuda.synchronize()
+    assert int(status) == 0 and all(torch.equal(out, want[i]) for i, out in got)
